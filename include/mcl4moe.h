@@ -538,6 +538,123 @@ int mcl4moe_copy_async(void* dst, const void* src, size_t bytes, mcl4moe_stream_
 int mcl4moe_copy_list_async(void* const* dst, const void* const* src, const uint64_t* bytes, int n,
                             mcl4moe_stream_t const* streams, int n_streams);
 
+/* ------------------------------------------------------------------------
+ * Routing from scores (beside mcl4moe_route, which serves the reference's plain
+ * softmax top-k): scores s = softmax (score 0) or sigmoid (score 1) of logits
+ * [T, E] (dtype 0 bf16, 1 fp32, 2 fp16; row stride ld elements), keys s + bias
+ * (bias fp32 [E] or NULL; it selects only), and, with groups > 1, only the
+ * top_groups groups (of E / groups consecutive experts) of the largest value: the
+ * sum of the two best keys (group_score 0) or the best key (1).  topk_idx int32
+ * [T, k]: the k best keys in falling order, ties to the lower id; an expert whose
+ * logit or bias is -inf is never chosen, slots without an expert are -1 with
+ * weight 0, and so are the rows where valid (uint8 [T] or NULL) is 0.  topk_w
+ * fp32 [T, k] = scale * s / (sum of the chosen s when renorm).  counts (int32 [E]
+ * or NULL): slots of each expert.  E <= 512, k <= 32.
+ * _backward: d_logits [T, E] (dtype of the logits, contiguous) for d_w fp32 [T, k].
+ * ------------------------------------------------------------------------ */
+int mcl4moe_route_scores(const void* logits, int dtype, int64_t ld, const float* bias, const uint8_t* valid, int64_t T,
+                         int E, int k, int score, int groups, int top_groups, int group_score, int renorm, float scale,
+                         int32_t* topk_idx, float* topk_w, int32_t* counts, mcl4moe_stream_t stream);
+int mcl4moe_route_scores_backward(const void* logits, int dtype, int64_t ld, const int32_t* topk_idx, const float* d_w,
+                                  int64_t T, int E, int k, int score, int renorm, float scale, void* d_logits,
+                                  mcl4moe_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * The norms around a block with its gate and residual sum (the layer's
+ * x + moe(moe_norm(x)), src/mcl4_coe/backbone.py:1269, RMSNorm
+ * src/mcl4_coe/ple.py:17):
+ *   n = branch * rsqrt(mean(branch^2) + eps) * post_weight   (n = branch without it)
+ *   y = residual_scale * x + branch_scale * act(gate) * n    -> stream_out
+ *   h = y * rsqrt(mean(y^2) + eps) * pre_weight              -> norm_out
+ * without a branch y = x and only h is computed.  dtypes as above; weights fp32
+ * [cols]; stream_out has x's type; all outputs are contiguous.  gate_mode 0: none,
+ * 1: [rows / gate_rows, cols], each row of it for gate_rows rows, 2: [rows],
+ * 3: [rows, cols] with row stride ld_gate.  gate_act 0: none, 1: sigmoid, 2: tanh.
+ * _backward: d_stream / d_normed are the gradients of y and h (either may be
+ * NULL: zero); outputs that are NULL are not computed; d_pre, d_post and the
+ * gate's gradient of modes 1 and 2 are fp32, that of mode 3 has the gate's type.
+ * The sums over rows are taken in a fixed order.  cols <= 16384.
+ * ------------------------------------------------------------------------ */
+typedef struct mcl4moe_norm_args {
+  int64_t rows;
+  int cols;
+  const void* x;
+  int64_t ld_x;
+  int x_dtype;
+  const void* branch;
+  int64_t ld_branch;
+  int branch_dtype;
+  const float* post_weight;
+  const float* pre_weight;
+  const void* gate;
+  int64_t ld_gate;
+  int64_t gate_rows;
+  int gate_dtype;
+  int gate_mode;
+  int gate_act;
+  int norm_dtype;
+  float residual_scale;
+  float branch_scale;
+  float eps;
+  void* stream_out;
+  void* norm_out;
+  /* backward */
+  const void* d_stream;
+  int64_t ld_d_stream;
+  const void* d_normed;
+  int64_t ld_d_normed;
+  void* d_x;
+  void* d_branch;
+  void* d_gate;
+  float* d_pre;
+  float* d_post;
+} mcl4moe_norm_args;
+
+int mcl4moe_residual_norm(const mcl4moe_norm_args* args, mcl4moe_stream_t stream);
+size_t mcl4moe_residual_norm_workspace_size(int64_t rows, int cols, int gate_mode, int64_t gate_rows);
+int mcl4moe_residual_norm_backward(const mcl4moe_norm_args* args, void* workspace, size_t workspace_bytes,
+                                   mcl4moe_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * One AdamW step over n tensors (host arrays of device pointers), in place:
+ *   g = grad * grad_scale;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
+ *   p = p (1 - lr wd) - lr / (1 - beta1^step) * m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
+ * param_dtype / grad_dtype 0 bf16, 1 fp32, 2 fp16.  masters (fp32 copies, NULL: none)
+ * take the update, the parameters their rounded values.  bits 32: fp32 states.
+ * bits 8: exp_avg e4m3fn and exp_avg_sq e5m2 codes with one fp32 power-of-two scale
+ * for each 256 elements of a tensor, rounded stochastically with Philox4x32-7 words
+ * keyed by seed, counted by (element / 4, tensor, step).  indices (NULL: 0 to n - 1):
+ * the tensors' numbers in that count.  step_dev (int64) and lr_dev (fp32), where not
+ * NULL, replace step and lr (a captured step); grad_scale: device fp32 or NULL.
+ * ------------------------------------------------------------------------ */
+typedef struct mcl4moe_adamw_args {
+  int n;
+  int param_dtype;
+  int grad_dtype;
+  int bits;
+  void* const* params;
+  const void* const* grads;
+  void* const* exp_avgs;
+  void* const* exp_avg_sqs;
+  float* const* exp_avg_scales;
+  float* const* exp_avg_sq_scales;
+  float* const* masters;
+  const int64_t* numels;
+  const int32_t* indices;
+  double lr;
+  double beta1;
+  double beta2;
+  double eps;
+  double weight_decay;
+  int64_t step;
+  const int64_t* step_dev;
+  const float* lr_dev;
+  const float* grad_scale;
+  uint64_t seed;
+} mcl4moe_adamw_args;
+
+int mcl4moe_adamw_step(const mcl4moe_adamw_args* args, mcl4moe_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

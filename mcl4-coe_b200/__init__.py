@@ -26,6 +26,9 @@ from .nvfp4 import (
     quantize_nvfp4,
     reset_gemm_counts,
 )
+from .optim import adamw_step
+from .norms import residual_norm
+from .routing import route_experts
 
 __all__ = [
     "CudaEPOps",
@@ -46,6 +49,9 @@ __all__ = [
     "convert_linear_to_nvfp4",
     "nvfp4_mm",
     "quantize_activations",
+    "adamw_step",
+    "residual_norm",
+    "route_experts",
 ]
 
 

@@ -9,7 +9,7 @@ else -> RuntimeError.
 from __future__ import annotations
 
 import ctypes
-from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_uint8, c_uint16, c_void_p
+from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_size_t, c_uint8, c_uint16, c_void_p
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libmcl4moe.so"
@@ -70,6 +70,12 @@ EXPORTS = (
     "mcl4moe_quantize_hadamard_t",
     "mcl4moe_nvfp4_linear_wgrad_workspace_size",
     "mcl4moe_nvfp4_linear_wgrad",
+    "mcl4moe_route_scores",
+    "mcl4moe_route_scores_backward",
+    "mcl4moe_residual_norm",
+    "mcl4moe_residual_norm_workspace_size",
+    "mcl4moe_residual_norm_backward",
+    "mcl4moe_adamw_step",
 )
 
 
@@ -124,6 +130,37 @@ class MoeBwdArgs(ctypes.Structure):
         ("seed_down", ctypes.c_uint64), ("seed_up", ctypes.c_uint64),
         ("d_y", c_void_p), ("d_up", c_void_p), ("d_rows", c_void_p), ("d_w", c_void_p),
         ("error_word", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+    ]
+
+
+class NormArgs(ctypes.Structure):
+    """Mirror of ``mcl4moe_norm_args``."""
+
+    _fields_ = [
+        ("rows", c_int64), ("cols", c_int),
+        ("x", c_void_p), ("ld_x", c_int64), ("x_dtype", c_int),
+        ("branch", c_void_p), ("ld_branch", c_int64), ("branch_dtype", c_int),
+        ("post_weight", c_void_p), ("pre_weight", c_void_p),
+        ("gate", c_void_p), ("ld_gate", c_int64), ("gate_rows", c_int64),
+        ("gate_dtype", c_int), ("gate_mode", c_int), ("gate_act", c_int), ("norm_dtype", c_int),
+        ("residual_scale", c_float), ("branch_scale", c_float), ("eps", c_float),
+        ("stream_out", c_void_p), ("norm_out", c_void_p),
+        ("d_stream", c_void_p), ("ld_d_stream", c_int64), ("d_normed", c_void_p), ("ld_d_normed", c_int64),
+        ("d_x", c_void_p), ("d_branch", c_void_p), ("d_gate", c_void_p), ("d_pre", c_void_p), ("d_post", c_void_p),
+    ]
+
+
+class AdamwArgs(ctypes.Structure):
+    """Mirror of ``mcl4moe_adamw_args`` (the lists are addresses of host arrays)."""
+
+    _fields_ = [
+        ("n", c_int), ("param_dtype", c_int), ("grad_dtype", c_int), ("bits", c_int),
+        ("params", c_void_p), ("grads", c_void_p), ("exp_avgs", c_void_p), ("exp_avg_sqs", c_void_p),
+        ("exp_avg_scales", c_void_p), ("exp_avg_sq_scales", c_void_p), ("masters", c_void_p),
+        ("numels", c_void_p), ("indices", c_void_p),
+        ("lr", c_double), ("beta1", c_double), ("beta2", c_double), ("eps", c_double), ("weight_decay", c_double),
+        ("step", c_int64), ("step_dev", c_void_p), ("lr_dev", c_void_p), ("grad_scale", c_void_p),
+        ("seed", ctypes.c_uint64),
     ]
 
 
@@ -276,6 +313,20 @@ def load() -> ctypes.CDLL:
     lib.mcl4moe_set_expert_tiling.argtypes = [c_int]
     lib.mcl4moe_moe_backward_dx.restype = c_int
     lib.mcl4moe_moe_backward_dx.argtypes = [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p]
+    lib.mcl4moe_route_scores.restype = c_int
+    lib.mcl4moe_route_scores.argtypes = [c_void_p, c_int, c_int64, c_void_p, c_void_p, c_int64, c_int, c_int, c_int,
+                                         c_int, c_int, c_int, c_int, c_float, c_void_p, c_void_p, c_void_p, c_void_p]
+    lib.mcl4moe_route_scores_backward.restype = c_int
+    lib.mcl4moe_route_scores_backward.argtypes = [c_void_p, c_int, c_int64, c_void_p, c_void_p, c_int64, c_int, c_int,
+                                                  c_int, c_int, c_float, c_void_p, c_void_p]
+    lib.mcl4moe_residual_norm.restype = c_int
+    lib.mcl4moe_residual_norm.argtypes = [POINTER(NormArgs), c_void_p]
+    lib.mcl4moe_residual_norm_workspace_size.restype = c_size_t
+    lib.mcl4moe_residual_norm_workspace_size.argtypes = [c_int64, c_int, c_int, c_int64]
+    lib.mcl4moe_residual_norm_backward.restype = c_int
+    lib.mcl4moe_residual_norm_backward.argtypes = [POINTER(NormArgs), c_void_p, c_size_t, c_void_p]
+    lib.mcl4moe_adamw_step.restype = c_int
+    lib.mcl4moe_adamw_step.argtypes = [POINTER(AdamwArgs), c_void_p]
     _lib = lib
     return lib
 
@@ -293,5 +344,5 @@ def check(status: int, what: str) -> None:
     raise RuntimeError(msg)
 
 
-__all__ = ["load", "check", "MoeArgs", "MoeBwdArgs", "EXPORTS", "LIB_PATH", "ExtensionMissing",
+__all__ = ["load", "check", "MoeArgs", "MoeBwdArgs", "NormArgs", "AdamwArgs", "EXPORTS", "LIB_PATH", "ExtensionMissing",
            "c_float", "c_uint8", "c_uint16"]

@@ -17,7 +17,7 @@ HERE = Path(__file__).resolve().parent
 CSRC = HERE / "csrc"
 LIB = HERE / "libmcl4moe.so"
 SOURCES = ["quant.cu", "router.cu", "route.cu", "gemm_fp4.cu", "api.cu", "noalloc.cu", "ep.cu", "peer.cu",
-           "backward.cu", "wgrad.cu", "linear_bwd.cu"]
+           "backward.cu", "wgrad.cu", "linear_bwd.cu", "scores.cu", "norm.cu", "adamw.cu"]
 HEADERS = ["common.cuh", "kernels.cuh", "sr.cuh"]
 
 NVCC_FLAGS = [
