@@ -570,8 +570,9 @@ int mcl4moe_route_scores_backward(const void* logits, int dtype, int64_t ld, con
  * [cols]; stream_out has x's type; all outputs are contiguous.  gate_mode 0: none,
  * 1: [rows / gate_rows, cols], each row of it for gate_rows rows, 2: [rows],
  * 3: [rows, cols] with row stride ld_gate.  gate_act 0: none, 1: sigmoid, 2: tanh.
- * _backward: d_stream / d_normed are the gradients of y and h (either may be
- * NULL: zero); outputs that are NULL are not computed; d_pre, d_post and the
+ * stats (fp32 [rows, 2] or NULL) receives the two reciprocal root mean squares.
+ * _backward reads stats (needed with post_weight or d_normed); d_stream / d_normed
+ * are the gradients of y and h (either may be NULL: zero); outputs that are NULL are not computed; d_pre, d_post and the
  * gate's gradient of modes 1 and 2 are fp32, that of mode 3 has the gate's type.
  * The sums over rows are taken in a fixed order.  cols <= 16384.
  * ------------------------------------------------------------------------ */
@@ -598,6 +599,7 @@ typedef struct mcl4moe_norm_args {
   float eps;
   void* stream_out;
   void* norm_out;
+  float* stats;
   /* backward */
   const void* d_stream;
   int64_t ld_d_stream;

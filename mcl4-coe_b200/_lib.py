@@ -144,7 +144,7 @@ class NormArgs(ctypes.Structure):
         ("gate", c_void_p), ("ld_gate", c_int64), ("gate_rows", c_int64),
         ("gate_dtype", c_int), ("gate_mode", c_int), ("gate_act", c_int), ("norm_dtype", c_int),
         ("residual_scale", c_float), ("branch_scale", c_float), ("eps", c_float),
-        ("stream_out", c_void_p), ("norm_out", c_void_p),
+        ("stream_out", c_void_p), ("norm_out", c_void_p), ("stats", c_void_p),
         ("d_stream", c_void_p), ("ld_d_stream", c_int64), ("d_normed", c_void_p), ("ld_d_normed", c_int64),
         ("d_x", c_void_p), ("d_branch", c_void_p), ("d_gate", c_void_p), ("d_pre", c_void_p), ("d_post", c_void_p),
     ]

@@ -58,24 +58,25 @@ def _fill(args, x, branch, post, pre, gate, mode, gate_rows, act, norm_dtype, sc
     return args
 
 
-def _norm_forward(x, branch, post, pre, gate, mode, gate_rows, act, norm_dtype, scales):
+def _norm_forward(x, branch, post, pre, gate, mode, gate_rows, act, norm_dtype, scales, stats=None):
     y = None if branch is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
     h = None if pre is None else torch.empty(x.shape, dtype=norm_dtype, device=x.device)
     if x.shape[0] == 0:
         return y, h
     args = _fill(_lib.NormArgs(), x, branch, post, pre, gate, mode, gate_rows, act, norm_dtype, scales)
-    args.stream_out, args.norm_out = _ptr(y), _ptr(h)
+    args.stream_out, args.norm_out, args.stats = _ptr(y), _ptr(h), _ptr(stats)
     _launch(x.device, "mcl4moe_residual_norm", _lib.load().mcl4moe_residual_norm, args)
     return y, h
 
 
 class _ResidualNorm(torch.autograd.Function):
-    """Saves the inputs alone: the backward computes the norms again from them."""
+    """Saves the inputs and the rows' two reciprocal root mean squares; the backward computes the rest again."""
 
     @staticmethod
     def forward(ctx, x, branch, post, pre, gate, mode, gate_rows, act, norm_dtype, scales):
-        y, h = _norm_forward(x, branch, post, pre, gate, mode, gate_rows, act, norm_dtype, scales)
-        ctx.save_for_backward(x, branch, post, pre, gate)
+        stats = torch.empty((x.shape[0], 2), dtype=torch.float32, device=x.device)
+        y, h = _norm_forward(x, branch, post, pre, gate, mode, gate_rows, act, norm_dtype, scales, stats)
+        ctx.save_for_backward(x, branch, post, pre, gate, stats)
         ctx.args = (mode, gate_rows, act, norm_dtype, scales)
         ctx.set_materialize_grads(False)
         return y, h
@@ -85,7 +86,7 @@ class _ResidualNorm(torch.autograd.Function):
     def backward(ctx, d_y, d_h):
         if d_y is None and d_h is None:
             return (None,) * 10
-        x, branch, post, pre, gate = ctx.saved_tensors
+        x, branch, post, pre, gate, stats = ctx.saved_tensors
         mode, gate_rows, act, norm_dtype, scales = ctx.args
         need = ctx.needs_input_grad
         if x.shape[0] == 0:
@@ -94,6 +95,7 @@ class _ResidualNorm(torch.autograd.Function):
         lib = _lib.load()
         dev = x.device
         args = _fill(_lib.NormArgs(), x, branch, post, pre, gate, mode, gate_rows, act, norm_dtype, scales)
+        args.stats = stats.data_ptr()
         if d_y is not None:
             d_y = _rows(d_y.to(x.dtype))
             args.d_stream, args.ld_d_stream = d_y.data_ptr(), _ld(d_y)
