@@ -12,8 +12,8 @@
 //
 // Both directions are bound by HBM (forward 2 reads and 2 writes of a row, backward 4 and 2), so a
 // row is read once: it stays in the registers of its team (a warp for up to 256 columns, else a
-// CTA, 8 or 16 columns a thread) between the reductions, and the next row's loads are issued
-// before them.  Teams are persistent, which keeps the columns' factors in registers and, in the
+// CTA, 8 or 16 columns a thread) between the reductions, and the next rows are under way to shared
+// memory meanwhile.  Teams are persistent, which keeps the columns' factors in registers and, in the
 // backward, the column sums: a row of partial sums per team, added afterwards in their order.
 // With one gate row per part of the rows, dw_post and dg both come from one column sum
 //   S = sum over rows of dz uh:  dw_post = bs act(g) S,  dg = bs act'(g) w_post S.
@@ -68,40 +68,87 @@ struct __align__(16) Pack8 {
   T v[8];
 };
 
+// Eight float32 as four pairs: one instruction for two products or sums.
+struct V8 {
+  uint64_t p[4];
+  __device__ __forceinline__ float get(int i) const {
+    float a, b;
+    f2unpack(p[i >> 1], a, b);
+    return i & 1 ? b : a;
+  }
+  __device__ __forceinline__ void fill(float v) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] = f2pack(v, v);
+  }
+};
+__device__ __forceinline__ uint64_t ffma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ V8 mul(const V8& a, const V8& b) {
+  V8 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r.p[i] = fmul2(a.p[i], b.p[i]);
+  return r;
+}
+__device__ __forceinline__ V8 mul(const V8& a, float s) {
+  V8 r;
+  const uint64_t ss = f2pack(s, s);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r.p[i] = fmul2(a.p[i], ss);
+  return r;
+}
+__device__ __forceinline__ V8 fma(const V8& a, const V8& b, const V8& c) {
+  V8 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r.p[i] = ffma2(a.p[i], b.p[i], c.p[i]);
+  return r;
+}
+__device__ __forceinline__ V8 fma(const V8& a, float s, const V8& c) {
+  V8 r;
+  const uint64_t ss = f2pack(s, s);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r.p[i] = ffma2(a.p[i], ss, c.p[i]);
+  return r;
+}
+__device__ __forceinline__ float total(const V8& a) {
+  float x, y;
+  f2unpack(fadd2(fadd2(a.p[0], a.p[1]), fadd2(a.p[2], a.p[3])), x, y);
+  return x + y;
+}
+
 template <bool VEC>
 __device__ __forceinline__ int col_of(int chunk, int i, int tid, int team) {
   return VEC ? (chunk * team + tid) * 8 + i : (chunk * 8 + i) * team + tid;
 }
 
-template <typename T, bool VEC>
-__device__ __forceinline__ void load8(Pack8<T>& d, const T* row, int chunk, int tid, int team, int cols) {
-  if (VEC) {
-    const int c = (chunk * team + tid) * 8;
-    uint4* w = reinterpret_cast<uint4*>(&d);
-    if (c < cols) {
-      const uint4* src = reinterpret_cast<const uint4*>(row + c);
+template <typename T>
+__device__ __forceinline__ V8 unpack8(const Pack8<T>& d) {
+  V8 r;
 #pragma unroll
-      for (int i = 0; i < int(sizeof(T)) / 2; ++i) w[i] = __ldg(src + i);
-    } else {
+  for (int i = 0; i < 4; ++i) r.p[i] = f2pack(elem_f(d.v[2 * i]), elem_f(d.v[2 * i + 1]));
+  return r;
+}
+
+template <typename T>
+__device__ __forceinline__ V8 load8(const T* row, int chunk, int tid, int team, int cols) {
+  Pack8<T> d;
 #pragma unroll
-      for (int i = 0; i < int(sizeof(T)) / 2; ++i) w[i] = make_uint4(0u, 0u, 0u, 0u);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int c = col_of<false>(chunk, i, tid, team);
-      d.v[i] = c < cols ? __ldg(row + c) : T(0.f);
-    }
+  for (int i = 0; i < 8; ++i) {
+    const int c = col_of<false>(chunk, i, tid, team);
+    d.v[i] = c < cols ? __ldg(row + c) : T(0.f);
   }
+  return unpack8(d);
 }
 template <typename T, bool VEC>
-__device__ __forceinline__ void store8(T* row, const float (&v)[8], int chunk, int tid, int team, int cols) {
+__device__ __forceinline__ void store8(T* row, const V8& v, int chunk, int tid, int team, int cols) {
   if (VEC) {
     const int c = (chunk * team + tid) * 8;
     if (c >= cols) return;
     Pack8<T> p;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) elem_set(p.v[i], v[i]);
+    for (int i = 0; i < 8; ++i) elem_set(p.v[i], v.get(i));
     uint4* dst = reinterpret_cast<uint4*>(row + c);
     const uint4* w = reinterpret_cast<const uint4*>(&p);
 #pragma unroll
@@ -110,52 +157,112 @@ __device__ __forceinline__ void store8(T* row, const float (&v)[8], int chunk, i
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int c = col_of<false>(chunk, i, tid, team);
-      if (c < cols) elem_set(row[c], v[i]);
+      if (c < cols) elem_set(row[c], v.get(i));
     }
   }
 }
 
+// The rows ahead of a thread, in shared memory: it copies its own elements there (cp.async, 16
+// bytes each) `depth` rows ahead and reads them back itself, so that no barrier stands between and
+// the loads in flight need no registers.  Slots of a row: up to five operands of NCH chunks.
+// Without VEC the elements come straight from memory when they are asked for.
+template <int NCH, bool VEC>
+struct Ahead {
+  char* mine;       // this thread's first 16 bytes
+  uint32_t stride;  // bytes between the 16-byte pieces of a thread
+  uint32_t stage;   // bytes of a row
+  int depth, slot;
+  template <typename T>
+  __device__ __forceinline__ void fetch(const T* row, uint32_t at, int s, int tid, int team, int cols) const {
+    if constexpr (VEC) {
+#pragma unroll
+      for (int j = 0; j < NCH; ++j) {
+        const int c = (j * team + tid) * 8;
+        if (c >= cols) continue;
+#pragma unroll
+        for (int i = 0; i < int(sizeof(T)) / 2; ++i) {
+          const uint32_t dst = uint32_t(__cvta_generic_to_shared(mine + s * stage + (at + j * (sizeof(T) / 2) + i) * stride));
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(row + c + i * (16 / sizeof(T)))
+                       : "memory");
+        }
+      }
+    }
+  }
+  template <typename T>
+  __device__ __forceinline__ V8 take(const T* row, uint32_t at, int j, int tid, int team, int cols) const {
+    if constexpr (!VEC) {
+      return load8(row, j, tid, team, cols);
+    } else {
+      Pack8<T> d;
+      uint4* w = reinterpret_cast<uint4*>(&d);
+      const bool in = (j * team + tid) * 8 < cols;
+#pragma unroll
+      for (int i = 0; i < int(sizeof(T)) / 2; ++i)
+        w[i] = in ? *reinterpret_cast<const uint4*>(mine + slot * stage + (at + j * (sizeof(T) / 2) + i) * stride)
+                  : make_uint4(0u, 0u, 0u, 0u);
+      return unpack8(d);
+    }
+  }
+  __device__ __forceinline__ void commit() const {
+    if (VEC) asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  // The oldest of `depth` committed rows is there.
+  __device__ __forceinline__ void wait() const {
+    if (!VEC) return;
+    if (depth >= 4) asm volatile("cp.async.wait_group 3;" ::: "memory");
+    else if (depth == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
+    else if (depth == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
+    else asm volatile("cp.async.wait_group 0;" ::: "memory");
+  }
+  __device__ __forceinline__ void next() { slot = slot + 1 == depth ? 0 : slot + 1; }
+};
+
 // Sums over the team, the same order every time; every thread gets them.  One barrier per call:
 // three buffers in turn, so that a buffer is written again only behind the barrier after its reads.
 struct TeamSum {
-  float2* buf;  // [3][32] shared, or unused by a one-warp team
-  int turn;
-  __device__ __forceinline__ float2 operator()(float a, float b) {
+  float* buf;  // [3][2][32] shared, or null for a one-warp team
+  int warps, turn;
+  __device__ __forceinline__ float across(const float* t) const {
+    float s = 0.f;
+#pragma unroll 4
+    for (int w = 0; w < warps; ++w) s += t[w];
+    return s;
+  }
+  __device__ __forceinline__ float one(float a) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+    if (buf == nullptr) return a;
+    float* t = buf + turn * 64;
+    turn = turn == 2 ? 0 : turn + 1;
+    if ((threadIdx.x & 31) == 0) t[threadIdx.x >> 5] = a;
+    __syncthreads();
+    return across(t);
+  }
+  __device__ __forceinline__ float2 two(float a, float b) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       a += __shfl_xor_sync(0xffffffffu, a, o);
       b += __shfl_xor_sync(0xffffffffu, b, o);
     }
     if (buf == nullptr) return make_float2(a, b);
-    float2* t = buf + turn * 32;
+    float* t = buf + turn * 64;
     turn = turn == 2 ? 0 : turn + 1;
-    if ((threadIdx.x & 31) == 0) t[threadIdx.x >> 5] = make_float2(a, b);
-    __syncthreads();
-    float2 s = make_float2(0.f, 0.f);
-    for (int w = 0; w < int(blockDim.x >> 5); ++w) {
-      s.x += t[w].x;
-      s.y += t[w].y;
+    if ((threadIdx.x & 31) == 0) {
+      t[threadIdx.x >> 5] = a;
+      t[32 + (threadIdx.x >> 5)] = b;
     }
-    return s;
+    __syncthreads();
+    return make_float2(across(t), across(t + 32));
   }
 };
 
-// The gate of a row where it is not one of the columns' factors.
-template <typename TU, int NCH, bool VEC>
-__device__ __forceinline__ void load_gate(Pack8<TU> (&raw)[NCH], float& one, const NormArgs& a, int64_t r, int tid, int team) {
-  if (a.gate_mode == kGateRow) one = load_f(a.gate, a.gate_dtype, r);
-  if (a.gate_mode == kGateFull)
-#pragma unroll
-    for (int j = 0; j < NCH; ++j)
-      load8<TU, VEC>(raw[j], static_cast<const TU*>(a.gate) + r * a.ld_gate, j, tid, team, a.cols);
-}
-
 // Column factors of the team: k = bs act(g) w_post (the gate only where it is the columns'), w = w_pre.
 template <int NCH, bool VEC>
-__device__ __forceinline__ void load_factors(const NormArgs& a, int64_t group, int tid, int team, float (&k)[NCH][8],
-                                             float (&w)[NCH][8]) {
+__device__ __forceinline__ void load_factors(const NormArgs& a, int64_t group, int tid, int team, V8 (&k)[NCH],
+                                             V8 (&w)[NCH]) {
 #pragma unroll
-  for (int j = 0; j < NCH; ++j)
+  for (int j = 0; j < NCH; ++j) {
+    float kf[8], wf[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int c = col_of<VEC>(j, i, tid, team);
@@ -164,226 +271,247 @@ __device__ __forceinline__ void load_factors(const NormArgs& a, int64_t group, i
       if (in && a.post_weight != nullptr) f *= __ldg(a.post_weight + c);
       if (in && a.gate_mode == kGateChannel)
         f *= act_of(load_f(a.gate, a.gate_dtype, group * a.cols + c), a.gate_act);
-      k[j][i] = f;
-      w[j][i] = in && a.pre_weight != nullptr ? __ldg(a.pre_weight + c) : 0.f;
+      kf[i] = f;
+      wf[i] = in && a.pre_weight != nullptr ? __ldg(a.pre_weight + c) : 0.f;
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      k[j].p[i] = f2pack(kf[2 * i], kf[2 * i + 1]);
+      w[j].p[i] = f2pack(wf[2 * i], wf[2 * i + 1]);
+    }
+  }
 }
 
 struct TeamPlan {
   int64_t parts;       // teams of a group of rows
   int64_t group_rows;
   int64_t teams;       // in all
+  int depth;           // rows ahead in shared memory
 };
 
-template <typename TX, typename TU, int NCH, bool VEC>
+// 16-byte pieces of a thread's row, by operand.
+template <typename TX, typename TU, int NCH>
+struct Slots {
+  static constexpr uint32_t x = 0, px = NCH * sizeof(TX) / 2, pu = NCH * sizeof(TU) / 2;
+  static constexpr uint32_t u = px, gate = px + pu, dy = px + 2 * pu, dh = 2 * px + 2 * pu;
+  static constexpr uint32_t forward = px + 2 * pu, backward = 2 * px + 3 * pu;
+};
+
+// What a team works on: its place in the CTA, its rows and the rows ahead.
+template <int NCH, bool VEC>
+struct Team {
+  int team, tid;
+  int64_t id, group, end;
+  TeamSum sum;
+  Ahead<NCH, VEC> ahead;
+  __device__ __forceinline__ Team(const NormArgs& a, const TeamPlan& plan, char* smem, float* buf, uint32_t pieces) {
+    const bool warp_team = a.cols <= 256;
+    team = warp_team ? 32 : int(blockDim.x);
+    tid = warp_team ? int(threadIdx.x & 31) : int(threadIdx.x);
+    id = warp_team ? int64_t(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5) : int64_t(blockIdx.x);
+    group = id / plan.parts;
+    end = (group + 1) * plan.group_rows;
+    sum = TeamSum{warp_team ? nullptr : buf, int(blockDim.x >> 5), 0};
+    ahead = Ahead<NCH, VEC>{smem + threadIdx.x * 16, blockDim.x * 16, blockDim.x * 16 * pieces, plan.depth, 0};
+  }
+};
+
+template <typename TX, typename TU, int NCH, bool VEC, bool FULL>
 __global__ void __launch_bounds__(NCH == 1 ? 256 : 512, NCH == 1 ? 3 : 1)
     residual_norm_team_kernel(const NormArgs a, const TeamPlan plan) {
-  __shared__ float2 buf[3 * 32];
-  const bool warp_team = a.cols <= 256;
-  const int team = warp_team ? 32 : int(blockDim.x);
-  const int tid = warp_team ? int(threadIdx.x & 31) : int(threadIdx.x);
-  const int64_t id = warp_team ? int64_t(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5) : int64_t(blockIdx.x);
-  if (id >= plan.teams) return;  // a whole team: no barrier is left behind
-  TeamSum sum{warp_team ? nullptr : buf, 0};
-  const int64_t group = id / plan.parts;
-  const int64_t end = (group + 1) * plan.group_rows;
-  float k[NCH][8], w[NCH][8];
-  load_factors<NCH, VEC>(a, group, tid, team, k, w);
-  const float inv = 1.f / float(a.cols);
-  Pack8<TX> x[NCH];
-  Pack8<TU> u[NCH], g[NCH];
-  float g1 = 1.f;
-  auto load = [&](int64_t r) {
+  extern __shared__ __align__(16) char smem[];
+  __shared__ float buf[3 * 64];
+  using S = Slots<TX, TU, NCH>;
+  Team<NCH, VEC> t(a, plan, smem, buf, FULL ? S::forward : S::gate);
+  if (t.id >= plan.teams) return;  // a whole team: no barrier is left behind
+  const int tid = t.tid, team = t.team, cols = a.cols;
+  V8 k[NCH], w[NCH];
+  load_factors<NCH, VEC>(a, t.group, tid, team, k, w);
+  const float inv = 1.f / float(cols);
+  const bool branch = a.branch != nullptr;
+  const TX* px = static_cast<const TX*>(a.x);
+  const TU* pu = static_cast<const TU*>(a.branch);
+  const TU* pg = static_cast<const TU*>(a.gate);
+  auto fetch = [&](int64_t r, int s) {
+    if (r < t.end) {
+      t.ahead.fetch(px + r * a.ld_x, S::x, s, tid, team, cols);
+      if (branch) t.ahead.fetch(pu + r * a.ld_branch, S::u, s, tid, team, cols);
+      if (FULL) t.ahead.fetch(pg + r * a.ld_gate, S::gate, s, tid, team, cols);
+    }
+    t.ahead.commit();
+  };
+  int64_t r = t.group * plan.group_rows + t.id % plan.parts;
+  for (int s = 0; s < plan.depth; ++s) fetch(r + s * plan.parts, s);
+  for (; r < t.end; r += plan.parts) {
+    t.ahead.wait();
+    V8 y[NCH], f[NCH];
+    float ru = 1.f, s = 0.f;
 #pragma unroll
     for (int j = 0; j < NCH; ++j) {
-      load8<TX, VEC>(x[j], static_cast<const TX*>(a.x) + r * a.ld_x, j, tid, team, a.cols);
-      if (a.branch != nullptr) load8<TU, VEC>(u[j], static_cast<const TU*>(a.branch) + r * a.ld_branch, j, tid, team, a.cols);
-    }
-    load_gate<TU, NCH, VEC>(g, g1, a, r, tid, team);
-  };
-  int64_t r = group * plan.group_rows + id % plan.parts;
-  if (r < end) load(r);
-  for (; r < end; r += plan.parts) {
-    float y[NCH][8];
-    float ru = 1.f;
-    if (a.branch != nullptr) {
-      float f[NCH][8];
+      y[j] = t.ahead.take(px + r * a.ld_x, S::x, j, tid, team, cols);
+      if (!branch) continue;
+      const V8 u = t.ahead.take(pu + r * a.ld_branch, S::u, j, tid, team, cols);
+      f[j] = mul(u, k[j]);
+      if (FULL) {
+        const V8 g = t.ahead.take(pg + r * a.ld_gate, S::gate, j, tid, team, cols);
 #pragma unroll
-      for (int j = 0; j < NCH; ++j)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          f[j][i] = k[j][i] * elem_f(u[j].v[i]);
-          y[j][i] = a.residual_scale * elem_f(x[j].v[i]);
-        }
-      if (a.post_weight != nullptr) {
-        float s = 0.f;
-#pragma unroll
-        for (int j = 0; j < NCH; ++j)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) s += elem_f(u[j].v[i]) * elem_f(u[j].v[i]);
-        ru = rsqrtf(sum(s, 0.f).x * inv + a.eps);
+        for (int i = 0; i < 4; ++i)
+          f[j].p[i] = fmul2(f[j].p[i], f2pack(act_of(g.get(2 * i), a.gate_act), act_of(g.get(2 * i + 1), a.gate_act)));
       }
-      if (a.gate_mode == kGateFull) {
-#pragma unroll
-        for (int j = 0; j < NCH; ++j)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) f[j][i] *= act_of(elem_f(g[j].v[i]), a.gate_act);
-      }
-      const float scale = a.gate_mode == kGateRow ? ru * act_of(g1, a.gate_act) : ru;
-#pragma unroll
-      for (int j = 0; j < NCH; ++j)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[j][i] += scale * f[j][i];
-    } else {
-#pragma unroll
-      for (int j = 0; j < NCH; ++j)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[j][i] = elem_f(x[j].v[i]);
+      s += total(mul(u, u));
     }
-    const int64_t next = r + plan.parts;
-    if (next < end) load(next);
-    if (a.stream_out != nullptr)
-#pragma unroll
-      for (int j = 0; j < NCH; ++j)
-        store8<TX, VEC>(static_cast<TX*>(a.stream_out) + r * a.cols, y[j], j, tid, team, a.cols);
-    float ry = 1.f;
-    if (a.pre_weight != nullptr) {
-      float s = 0.f;
-#pragma unroll
-      for (int j = 0; j < NCH; ++j)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) s += y[j][i] * y[j][i];
-      ry = rsqrtf(sum(s, 0.f).x * inv + a.eps);
+    const float gate = a.gate_mode == kGateRow ? act_of(load_f(a.gate, a.gate_dtype, r), a.gate_act) : 1.f;
+    fetch(r + plan.depth * plan.parts, t.ahead.slot);
+    t.ahead.next();
+    if (branch) {
+      if (a.post_weight != nullptr) ru = rsqrtf(t.sum.one(s) * inv + a.eps);
+      const float scale = ru * gate;
 #pragma unroll
       for (int j = 0; j < NCH; ++j) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[j][i] *= ry * w[j][i];
-        store8<TU, VEC>(static_cast<TU*>(a.norm_out) + r * a.cols, y[j], j, tid, team, a.cols);
+        y[j] = fma(f[j], scale, mul(y[j], a.residual_scale));
+        store8<TX, VEC>(static_cast<TX*>(a.stream_out) + r * cols, y[j], j, tid, team, cols);
       }
+    }
+    float ry = 1.f;
+    if (a.pre_weight != nullptr) {
+      s = 0.f;
+#pragma unroll
+      for (int j = 0; j < NCH; ++j) s += total(mul(y[j], y[j]));
+      ry = rsqrtf(t.sum.one(s) * inv + a.eps);
+#pragma unroll
+      for (int j = 0; j < NCH; ++j)
+        store8<TU, VEC>(static_cast<TU*>(a.norm_out) + r * cols, mul(mul(y[j], ry), w[j]), j, tid, team, cols);
     }
     if (a.stats != nullptr && tid == 0) *reinterpret_cast<float2*>(a.stats + 2 * r) = make_float2(ru, ry);
   }
 }
 
-template <typename TX, typename TU, int NCH, bool VEC>
+template <typename TX, typename TU, int NCH, bool VEC, bool FULL>
 __global__ void __launch_bounds__(NCH == 1 ? 256 : 512, NCH == 1 ? 2 : 1)
     residual_norm_team_bwd_kernel(const NormArgs a, const TeamPlan plan, float* partial) {
-  __shared__ float2 buf[3 * 32];
-  const bool warp_team = a.cols <= 256;
-  const int team = warp_team ? 32 : int(blockDim.x);
-  const int tid = warp_team ? int(threadIdx.x & 31) : int(threadIdx.x);
-  const int64_t id = warp_team ? int64_t(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5) : int64_t(blockIdx.x);
-  if (id >= plan.teams) return;
-  TeamSum sum{warp_team ? nullptr : buf, 0};
-  const int64_t group = id / plan.parts;
-  const int64_t end = (group + 1) * plan.group_rows;
-  float k[NCH][8], w[NCH][8], acc_pre[NCH][8], acc_s[NCH][8];
-  load_factors<NCH, VEC>(a, group, tid, team, k, w);
+  extern __shared__ __align__(16) char smem[];
+  __shared__ float buf[3 * 64];
+  using S = Slots<TX, TU, NCH>;
+  Team<NCH, VEC> t(a, plan, smem, buf, S::backward);
+  if (t.id >= plan.teams) return;
+  const int tid = t.tid, team = t.team, cols = a.cols;
+  V8 k[NCH], w[NCH], acc_pre[NCH], acc_s[NCH];
+  load_factors<NCH, VEC>(a, t.group, tid, team, k, w);
 #pragma unroll
-  for (int j = 0; j < NCH; ++j)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) acc_pre[j][i] = acc_s[j][i] = 0.f;
-  const float inv = 1.f / float(a.cols);
+  for (int j = 0; j < NCH; ++j) {
+    acc_pre[j].fill(0.f);
+    acc_s[j].fill(0.f);
+  }
+  const float inv = 1.f / float(cols);
   const bool normed = a.d_normed != nullptr, post = a.post_weight != nullptr, branch = a.branch != nullptr;
   const float rs = branch ? a.residual_scale : 1.f;
-  Pack8<TX> x[NCH], dy[NCH];
-  Pack8<TU> u[NCH], dh[NCH], g[NCH];
-  float g1 = 0.f;
-  float2 st = make_float2(1.f, 1.f);
-  auto load = [&](int64_t r) {
+  const TX* px = static_cast<const TX*>(a.x);
+  const TU* pu = static_cast<const TU*>(a.branch);
+  const TU* pg = static_cast<const TU*>(a.gate);
+  const TX* pdy = static_cast<const TX*>(a.d_stream);
+  const TU* pdh = static_cast<const TU*>(a.d_normed);
+  auto fetch = [&](int64_t r, int s) {
+    if (r < t.end) {
+      if (normed) {
+        t.ahead.fetch(px + r * a.ld_x, S::x, s, tid, team, cols);
+        t.ahead.fetch(pdh + r * a.ld_d_normed, S::dh, s, tid, team, cols);
+      }
+      if (branch) t.ahead.fetch(pu + r * a.ld_branch, S::u, s, tid, team, cols);
+      if (FULL) t.ahead.fetch(pg + r * a.ld_gate, S::gate, s, tid, team, cols);
+      if (pdy != nullptr) t.ahead.fetch(pdy + r * a.ld_d_stream, S::dy, s, tid, team, cols);
+    }
+    t.ahead.commit();
+  };
+  int64_t r = t.group * plan.group_rows + t.id % plan.parts;
+  for (int s = 0; s < plan.depth; ++s) fetch(r + s * plan.parts, s);
+  for (; r < t.end; r += plan.parts) {
+    float2 st = make_float2(1.f, 1.f);
+    if (a.stats != nullptr) st = __ldg(reinterpret_cast<const float2*>(a.stats + 2 * r));
+    const float a1 = a.gate_mode == kGateRow ? act_of(load_f(a.gate, a.gate_dtype, r), a.gate_act) : 1.f;
+    const float ru = st.x, ry = st.y;
+    t.ahead.wait();
+    V8 z[NCH], uh[NCH], f[NCH];  // dz; u r_u; k with the row's or the element's gate
+    if (branch) {
+#pragma unroll
+      for (int j = 0; j < NCH; ++j) {
+        uh[j] = mul(t.ahead.take(pu + r * a.ld_branch, S::u, j, tid, team, cols), ru);
+        f[j] = a.gate_mode == kGateRow ? mul(k[j], a1) : k[j];
+        if (FULL) {
+          const V8 g = t.ahead.take(pg + r * a.ld_gate, S::gate, j, tid, team, cols);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            f[j].p[i] = fmul2(f[j].p[i], f2pack(act_of(g.get(2 * i), a.gate_act), act_of(g.get(2 * i + 1), a.gate_act)));
+        }
+      }
+    }
 #pragma unroll
     for (int j = 0; j < NCH; ++j) {
-      load8<TX, VEC>(x[j], static_cast<const TX*>(a.x) + r * a.ld_x, j, tid, team, a.cols);
-      if (branch) load8<TU, VEC>(u[j], static_cast<const TU*>(a.branch) + r * a.ld_branch, j, tid, team, a.cols);
-      if (a.d_stream != nullptr)
-        load8<TX, VEC>(dy[j], static_cast<const TX*>(a.d_stream) + r * a.ld_d_stream, j, tid, team, a.cols);
-      if (normed) load8<TU, VEC>(dh[j], static_cast<const TU*>(a.d_normed) + r * a.ld_d_normed, j, tid, team, a.cols);
+      if (pdy != nullptr) z[j] = t.ahead.take(pdy + r * a.ld_d_stream, S::dy, j, tid, team, cols);
+      else z[j].fill(0.f);
     }
-    load_gate<TU, NCH, VEC>(g, g1, a, r, tid, team);
-    if (a.stats != nullptr) st = *reinterpret_cast<const float2*>(a.stats + 2 * r);
-  };
-  int64_t r = group * plan.group_rows + id % plan.parts;
-  if (r < end) load(r);
-  for (; r < end; r += plan.parts) {
-    const float ru = st.x, ry = st.y;
-    const float a1 = a.gate_mode == kGateRow ? act_of(g1, a.gate_act) : 1.f;
-    // z: dz; uh: u r_u; f: the element's k, its gate applied
-    float z[NCH][8], uh[NCH][8], f[NCH][8];
-    float dot = 0.f;
-#pragma unroll
-    for (int j = 0; j < NCH; ++j)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        z[j][i] = a.d_stream != nullptr ? elem_f(dy[j].v[i]) : 0.f;
-        uh[j][i] = branch ? elem_f(u[j].v[i]) * ru : 0.f;
-        f[j][i] = a.gate_mode == kGateFull ? k[j][i] * act_of(elem_f(g[j].v[i]), a.gate_act) : k[j][i] * a1;
-      }
     if (normed) {
-      float yh[NCH][8];
+      V8 yh[NCH];
+      float dot = 0.f;
 #pragma unroll
-      for (int j = 0; j < NCH; ++j)
+      for (int j = 0; j < NCH; ++j) {
+        const V8 x = mul(t.ahead.take(px + r * a.ld_x, S::x, j, tid, team, cols), rs);
+        yh[j] = mul(branch ? fma(f[j], uh[j], x) : x, ry);
+        const V8 d = t.ahead.take(pdh + r * a.ld_d_normed, S::dh, j, tid, team, cols);
+        acc_pre[j] = fma(d, yh[j], acc_pre[j]);
+        const V8 dw = mul(d, w[j]);
+        dot += total(mul(dw, yh[j]));
+        z[j] = fma(dw, ry, z[j]);
+      }
+      const float mean = t.sum.one(dot) * (inv * ry);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float d = elem_f(dh[j].v[i]);
-          yh[j][i] = (rs * elem_f(x[j].v[i]) + f[j][i] * uh[j][i]) * ry;
-          acc_pre[j][i] += d * yh[j][i];
-          dot += d * w[j][i] * yh[j][i];
-        }
-      const float mean = sum(dot, 0.f).x * inv;
-#pragma unroll
-      for (int j = 0; j < NCH; ++j)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) z[j][i] += ry * (elem_f(dh[j].v[i]) * w[j][i] - yh[j][i] * mean);
+      for (int j = 0; j < NCH; ++j) z[j] = fma(yh[j], -mean, z[j]);
     }
     float dot_u = 0.f, dot_g = 0.f;
-    float slope[NCH][8];  // of the full gate: bs act'(g) w_post uh dz
-    const float s1 = act_slope(a1, a.gate_act);
+    if (branch) {
 #pragma unroll
-    for (int j = 0; j < NCH; ++j)
+      for (int j = 0; j < NCH; ++j) {
+        const V8 zu = mul(z[j], uh[j]);
+        if (post) dot_u += total(mul(f[j], zu));
+        if (a.gate_mode == kGateRow) dot_g += total(mul(k[j], zu));
+        if (FULL) {
+          const V8 g = t.ahead.take(pg + r * a.ld_gate, S::gate, j, tid, team, cols);
+          V8 dg = mul(k[j], zu), act;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float zu = z[j][i] * uh[j][i];
-        dot_u += f[j][i] * zu;
-        dot_g += k[j][i] * zu;
-        if (a.gate_mode == kGateFull) {
-          const float ga = act_of(elem_f(g[j].v[i]), a.gate_act);
-          slope[j][i] = act_slope(ga, a.gate_act) * (k[j][i] * zu);
-          acc_s[j][i] += ga * zu;
+          for (int i = 0; i < 4; ++i) {
+            const float g0 = act_of(g.get(2 * i), a.gate_act), g1 = act_of(g.get(2 * i + 1), a.gate_act);
+            act.p[i] = f2pack(g0, g1);
+            dg.p[i] = fmul2(dg.p[i], f2pack(act_slope(g0, a.gate_act), act_slope(g1, a.gate_act)));
+          }
+          acc_s[j] = fma(act, zu, acc_s[j]);
+          if (a.d_gate != nullptr) store8<TU, VEC>(static_cast<TU*>(a.d_gate) + r * cols, dg, j, tid, team, cols);
         } else {
-          acc_s[j][i] += a1 * zu;
+          acc_s[j] = fma(zu, a1, acc_s[j]);
         }
       }
-    const float row_slope = s1;
-    const int64_t here = r;
-    const int64_t next = r + plan.parts;
-    if (next < end) load(next);
-    if (a.d_x != nullptr)
-#pragma unroll
-      for (int j = 0; j < NCH; ++j) {
-        float o[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] = rs * z[j][i];
-        store8<TX, VEC>(static_cast<TX*>(a.d_x) + here * a.cols, o, j, tid, team, a.cols);
-      }
-    if (!branch) continue;
-    if (a.gate_mode == kGateFull && a.d_gate != nullptr)
+    }
+    fetch(r + plan.depth * plan.parts, t.ahead.slot);
+    t.ahead.next();
+    if (a.d_x != nullptr) {
 #pragma unroll
       for (int j = 0; j < NCH; ++j)
-        store8<TU, VEC>(static_cast<TU*>(a.d_gate) + here * a.cols, slope[j], j, tid, team, a.cols);
-    float mean_u = 0.f;
-    if (post || a.gate_mode == kGateRow) {
-      const float2 s = sum(dot_u, dot_g);
-      if (post) mean_u = s.x * inv;
-      if (a.gate_mode == kGateRow && tid == 0 && a.d_gate != nullptr) static_cast<float*>(a.d_gate)[here] = row_slope * s.y;
+        store8<TX, VEC>(static_cast<TX*>(a.d_x) + r * cols, mul(z[j], rs), j, tid, team, cols);
     }
-    if (a.d_branch != nullptr)
+    if (!branch) continue;
+    float mean_u = 0.f;
+    if (a.gate_mode == kGateRow) {
+      const float2 s = t.sum.two(dot_u, dot_g);
+      mean_u = s.x * inv;
+      if (tid == 0 && a.d_gate != nullptr) static_cast<float*>(a.d_gate)[r] = act_slope(a1, a.gate_act) * s.y;
+    } else if (post) {
+      mean_u = t.sum.one(dot_u) * inv;
+    }
+    if (a.d_branch != nullptr) {
+      mean_u = post ? -mean_u * ru : 0.f;
 #pragma unroll
-      for (int j = 0; j < NCH; ++j) {
-        float o[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] = ru * (f[j][i] * z[j][i] - uh[j][i] * mean_u);
-        store8<TU, VEC>(static_cast<TU*>(a.d_branch) + here * a.cols, o, j, tid, team, a.cols);
-      }
+      for (int j = 0; j < NCH; ++j)
+        store8<TU, VEC>(static_cast<TU*>(a.d_branch) + r * cols, fma(uh[j], mean_u, mul(mul(f[j], z[j]), ru)), j, tid, team,
+                        cols);
+    }
   }
   if (partial == nullptr) return;
 #pragma unroll
@@ -391,9 +519,9 @@ __global__ void __launch_bounds__(NCH == 1 ? 256 : 512, NCH == 1 ? 2 : 1)
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int c = col_of<VEC>(j, i, tid, team);
-      if (c >= a.cols) continue;
-      partial[id * a.cols + c] = acc_pre[j][i];
-      partial[(plan.teams + id) * a.cols + c] = acc_s[j][i];
+      if (c >= cols) continue;
+      partial[t.id * cols + c] = acc_pre[j].get(i);
+      partial[(plan.teams + t.id) * cols + c] = acc_s[j].get(i);
     }
 }
 
@@ -603,6 +731,7 @@ struct NormShape {
   bool wide;         // 16 columns a thread instead of 8
   int threads;       // of a CTA
   int rows_per_cta;  // teams of a CTA
+  int ctas_per_sm;
   TeamPlan plan;
   int64_t groups;
 };
@@ -616,8 +745,8 @@ NormShape norm_shape(int64_t rows, int cols, int gate_mode, int64_t gate_rows, b
   s.rows_per_cta = cols <= 256 ? 4 : 1;
   if (cols > kTeamCols) s.threads = kNormThreads;
   const int64_t per_sm = cols > kTeamCols ? 512 : s.wide ? 512 : backward ? 512 : 768;
-  const int64_t ctas = per_sm / s.threads > 0 ? per_sm / s.threads : 1;
-  const int64_t want = ctas * num_sms() * s.rows_per_cta;
+  s.ctas_per_sm = per_sm / s.threads > 0 ? int(per_sm / s.threads) : 1;
+  const int64_t want = int64_t(s.ctas_per_sm) * num_sms() * s.rows_per_cta;
   s.groups = gate_mode == kGateChannel ? rows / gate_rows : 1;
   s.plan.group_rows = gate_mode == kGateChannel ? gate_rows : rows;
   int64_t parts = want / s.groups;
@@ -651,33 +780,53 @@ bool norm_in_registers(const NormArgs& a) {
   return a.x_dtype == a.norm_dtype || a.x_dtype == 1;
 }
 
-template <typename TX, typename TU, int NCH, bool VEC>
-void launch_team(const NormArgs& a, const NormShape& s, bool backward, float* partial, cudaStream_t stream) {
+// Rows ahead: up to four, as many as the CTAs that are resident at once have room for.
+constexpr int kAheadBytes = 200 * 1024;  // of an SM's shared memory
+
+template <typename TX, typename TU, int NCH, bool VEC, bool FULL>
+int launch_team(const NormArgs& a, NormShape s, bool backward, float* partial, cudaStream_t stream) {
+  using S = Slots<TX, TU, NCH>;
+  const int stage = s.threads * 16 * int(backward ? S::backward : FULL ? S::forward : S::gate);
+  int depth = kAheadBytes / s.ctas_per_sm / stage;
+  depth = depth > 4 ? 4 : depth < 1 ? 1 : depth;
+  const int smem = VEC ? depth * stage : 0;
+  s.plan.depth = VEC ? depth : 0;
   const unsigned grid = unsigned((s.plan.teams + s.rows_per_cta - 1) / s.rows_per_cta);
-  if (backward) residual_norm_team_bwd_kernel<TX, TU, NCH, VEC><<<grid, s.threads, 0, stream>>>(a, s.plan, partial);
-  else residual_norm_team_kernel<TX, TU, NCH, VEC><<<grid, s.threads, 0, stream>>>(a, s.plan);
+  if (backward) {
+    static std::atomic<uint64_t> raised{0};
+    if (VEC && !raise_smem_limit(residual_norm_team_bwd_kernel<TX, TU, NCH, VEC, FULL>, 220 * 1024, raised))
+      return MCL4MOE_ERR_CUDA;
+    residual_norm_team_bwd_kernel<TX, TU, NCH, VEC, FULL><<<grid, s.threads, smem, stream>>>(a, s.plan, partial);
+  } else {
+    static std::atomic<uint64_t> raised{0};
+    if (VEC && !raise_smem_limit(residual_norm_team_kernel<TX, TU, NCH, VEC, FULL>, 220 * 1024, raised))
+      return MCL4MOE_ERR_CUDA;
+    residual_norm_team_kernel<TX, TU, NCH, VEC, FULL><<<grid, s.threads, smem, stream>>>(a, s.plan);
+  }
+  return MCL4MOE_OK;
+}
+template <typename TX, typename TU, int NCH, bool VEC>
+int launch_team(const NormArgs& a, const NormShape& s, bool backward, float* partial, cudaStream_t stream) {
+  return a.gate_mode == kGateFull ? launch_team<TX, TU, NCH, VEC, true>(a, s, backward, partial, stream)
+                                  : launch_team<TX, TU, NCH, VEC, false>(a, s, backward, partial, stream);
 }
 template <typename TX, typename TU>
-void launch_team(const NormArgs& a, const NormShape& s, bool backward, float* partial, cudaStream_t stream) {
+int launch_team(const NormArgs& a, const NormShape& s, bool backward, float* partial, cudaStream_t stream) {
   const bool vec = norm_vectors(a);
-  if (s.wide) {
-    if (vec) launch_team<TX, TU, 2, true>(a, s, backward, partial, stream);
-    else launch_team<TX, TU, 2, false>(a, s, backward, partial, stream);
-  } else {
-    if (vec) launch_team<TX, TU, 1, true>(a, s, backward, partial, stream);
-    else launch_team<TX, TU, 1, false>(a, s, backward, partial, stream);
-  }
+  if (s.wide)
+    return vec ? launch_team<TX, TU, 2, true>(a, s, backward, partial, stream)
+               : launch_team<TX, TU, 2, false>(a, s, backward, partial, stream);
+  return vec ? launch_team<TX, TU, 1, true>(a, s, backward, partial, stream)
+             : launch_team<TX, TU, 1, false>(a, s, backward, partial, stream);
 }
-void launch_teams(const NormArgs& a, const NormShape& s, bool backward, float* partial, cudaStream_t stream) {
+int launch_teams(const NormArgs& a, const NormShape& s, bool backward, float* partial, cudaStream_t stream) {
   if (a.x_dtype == 1) {
-    if (a.norm_dtype == 0) launch_team<float, uint16_t>(a, s, backward, partial, stream);
-    else if (a.norm_dtype == 1) launch_team<float, float>(a, s, backward, partial, stream);
-    else launch_team<float, __half>(a, s, backward, partial, stream);
-  } else if (a.x_dtype == 0) {
-    launch_team<uint16_t, uint16_t>(a, s, backward, partial, stream);
-  } else {
-    launch_team<__half, __half>(a, s, backward, partial, stream);
+    if (a.norm_dtype == 0) return launch_team<float, uint16_t>(a, s, backward, partial, stream);
+    if (a.norm_dtype == 1) return launch_team<float, float>(a, s, backward, partial, stream);
+    return launch_team<float, __half>(a, s, backward, partial, stream);
   }
+  if (a.x_dtype == 0) return launch_team<uint16_t, uint16_t>(a, s, backward, partial, stream);
+  return launch_team<__half, __half>(a, s, backward, partial, stream);
 }
 
 }  // namespace
@@ -694,7 +843,8 @@ int mcl4moe_residual_norm(const mcl4moe_norm_args* a, mcl4moe_stream_t stream) {
   const NormShape s = norm_shape(a->rows, a->cols, a->gate_mode, a->gate_rows, false);
   if (s.plan.teams > (int64_t(1) << 30)) return MCL4MOE_ERR_UNSUPPORTED;
   if (norm_in_registers(*a)) {
-    launch_teams(*a, s, false, nullptr, stream);
+    const int team = launch_teams(*a, s, false, nullptr, stream);
+    if (team != MCL4MOE_OK) return team;
   } else {
     const int64_t grid = a->rows < int64_t(64) * num_sms() ? a->rows : int64_t(64) * num_sms();
     residual_norm_kernel<<<unsigned(grid), kNormThreads, 0, stream>>>(*a);
@@ -726,7 +876,8 @@ int mcl4moe_residual_norm_backward(const mcl4moe_norm_args* a, void* workspace, 
     return MCL4MOE_ERR_WORKSPACE;
   float* partial = sums ? static_cast<float*>(workspace) : nullptr;
   if (norm_in_registers(*a)) {
-    launch_teams(*a, s, true, partial, stream);
+    const int team = launch_teams(*a, s, true, partial, stream);
+    if (team != MCL4MOE_OK) return team;
   } else {
     static std::atomic<uint64_t> raised{0};
     if (!raise_smem_limit(residual_norm_bwd_kernel, 2 * kMaxNormCols * int(sizeof(float)), raised)) return MCL4MOE_ERR_CUDA;

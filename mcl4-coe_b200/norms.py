@@ -7,10 +7,11 @@ from __future__ import annotations
 
 import torch
 from torch import Tensor
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .nvfp4 import _ptr, _require_cuda
-from .routing import DTYPE_CODES, _launch, _ld, _rows
+from .routing import DTYPE_CODES, _f32, _launch, _ld, _rows
 
 GATE_ACTIVATIONS = ("none", "sigmoid", "tanh")
 MAX_COLS = 16384
@@ -23,6 +24,8 @@ _MAX_GROUPS = 65533
 
 def _gate_form(gate: Tensor, x: Tensor) -> tuple[Tensor, int, int]:
     """(gate, mode, rows that share a gate row) for a gate that broadcasts to ``x``."""
+    if gate.ndim == 1 and gate.shape[0] == x.shape[-1]:
+        return gate.contiguous().view(1, -1), _CHANNEL, max(1, x.numel() // x.shape[-1])
     if gate.ndim > x.ndim or any(g != 1 and g != s for g, s in zip(gate.shape[::-1], x.shape[::-1])):
         raise ValueError(f"gate {tuple(gate.shape)} does not broadcast to {tuple(x.shape)}")
     gate = gate.reshape((1,) * (x.ndim - gate.ndim) + tuple(gate.shape))
@@ -59,8 +62,8 @@ def _fill(args, x, branch, post, pre, gate, mode, gate_rows, act, norm_dtype, sc
 
 
 def _norm_forward(x, branch, post, pre, gate, mode, gate_rows, act, norm_dtype, scales, stats=None):
-    y = None if branch is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    h = None if pre is None else torch.empty(x.shape, dtype=norm_dtype, device=x.device)
+    y = None if branch is None else x.new_empty(x.shape)
+    h = None if pre is None else x.new_empty(x.shape, dtype=norm_dtype)
     if x.shape[0] == 0:
         return y, h
     args = _fill(_lib.NormArgs(), x, branch, post, pre, gate, mode, gate_rows, act, norm_dtype, scales)
@@ -74,7 +77,7 @@ class _ResidualNorm(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, branch, post, pre, gate, mode, gate_rows, act, norm_dtype, scales):
-        stats = torch.empty((x.shape[0], 2), dtype=torch.float32, device=x.device)
+        stats = x.new_empty((x.shape[0], 2), dtype=torch.float32)
         y, h = _norm_forward(x, branch, post, pre, gate, mode, gate_rows, act, norm_dtype, scales, stats)
         ctx.save_for_backward(x, branch, post, pre, gate, stats)
         ctx.args = (mode, gate_rows, act, norm_dtype, scales)
@@ -82,8 +85,18 @@ class _ResidualNorm(torch.autograd.Function):
         return y, h
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, d_y, d_h):
+        if torch.is_grad_enabled():  # create_graph: a second differentiation has to be refused
+            return _ResidualNorm._once(ctx, d_y, d_h)
+        return _ResidualNorm._gradients(ctx, d_y, d_h)
+
+    @staticmethod
+    @once_differentiable
+    def _once(ctx, d_y, d_h):
+        return _ResidualNorm._gradients(ctx, d_y, d_h)
+
+    @staticmethod
+    def _gradients(ctx, d_y, d_h):
         if d_y is None and d_h is None:
             return (None,) * 10
         x, branch, post, pre, gate, stats = ctx.saved_tensors
@@ -97,16 +110,16 @@ class _ResidualNorm(torch.autograd.Function):
         args = _fill(_lib.NormArgs(), x, branch, post, pre, gate, mode, gate_rows, act, norm_dtype, scales)
         args.stats = stats.data_ptr()
         if d_y is not None:
-            d_y = _rows(d_y.to(x.dtype))
+            d_y = _rows(d_y)
             args.d_stream, args.ld_d_stream = d_y.data_ptr(), _ld(d_y)
         if d_h is not None:
-            d_h = _rows(d_h.to(norm_dtype))
+            d_h = _rows(d_h)
             args.d_normed, args.ld_d_normed = d_h.data_ptr(), _ld(d_h)
 
         def out(wanted, like, attr, dtype=None):
             if like is None or not wanted:
                 return None
-            t = torch.empty(like.shape, dtype=dtype or like.dtype, device=dev)
+            t = x.new_empty(like.shape, dtype=dtype or like.dtype)
             setattr(args, attr, t.data_ptr())
             return t
 
@@ -118,9 +131,9 @@ class _ResidualNorm(torch.autograd.Function):
         ws, nbytes = None, 0
         if d_post is not None or d_pre is not None or (d_gate is not None and mode == _CHANNEL):
             nbytes = lib.mcl4moe_residual_norm_workspace_size(args.rows, args.cols, args.gate_mode, args.gate_rows)
-            ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+            ws = x.new_empty((nbytes,), dtype=torch.uint8)
         _launch(dev, "mcl4moe_residual_norm_backward", lib.mcl4moe_residual_norm_backward, args, _ptr(ws), nbytes)
-        if d_gate is not None:
+        if d_gate is not None and d_gate.dtype != gate.dtype:
             d_gate = d_gate.to(gate.dtype)
         return (d_x, d_branch, d_post, d_pre, d_gate) + (None,) * 5
 
@@ -171,9 +184,7 @@ def residual_norm(x: Tensor, branch: Tensor | None = None, *, post_weight: Tenso
     if gate is not None:
         gate_2d, mode, gate_rows = _gate_form(gate, x)
     _require_cuda(x, "residual_norm")
-    tensors = (_rows(x), None if branch is None else _rows(branch),
-               None if post_weight is None else post_weight.to(torch.float32).contiguous(),
-               None if pre_weight is None else pre_weight.to(torch.float32).contiguous(), gate_2d)
+    tensors = (_rows(x), None if branch is None else _rows(branch), _f32(post_weight), _f32(pre_weight), gate_2d)
     rest = (mode, gate_rows, GATE_ACTIVATIONS.index(gate_activation), norm_dtype,
             (float(residual_scale), float(branch_scale), float(eps)))
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):

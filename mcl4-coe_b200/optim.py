@@ -22,21 +22,17 @@ from .routing import DTYPE_CODES, _launch
 STATE_BLOCK = 256  # elements of a tensor that share a scale of its 8-bit moments
 
 
-def _pointers(tensors: Sequence[Tensor]) -> tuple[array, int]:
-    a = array("Q", [t.data_ptr() for t in tensors])
-    return a, a.buffer_info()[0]
-
-
-def _check_list(name: str, tensors: Sequence[Tensor], params: Sequence[Tensor], dtype: torch.dtype,
-                sizes: Sequence[int] | None = None) -> None:
-    if len(tensors) != len(params):
-        raise ValueError(f"{name}: {len(tensors)} tensors for {len(params)} parameters")
-    dev = params[0].device
-    for i, t in enumerate(tensors):
-        n = params[i].numel() if sizes is None else sizes[i]
-        if t.dtype != dtype or t.numel() != n or t.device != dev or not t.is_contiguous():
-            raise ValueError(f"{name}[{i}] must be {n} contiguous {dtype} elements on {dev}, got {t.numel()} of "
-                             f"{t.dtype} on {t.device}")
+def _check_list(name: str, tensors: Sequence[Tensor], dtype: torch.dtype, device: int, sizes: list[int]) -> None:
+    if len(tensors) != len(sizes):
+        raise ValueError(f"{name}: {len(tensors)} tensors for {len(sizes)} parameters")
+    want = {(dtype, device, True)}
+    if {(t.dtype, t.get_device(), t.is_contiguous()) for t in tensors} == want and \
+            [t.numel() for t in tensors] == sizes:
+        return
+    for i, (t, n) in enumerate(zip(tensors, sizes)):
+        if (t.dtype, t.get_device(), t.is_contiguous()) not in want or t.numel() != n:
+            raise ValueError(f"{name}[{i}] must be {n} contiguous {dtype} elements on the first parameter's device, got "
+                             f"{t.numel()} of {t.dtype} on {t.device}")
 
 
 @torch.no_grad()
@@ -82,31 +78,30 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
     dev = first.device
     if first.dtype not in DTYPE_CODES or grads[0].dtype not in DTYPE_CODES:
         raise ValueError(f"parameters and gradients must be bf16, fp16 or fp32, got {first.dtype} and {grads[0].dtype}")
-    _check_list("params", params, params, first.dtype)
-    grads = [g if g.is_contiguous() else g.contiguous() for g in grads]
-    _check_list("grads", grads, params, grads[0].dtype)
-    _check_list("exp_avgs", exp_avgs, params, torch.float8_e4m3fn if eight else torch.float32)
-    _check_list("exp_avg_sqs", exp_avg_sqs, params, torch.float8_e5m2 if eight else torch.float32)
-    numels = array("q", [p.numel() for p in params])
+    index, sizes = first.get_device(), [p.numel() for p in params]
+    _check_list("params", params, first.dtype, index, sizes)
+    if not all(g.is_contiguous() for g in grads):
+        grads = [g.contiguous() for g in grads]
+    _check_list("grads", grads, grads[0].dtype, index, sizes)
+    _check_list("exp_avgs", exp_avgs, torch.float8_e4m3fn if eight else torch.float32, index, sizes)
+    _check_list("exp_avg_sqs", exp_avg_sqs, torch.float8_e5m2 if eight else torch.float32, index, sizes)
+    numels = array("q", sizes)
     changed = [*params, *exp_avgs, *exp_avg_sqs]
     if eight:
-        blocks = [-(-n // STATE_BLOCK) for n in numels]
-        _check_list("exp_avg_scales", exp_avg_scales, params, torch.float32, blocks)
-        _check_list("exp_avg_sq_scales", exp_avg_sq_scales, params, torch.float32, blocks)
+        blocks = [-(-n // STATE_BLOCK) for n in sizes]
+        _check_list("exp_avg_scales", exp_avg_scales, torch.float32, index, blocks)
+        _check_list("exp_avg_sq_scales", exp_avg_sq_scales, torch.float32, index, blocks)
         changed += [*exp_avg_scales, *exp_avg_sq_scales]
     if masters is not None:
-        _check_list("masters", masters, params, torch.float32)
-        if any(m is p for m, p in zip(masters, params)):
-            raise ValueError("masters must be tensors of their own")
+        _check_list("masters", masters, torch.float32, index, sizes)
         changed += list(masters)
+    if len({id(t) for t in changed}) != len(changed):
+        raise ValueError("a tensor is in the lists twice")
     for name, t, dtype in (("step", step, torch.int64), ("lr", lr, torch.float32), ("grad_scale", grad_scale, torch.float32)):
         if isinstance(t, Tensor) and (t.dtype != dtype or t.numel() != 1 or t.device != dev):
             raise ValueError(f"{name} as a tensor must be one {dtype} on {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
     if indices is not None and len(indices) != len(params):
         raise ValueError(f"{len(indices)} indices for {len(params)} parameters")
-    written = [t.data_ptr() for t in changed if t.numel()]
-    if len(set(written)) != len(written):
-        raise ValueError("a tensor is in the lists twice")
     _require_cuda(first, "adamw_step")
     args = _lib.AdamwArgs(n=len(params), param_dtype=DTYPE_CODES[first.dtype],
                           grad_dtype=DTYPE_CODES[grads[0].dtype], bits=8 if eight else 32, beta1=beta1, beta2=beta2,
@@ -117,9 +112,8 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
                           ("exp_avg_scales", exp_avg_scales), ("exp_avg_sq_scales", exp_avg_sq_scales),
                           ("masters", masters)):
         if tensors is not None:
-            a, address = _pointers(tensors)
-            keep.append(a)
-            setattr(args, name, address)
+            keep.append(array("Q", [t.data_ptr() for t in tensors]))
+            setattr(args, name, keep[-1].buffer_info()[0])
     if indices is not None:
         a = array("i", indices)
         keep.append(a)

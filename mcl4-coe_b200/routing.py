@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import torch
 from torch import Tensor
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .nvfp4 import _ptr, _require_cuda
@@ -20,23 +21,39 @@ GROUP_SCORES = ("top2", "max")
 MAX_EXPERTS, MAX_TOP_K = 512, 32
 
 
+# The raw handle of a device's current stream; the public route builds a Stream object first.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _launch(device: torch.device, what: str, fn, *args) -> None:
     """One library call on ``device``'s current stream (``device`` need not be the current one)."""
-    if device.index == torch.cuda.current_device():
-        st = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    index = device.index
+    if index == torch.cuda.current_device():
+        st = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(device):
-            st = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+            st = fn(*args, _raw_stream(index))
     if st != _lib.OK:
         _lib.check(st, what)
 
 
 def _rows(t: Tensor) -> Tensor:
     """``t`` as rows [n, last] whose elements are next to each other and whose rows do not overlap."""
-    t = t.reshape(-1, t.shape[-1])
+    if t.ndim != 2:
+        t = t.reshape(-1, t.shape[-1])
+    if t.is_contiguous():
+        return t
     if (t.stride(1) != 1 and t.shape[1] > 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
         t = t.contiguous()
     return t
+
+
+def _f32(t: Tensor | None) -> Tensor | None:
+    """``t`` as contiguous float32 (differentiably)."""
+    if t is None or (t.dtype == torch.float32 and t.is_contiguous()):
+        return t
+    return t.to(torch.float32).contiguous()
 
 
 def _ld(t: Tensor) -> int:
@@ -45,11 +62,10 @@ def _ld(t: Tensor) -> int:
 
 def _route_forward(logits, k, score, bias, groups, top_groups, group_score, renorm, scale, valid):
     n, E = logits.shape
-    dev = logits.device
-    idx = torch.empty((n, k), dtype=torch.int32, device=dev)
-    w = torch.empty((n, k), dtype=torch.float32, device=dev)
-    counts = torch.empty((E,), dtype=torch.int32, device=dev)
-    _launch(dev, "mcl4moe_route_scores", _lib.load().mcl4moe_route_scores, logits.data_ptr(),
+    idx = logits.new_empty((n, k), dtype=torch.int32)
+    w = logits.new_empty((n, k), dtype=torch.float32)
+    counts = logits.new_empty((E,), dtype=torch.int32)
+    _launch(logits.device, "mcl4moe_route_scores", _lib.load().mcl4moe_route_scores, logits.data_ptr(),
             DTYPE_CODES[logits.dtype], _ld(logits), _ptr(bias), _ptr(valid), n, E, k, score, groups, top_groups,
             group_score, renorm, scale, idx.data_ptr(), w.data_ptr(), counts.data_ptr())
     return w, idx, counts
@@ -66,19 +82,29 @@ class _RouteScores(torch.autograd.Function):
         return w, idx, counts
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, d_w, _d_idx, _d_counts):
+    def backward(ctx, d_w, d_idx, d_counts):
+        if torch.is_grad_enabled():  # create_graph: a second differentiation has to be refused
+            return _RouteScores._once(ctx, d_w)
+        return _RouteScores._gradients(ctx, d_w)
+
+    @staticmethod
+    def _gradients(ctx, d_w):
         if d_w is None:
             return (None,) * 10
         logits, idx = ctx.saved_tensors
         k, score, renorm, scale = ctx.args
         n, E = logits.shape
-        d_w = d_w.to(torch.float32).contiguous()
-        d_logits = torch.empty((n, E), dtype=logits.dtype, device=logits.device)
+        d_w = _f32(d_w)
+        d_logits = logits.new_empty((n, E))
         _launch(logits.device, "mcl4moe_route_scores_backward", _lib.load().mcl4moe_route_scores_backward,
                 logits.data_ptr(), DTYPE_CODES[logits.dtype], _ld(logits), idx.data_ptr(), d_w.data_ptr(), n, E, k,
                 score, renorm, scale, d_logits.data_ptr())
         return (d_logits,) + (None,) * 9
+
+    @staticmethod
+    @once_differentiable
+    def _once(ctx, d_w):
+        return _RouteScores._gradients(ctx, d_w)
 
 
 def route_experts(logits: Tensor, top_k: int, *, score: str = "softmax", bias: Tensor | None = None,
@@ -122,12 +148,13 @@ def route_experts(logits: Tensor, top_k: int, *, score: str = "softmax", bias: T
     if bias is not None:
         if bias.shape != (E,) or bias.device != dev:
             raise ValueError(f"bias must have one entry per expert on {dev}, got {tuple(bias.shape)} on {bias.device}")
-        bias = bias.detach().to(torch.float32).contiguous()
+        bias = _f32(bias.detach())
     if valid is not None:
         if valid.shape != logits.shape[:-1] or valid.device != dev:
             raise ValueError("valid must have one entry per token on the logits' device")
+        if valid.dtype != torch.bool:
+            valid = valid != 0
         valid = valid.contiguous()
-        valid = valid.view(torch.uint8) if valid.dtype == torch.bool else (valid != 0).view(torch.uint8)
     _require_cuda(logits, "route_experts")
     lead = logits.shape[:-1]
     args = (_rows(logits), top_k, SCORE_FUNCTIONS.index(score), bias, num_groups, top_groups,
