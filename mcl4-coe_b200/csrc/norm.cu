@@ -45,7 +45,7 @@ __device__ __forceinline__ void store_f(void* p, int dtype, int64_t i, float v) 
 }
 
 __device__ __forceinline__ float act_of(float g, int act) {
-  return act == kActSigmoid ? 1.f / (1.f + expf(-g)) : act == kActTanh ? tanhf(g) : g;
+  return act == kActSigmoid ? __fdividef(1.f, 1.f + expf(-g)) : act == kActTanh ? tanhf(g) : g;
 }
 // act'(g) from a = act(g)
 __device__ __forceinline__ float act_slope(float a, int act) {
@@ -54,19 +54,17 @@ __device__ __forceinline__ float act_slope(float a, int act) {
 
 // ---------------------------------------------------------------- rows in registers
 
-// Eight elements of a row per chunk: VEC consecutive ones by 16-byte accesses, else (odd widths,
-// strides or addresses) every team-th one, so that a warp's accesses still lie side by side.
+// Eight elements of a row per chunk, so laid out that a warp's accesses lie side by side: eight
+// consecutive ones (16-bit operands, 16 bytes a thread), twice four (with a 32-bit stream, where
+// eight would leave every other 16 bytes to the next access: 16384 x 2048 float32 forward 135 us),
+// or every team-th one (odd widths, strides or addresses).
+enum { kSingles = 0, kEights = 1, kFours = 2 };
 __device__ __forceinline__ float elem_f(float v) { return v; }
 __device__ __forceinline__ float elem_f(uint16_t v) { return bf16_to_f32(v); }
 __device__ __forceinline__ float elem_f(__half v) { return __half2float(v); }
 __device__ __forceinline__ void elem_set(float& d, float v) { d = v; }
 __device__ __forceinline__ void elem_set(uint16_t& d, float v) { d = f32_to_bf16(v); }
 __device__ __forceinline__ void elem_set(__half& d, float v) { d = __float2half_rn(v); }
-
-template <typename T>
-struct __align__(16) Pack8 {
-  T v[8];
-};
 
 // Eight float32 as four pairs: one instruction for two products or sums.
 struct V8 {
@@ -112,128 +110,251 @@ __device__ __forceinline__ V8 fma(const V8& a, float s, const V8& c) {
   for (int i = 0; i < 4; ++i) r.p[i] = ffma2(a.p[i], ss, c.p[i]);
   return r;
 }
-__device__ __forceinline__ float total(const V8& a) {
+__device__ __forceinline__ V8 act8(const V8& g, int act) {
+  if (act == kActNone) return g;
+  V8 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float a, b;
+    f2unpack(g.p[i], a, b);
+    r.p[i] = f2pack(act_of(a, act), act_of(b, act));
+  }
+  return r;
+}
+__device__ __forceinline__ V8 slope8(const V8& g, int act) {
+  V8 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float a, b;
+    f2unpack(g.p[i], a, b);
+    r.p[i] = f2pack(act_slope(a, act), act_slope(b, act));
+  }
+  return r;
+}
+__device__ __forceinline__ V8 add(const V8& a, const V8& b) {
+  V8 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r.p[i] = fadd2(a.p[i], b.p[i]);
+  return r;
+}
+// Sum of the products.
+__device__ __forceinline__ float dot8(const V8& a, const V8& b) {
   float x, y;
-  f2unpack(fadd2(fadd2(a.p[0], a.p[1]), fadd2(a.p[2], a.p[3])), x, y);
+  f2unpack(fadd2(ffma2(a.p[0], b.p[0], fmul2(a.p[1], b.p[1])), ffma2(a.p[2], b.p[2], fmul2(a.p[3], b.p[3]))), x, y);
   return x + y;
 }
 
-template <bool VEC>
+template <int LAY>
 __device__ __forceinline__ int col_of(int chunk, int i, int tid, int team) {
-  return VEC ? (chunk * team + tid) * 8 + i : (chunk * 8 + i) * team + tid;
+  if (LAY == kEights) return (chunk * team + tid) * 8 + i;
+  if (LAY == kFours) return (chunk * 2 + (i >> 2)) * team * 4 + tid * 4 + (i & 3);
+  return (chunk * 8 + i) * team + tid;
 }
 
+// Two elements of one 32-bit word.
 template <typename T>
-__device__ __forceinline__ V8 unpack8(const Pack8<T>& d) {
-  V8 r;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) r.p[i] = f2pack(elem_f(d.v[2 * i]), elem_f(d.v[2 * i + 1]));
-  return r;
+__device__ __forceinline__ uint64_t unpack2(uint32_t w);
+template <>
+__device__ __forceinline__ uint64_t unpack2<uint16_t>(uint32_t w) {
+  return f2pack(bf16x2_lo(w), bf16x2_hi(w));
+}
+template <>
+__device__ __forceinline__ uint64_t unpack2<__half>(uint32_t w) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+  return f2pack(f.x, f.y);
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(uint64_t v);
+template <>
+__device__ __forceinline__ uint32_t pack2<uint16_t>(uint64_t v) {
+  float a, b;
+  f2unpack(v, a, b);
+  return pack_bf16x2(a, b);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(uint64_t v) {
+  float a, b;
+  f2unpack(v, a, b);
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
 }
 
 template <typename T>
 __device__ __forceinline__ V8 load8(const T* row, int chunk, int tid, int team, int cols) {
-  Pack8<T> d;
+  float v[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const int c = col_of<false>(chunk, i, tid, team);
-    d.v[i] = c < cols ? __ldg(row + c) : T(0.f);
+    const int c = col_of<kSingles>(chunk, i, tid, team);
+    v[i] = c < cols ? elem_f(__ldg(row + c)) : 0.f;
   }
-  return unpack8(d);
+  V8 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r.p[i] = f2pack(v[2 * i], v[2 * i + 1]);
+  return r;
 }
-template <typename T, bool VEC>
+template <typename T, int LAY>
 __device__ __forceinline__ void store8(T* row, const V8& v, int chunk, int tid, int team, int cols) {
-  if (VEC) {
-    const int c = (chunk * team + tid) * 8;
-    if (c >= cols) return;
-    Pack8<T> p;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) elem_set(p.v[i], v.get(i));
-    uint4* dst = reinterpret_cast<uint4*>(row + c);
-    const uint4* w = reinterpret_cast<const uint4*>(&p);
-#pragma unroll
-    for (int i = 0; i < int(sizeof(T)) / 2; ++i) dst[i] = w[i];
-  } else {
+  if constexpr (LAY == kSingles) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int c = col_of<false>(chunk, i, tid, team);
+      const int c = col_of<kSingles>(chunk, i, tid, team);
       if (c < cols) elem_set(row[c], v.get(i));
+    }
+  } else if constexpr (LAY == kEights) {
+    const int c = col_of<kEights>(chunk, 0, tid, team);
+    if (c < cols)
+      *reinterpret_cast<uint4*>(row + c) = make_uint4(pack2<T>(v.p[0]), pack2<T>(v.p[1]), pack2<T>(v.p[2]), pack2<T>(v.p[3]));
+  } else {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int c = col_of<kFours>(chunk, 4 * h, tid, team);
+      if (c >= cols) continue;
+      if constexpr (sizeof(T) == 4) {
+        const uint2 lo = *reinterpret_cast<const uint2*>(&v.p[2 * h]), hi = *reinterpret_cast<const uint2*>(&v.p[2 * h + 1]);
+        *reinterpret_cast<uint4*>(row + c) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+      } else {
+        *reinterpret_cast<uint2*>(row + c) = make_uint2(pack2<T>(v.p[2 * h]), pack2<T>(v.p[2 * h + 1]));
+      }
     }
   }
 }
 
+// First element of a row: one wide multiply-add from launch constants, so that a row costs no
+// registers between its uses.
+template <typename T>
+__device__ __forceinline__ T* row_at(T* base, uint32_t row, uint32_t ld_bytes) {
+  return reinterpret_cast<T*>(reinterpret_cast<uintptr_t>(base) + uint64_t(row) * ld_bytes);
+}
+
 // The rows ahead of a thread, in shared memory: it copies its own elements there (cp.async, 16
 // bytes each) `depth` rows ahead and reads them back itself, so that no barrier stands between and
-// the loads in flight need no registers.  Slots of a row: up to five operands of NCH chunks.
-// Without VEC the elements come straight from memory when they are asked for.
-template <int NCH, bool VEC>
+// the loads in flight need no registers.  A row has a 16-byte piece for each eight 16-bit or four
+// 32-bit elements of an operand; a thread's pieces lie `stride` bytes apart.
+// Single elements come straight from memory when they are asked for.
+template <int NCH, int LAY>
 struct Ahead {
-  char* mine;       // this thread's first 16 bytes
-  uint32_t stride;  // bytes between the 16-byte pieces of a thread
-  uint32_t stage;   // bytes of a row
-  int depth, slot;
+  uint32_t mine;    // shared address of this thread's first piece
+  uint32_t stride, stage, end;  // bytes: between pieces, of a row, of all rows
+  uint32_t slot;    // offset of the row at work
+  int depth, tid, team, cols;
+  bool in[2 * NCH];  // the half chunk lies inside the row
+
+  template <int BYTES>
+  static __device__ __forceinline__ void copy(uint32_t to, const void* from) {
+    if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to), "l"(from) : "memory");
+  }
   template <typename T>
-  __device__ __forceinline__ void fetch(const T* row, uint32_t at, int s, int tid, int team, int cols) const {
-    if constexpr (VEC) {
+  __device__ __forceinline__ void fetch(const T* row, uint32_t at, uint32_t to) const {
+    if constexpr (LAY == kEights) {
 #pragma unroll
-      for (int j = 0; j < NCH; ++j) {
-        const int c = (j * team + tid) * 8;
-        if (c >= cols) continue;
+      for (int j = 0; j < NCH; ++j)
+        if (in[2 * j]) copy<16>(mine + to + (at + j) * stride, row + col_of<LAY>(j, 0, tid, team));
+    } else if constexpr (LAY == kFours) {
 #pragma unroll
-        for (int i = 0; i < int(sizeof(T)) / 2; ++i) {
-          const uint32_t dst = uint32_t(__cvta_generic_to_shared(mine + s * stage + (at + j * (sizeof(T) / 2) + i) * stride));
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(row + c + i * (16 / sizeof(T)))
-                       : "memory");
+      for (int h = 0; h < 2 * NCH; ++h)
+        if (in[h]) {
+          const T* from = row + col_of<LAY>(h >> 1, 4 * (h & 1), tid, team);
+          if constexpr (sizeof(T) == 4) copy<16>(mine + to + (at + h) * stride, from);
+          else copy<8>(mine + to + (at + (h >> 1)) * stride + 8 * (h & 1), from);
         }
-      }
     }
   }
   template <typename T>
-  __device__ __forceinline__ V8 take(const T* row, uint32_t at, int j, int tid, int team, int cols) const {
-    if constexpr (!VEC) {
+  __device__ __forceinline__ V8 take(const T* row, uint32_t at, int j) const {
+    if constexpr (LAY == kSingles) {
       return load8(row, j, tid, team, cols);
     } else {
-      Pack8<T> d;
-      uint4* w = reinterpret_cast<uint4*>(&d);
-      const bool in = (j * team + tid) * 8 < cols;
-#pragma unroll
-      for (int i = 0; i < int(sizeof(T)) / 2; ++i)
-        w[i] = in ? *reinterpret_cast<const uint4*>(mine + slot * stage + (at + j * (sizeof(T) / 2) + i) * stride)
-                  : make_uint4(0u, 0u, 0u, 0u);
-      return unpack8(d);
+      V8 r;
+      const uint32_t from = mine + slot + (at + j * uint32_t(sizeof(T) / 2)) * stride;
+      const uint4 w = lds16(from);
+      if constexpr (sizeof(T) == 4) {
+        const uint4 v = lds16(from + stride);
+        r.p[0] = f2pack(__uint_as_float(w.x), __uint_as_float(w.y));
+        r.p[1] = f2pack(__uint_as_float(w.z), __uint_as_float(w.w));
+        r.p[2] = f2pack(__uint_as_float(v.x), __uint_as_float(v.y));
+        r.p[3] = f2pack(__uint_as_float(v.z), __uint_as_float(v.w));
+      } else {
+        r.p[0] = unpack2<T>(w.x);
+        r.p[1] = unpack2<T>(w.y);
+        r.p[2] = unpack2<T>(w.z);
+        r.p[3] = unpack2<T>(w.w);
+      }
+      return r;
     }
   }
+  static __device__ __forceinline__ uint4 lds16(uint32_t at) {
+    uint4 w;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(at) : "memory");
+    return w;
+  }
+  // Chunks behind the row's end are never fetched: zero once, zero for all rows.
+  __device__ __forceinline__ void clear() const {
+    if constexpr (LAY != kSingles) {
+      bool all = true;
+#pragma unroll
+      for (int j = 0; j < 2 * NCH; ++j) all = all && in[j];
+      if (!all)
+        for (uint32_t at = 0; at < end; at += stride)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(mine + at), "r"(0) : "memory");
+    }
+  }
+  // Eight values of this thread's own, behind the rows.
+  __device__ __forceinline__ void keep(int which, const V8& v) const {
+    const uint32_t to = mine + end + uint32_t(2 * which) * stride;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float a, b, c, d;
+      f2unpack(v.p[2 * h], a, b);
+      f2unpack(v.p[2 * h + 1], c, d);
+      asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to + h * stride), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
+    }
+  }
+  __device__ __forceinline__ V8 kept(int which) const {
+    V8 r;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint4 w = lds16(mine + end + uint32_t(2 * which + h) * stride);
+      r.p[2 * h] = f2pack(__uint_as_float(w.x), __uint_as_float(w.y));
+      r.p[2 * h + 1] = f2pack(__uint_as_float(w.z), __uint_as_float(w.w));
+    }
+    return r;
+  }
   __device__ __forceinline__ void commit() const {
-    if (VEC) asm volatile("cp.async.commit_group;" ::: "memory");
+    if (LAY != kSingles) asm volatile("cp.async.commit_group;" ::: "memory");
   }
   // The oldest of `depth` committed rows is there.
   __device__ __forceinline__ void wait() const {
-    if (!VEC) return;
+    if (LAY == kSingles) return;
     if (depth >= 4) asm volatile("cp.async.wait_group 3;" ::: "memory");
     else if (depth == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
     else if (depth == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
     else asm volatile("cp.async.wait_group 0;" ::: "memory");
   }
-  __device__ __forceinline__ void next() { slot = slot + 1 == depth ? 0 : slot + 1; }
+  __device__ __forceinline__ void next() { slot = slot + stage == end ? 0 : slot + stage; }
 };
 
 // Sums over the team, the same order every time; every thread gets them.  One barrier per call:
 // three buffers in turn, so that a buffer is written again only behind the barrier after its reads.
+template <int WARPS>
 struct TeamSum {
-  float* buf;  // [3][2][32] shared, or null for a one-warp team
-  int warps, turn;
-  __device__ __forceinline__ float across(const float* t) const {
+  float* buf;  // [3][2][WARPS] shared, zero where there is no such warp; or null for a one-warp team
+  int turn;
+  static __device__ __forceinline__ float across(const float* t) {
     float s = 0.f;
-#pragma unroll 4
-    for (int w = 0; w < warps; ++w) s += t[w];
+#pragma unroll
+    for (int w = 0; w < WARPS; w += 4) {
+      const float4 v = *reinterpret_cast<const float4*>(t + w);
+      s += (v.x + v.y) + (v.z + v.w);
+    }
     return s;
   }
   __device__ __forceinline__ float one(float a) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
     if (buf == nullptr) return a;
-    float* t = buf + turn * 64;
-    turn = turn == 2 ? 0 : turn + 1;
+    float* t = buf + turn;
+    turn = turn == 4 * WARPS ? 0 : turn + 2 * WARPS;
     if ((threadIdx.x & 31) == 0) t[threadIdx.x >> 5] = a;
     __syncthreads();
     return across(t);
@@ -245,19 +366,19 @@ struct TeamSum {
       b += __shfl_xor_sync(0xffffffffu, b, o);
     }
     if (buf == nullptr) return make_float2(a, b);
-    float* t = buf + turn * 64;
-    turn = turn == 2 ? 0 : turn + 1;
+    float* t = buf + turn;
+    turn = turn == 4 * WARPS ? 0 : turn + 2 * WARPS;
     if ((threadIdx.x & 31) == 0) {
       t[threadIdx.x >> 5] = a;
-      t[32 + (threadIdx.x >> 5)] = b;
+      t[WARPS + (threadIdx.x >> 5)] = b;
     }
     __syncthreads();
-    return make_float2(across(t), across(t + 32));
+    return make_float2(across(t), across(t + WARPS));
   }
 };
 
 // Column factors of the team: k = bs act(g) w_post (the gate only where it is the columns'), w = w_pre.
-template <int NCH, bool VEC>
+template <int NCH, int LAY>
 __device__ __forceinline__ void load_factors(const NormArgs& a, int64_t group, int tid, int team, V8 (&k)[NCH],
                                              V8 (&w)[NCH]) {
 #pragma unroll
@@ -265,7 +386,7 @@ __device__ __forceinline__ void load_factors(const NormArgs& a, int64_t group, i
     float kf[8], wf[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int c = col_of<VEC>(j, i, tid, team);
+      const int c = col_of<LAY>(j, i, tid, team);
       const bool in = c < a.cols;
       float f = in ? a.branch_scale : 0.f;
       if (in && a.post_weight != nullptr) f *= __ldg(a.post_weight + c);
@@ -293,160 +414,211 @@ struct TeamPlan {
 template <typename TX, typename TU, int NCH>
 struct Slots {
   static constexpr uint32_t x = 0, px = NCH * sizeof(TX) / 2, pu = NCH * sizeof(TU) / 2;
-  static constexpr uint32_t u = px, gate = px + pu, dy = px + 2 * pu, dh = 2 * px + 2 * pu;
-  static constexpr uint32_t forward = px + 2 * pu, backward = 2 * px + 3 * pu;
+  static constexpr uint32_t u = px, dy = px + pu, dh = 2 * px + pu, gate_b = 2 * px + 2 * pu;
+  static constexpr uint32_t gate = px + pu, forward = px + 2 * pu, plain = 2 * px + 2 * pu, backward = 2 * px + 3 * pu;
 };
 
+constexpr int kBwdCtas = 3;  // of the backward's small teams, resident together
+
+// Warps of the largest team.
+template <int NCH>
+constexpr int kTeamWarps = NCH == 1 ? 8 : 16;
+
 // What a team works on: its place in the CTA, its rows and the rows ahead.
-template <int NCH, bool VEC>
+template <int NCH, int LAY>
 struct Team {
   int team, tid;
-  int64_t id, group, end;
-  TeamSum sum;
-  Ahead<NCH, VEC> ahead;
+  int64_t id, group;
+  uint32_t row;  // the first
+  int rows;
+  TeamSum<kTeamWarps<NCH>> sum;
+  Ahead<NCH, LAY> ahead;
   __device__ __forceinline__ Team(const NormArgs& a, const TeamPlan& plan, char* smem, float* buf, uint32_t pieces) {
     const bool warp_team = a.cols <= 256;
     team = warp_team ? 32 : int(blockDim.x);
     tid = warp_team ? int(threadIdx.x & 31) : int(threadIdx.x);
     id = warp_team ? int64_t(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5) : int64_t(blockIdx.x);
     group = id / plan.parts;
-    end = (group + 1) * plan.group_rows;
-    sum = TeamSum{warp_team ? nullptr : buf, int(blockDim.x >> 5), 0};
-    ahead = Ahead<NCH, VEC>{smem + threadIdx.x * 16, blockDim.x * 16, blockDim.x * 16 * pieces, plan.depth, 0};
+    sum = TeamSum<kTeamWarps<NCH>>{warp_team ? nullptr : buf, 0};
+    if (!warp_team) {
+      for (int i = threadIdx.x; i < 6 * kTeamWarps<NCH>; i += blockDim.x) buf[i] = 0.f;
+      __syncthreads();
+    }
+    ahead.mine = uint32_t(__cvta_generic_to_shared(smem)) + threadIdx.x * 16;
+    ahead.stride = blockDim.x * 16;
+    ahead.stage = ahead.stride * pieces;
+    ahead.end = ahead.stage * plan.depth;
+    ahead.slot = 0;
+    ahead.depth = plan.depth;
+    ahead.tid = tid;
+    ahead.team = team;
+    ahead.cols = a.cols;
+#pragma unroll
+    for (int h = 0; h < 2 * NCH; ++h) ahead.in[h] = col_of<LAY>(h >> 1, 4 * (h & 1), tid, team) < a.cols;
+    ahead.clear();
+    const int64_t part = id % plan.parts;
+    row = uint32_t(group * plan.group_rows + part);
+    rows = int((plan.group_rows - part + plan.parts - 1) / plan.parts);
   }
 };
 
-template <typename TX, typename TU, int NCH, bool VEC, bool FULL>
+template <typename TX, typename TU, int NCH, int LAY, bool GATED>
 __global__ void __launch_bounds__(NCH == 1 ? 256 : 512, NCH == 1 ? 3 : 1)
     residual_norm_team_kernel(const NormArgs a, const TeamPlan plan) {
   extern __shared__ __align__(16) char smem[];
-  __shared__ float buf[3 * 64];
+  __shared__ __align__(16) float buf[3 * 2 * kTeamWarps<NCH>];
   using S = Slots<TX, TU, NCH>;
-  Team<NCH, VEC> t(a, plan, smem, buf, FULL ? S::forward : S::gate);
+  Team<NCH, LAY> t(a, plan, smem, buf, GATED ? S::forward : S::gate);
   if (t.id >= plan.teams) return;  // a whole team: no barrier is left behind
   const int tid = t.tid, team = t.team, cols = a.cols;
   V8 k[NCH], w[NCH];
-  load_factors<NCH, VEC>(a, t.group, tid, team, k, w);
+  load_factors<NCH, LAY>(a, t.group, tid, team, k, w);
   const float inv = 1.f / float(cols);
   const bool branch = a.branch != nullptr;
-  const TX* px = static_cast<const TX*>(a.x);
-  const TU* pu = static_cast<const TU*>(a.branch);
-  const TU* pg = static_cast<const TU*>(a.gate);
-  auto fetch = [&](int64_t r, int s) {
-    if (r < t.end) {
-      t.ahead.fetch(px + r * a.ld_x, S::x, s, tid, team, cols);
-      if (branch) t.ahead.fetch(pu + r * a.ld_branch, S::u, s, tid, team, cols);
-      if (FULL) t.ahead.fetch(pg + r * a.ld_gate, S::gate, s, tid, team, cols);
+  Ahead<NCH, LAY>& ahead = t.ahead;
+  uint32_t r = t.row;
+  const uint32_t parts = uint32_t(plan.parts);
+  const int rows = t.rows, depth = plan.depth;
+  // GATED: a gate of rows or elements; the columns' is in k
+  const bool full = GATED && a.gate_mode == kGateFull, by_row = GATED && a.gate_mode == kGateRow;
+  const uint32_t ld_x = uint32_t(a.ld_x * sizeof(TX)), ld_u = uint32_t(a.ld_branch * sizeof(TU));
+  const uint32_t ld_g = uint32_t(a.ld_gate * sizeof(TU)), out_x = uint32_t(cols * sizeof(TX)), out_u = uint32_t(cols * sizeof(TU));
+  auto x_row = [&](uint32_t row) { return row_at(static_cast<const TX*>(a.x), row, ld_x); };
+  auto u_row = [&](uint32_t row) { return row_at(static_cast<const TU*>(a.branch), row, ld_u); };
+  auto g_row = [&](uint32_t row) { return row_at(static_cast<const TU*>(a.gate), row, ld_g); };
+  auto fetch = [&](bool there, uint32_t row, uint32_t to) {
+    if (there) {
+      ahead.fetch(x_row(row), S::x, to);
+      if (branch) ahead.fetch(u_row(row), S::u, to);
+      if (full) ahead.fetch(g_row(row), S::gate, to);
     }
-    t.ahead.commit();
+    ahead.commit();
   };
-  int64_t r = t.group * plan.group_rows + t.id % plan.parts;
-  for (int s = 0; s < plan.depth; ++s) fetch(r + s * plan.parts, s);
-  for (; r < t.end; r += plan.parts) {
-    t.ahead.wait();
+  float g1 = by_row ? load_f(a.gate, a.gate_dtype, r) : 1.f;
+  for (int s = 0; s < depth; ++s) fetch(s < rows, r + s * parts, s * ahead.stage);
+  for (int n = 0; n < rows; ++n, r += parts) {
+    ahead.wait();
     V8 y[NCH], f[NCH];
     float ru = 1.f, s = 0.f;
 #pragma unroll
     for (int j = 0; j < NCH; ++j) {
-      y[j] = t.ahead.take(px + r * a.ld_x, S::x, j, tid, team, cols);
+      y[j] = ahead.take(x_row(r), S::x, j);
       if (!branch) continue;
-      const V8 u = t.ahead.take(pu + r * a.ld_branch, S::u, j, tid, team, cols);
-      f[j] = mul(u, k[j]);
-      if (FULL) {
-        const V8 g = t.ahead.take(pg + r * a.ld_gate, S::gate, j, tid, team, cols);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          f[j].p[i] = fmul2(f[j].p[i], f2pack(act_of(g.get(2 * i), a.gate_act), act_of(g.get(2 * i + 1), a.gate_act)));
-      }
-      s += total(mul(u, u));
+      const V8 v = ahead.take(u_row(r), S::u, j);
+      f[j] = mul(v, k[j]);
+      if (full) f[j] = mul(f[j], act8(ahead.take(g_row(r), S::gate, j), a.gate_act));
+      s += dot8(v, v);
     }
-    const float gate = a.gate_mode == kGateRow ? act_of(load_f(a.gate, a.gate_dtype, r), a.gate_act) : 1.f;
-    fetch(r + plan.depth * plan.parts, t.ahead.slot);
-    t.ahead.next();
+    const float gate = by_row ? act_of(g1, a.gate_act) : 1.f;
+    if (by_row && n + 1 < rows) g1 = load_f(a.gate, a.gate_dtype, r + parts);
+    fetch(n + depth < rows, r + depth * parts, ahead.slot);
+    ahead.next();
     if (branch) {
       if (a.post_weight != nullptr) ru = rsqrtf(t.sum.one(s) * inv + a.eps);
       const float scale = ru * gate;
 #pragma unroll
       for (int j = 0; j < NCH; ++j) {
         y[j] = fma(f[j], scale, mul(y[j], a.residual_scale));
-        store8<TX, VEC>(static_cast<TX*>(a.stream_out) + r * cols, y[j], j, tid, team, cols);
+        store8<TX, LAY>(row_at(static_cast<TX*>(a.stream_out), r, out_x), y[j], j, tid, team, cols);
       }
     }
     float ry = 1.f;
     if (a.pre_weight != nullptr) {
       s = 0.f;
 #pragma unroll
-      for (int j = 0; j < NCH; ++j) s += total(mul(y[j], y[j]));
+      for (int j = 0; j < NCH; ++j) s += dot8(y[j], y[j]);
       ry = rsqrtf(t.sum.one(s) * inv + a.eps);
 #pragma unroll
       for (int j = 0; j < NCH; ++j)
-        store8<TU, VEC>(static_cast<TU*>(a.norm_out) + r * cols, mul(mul(y[j], ry), w[j]), j, tid, team, cols);
+        store8<TU, LAY>(row_at(static_cast<TU*>(a.norm_out), r, out_u), mul(mul(y[j], ry), w[j]), j, tid, team, cols);
     }
-    if (a.stats != nullptr && tid == 0) *reinterpret_cast<float2*>(a.stats + 2 * r) = make_float2(ru, ry);
+    if (a.stats != nullptr && tid == 0) *row_at(reinterpret_cast<float2*>(a.stats), r, 8u) = make_float2(ru, ry);
   }
 }
 
-template <typename TX, typename TU, int NCH, bool VEC, bool FULL>
-__global__ void __launch_bounds__(NCH == 1 ? 256 : 512, NCH == 1 ? 2 : 1)
+// The columns' factors lie in shared memory behind the rows ahead, each thread's its own, so that
+// the registers hold two column sums and the row (three values a column) alone: 3 CTAs of 256
+// threads an SM instead of 2, and no spills with 16 columns a thread.
+template <typename TX, typename TU, int NCH, int LAY, bool GATED>
+__global__ void __launch_bounds__(NCH == 1 ? 256 : 512, NCH == 1 ? kBwdCtas : 1)
     residual_norm_team_bwd_kernel(const NormArgs a, const TeamPlan plan, float* partial) {
   extern __shared__ __align__(16) char smem[];
-  __shared__ float buf[3 * 64];
+  __shared__ __align__(16) float buf[3 * 2 * kTeamWarps<NCH>];
   using S = Slots<TX, TU, NCH>;
-  Team<NCH, VEC> t(a, plan, smem, buf, S::backward);
+  Team<NCH, LAY> t(a, plan, smem, buf, GATED ? S::backward : S::plain);
   if (t.id >= plan.teams) return;
   const int tid = t.tid, team = t.team, cols = a.cols;
-  V8 k[NCH], w[NCH], acc_pre[NCH], acc_s[NCH];
-  load_factors<NCH, VEC>(a, t.group, tid, team, k, w);
+  Ahead<NCH, LAY>& ahead = t.ahead;
+  V8 acc_pre[NCH], acc_s[NCH];
+  {
+    V8 k[NCH], w[NCH];
+    load_factors<NCH, LAY>(a, t.group, tid, team, k, w);
 #pragma unroll
-  for (int j = 0; j < NCH; ++j) {
-    acc_pre[j].fill(0.f);
-    acc_s[j].fill(0.f);
+    for (int j = 0; j < NCH; ++j) {
+      ahead.keep(2 * j, k[j]);
+      ahead.keep(2 * j + 1, w[j]);
+      acc_pre[j].fill(0.f);
+      acc_s[j].fill(0.f);
+    }
   }
   const float inv = 1.f / float(cols);
   const bool normed = a.d_normed != nullptr, post = a.post_weight != nullptr, branch = a.branch != nullptr;
+  const bool streamed = a.d_stream != nullptr;
   const float rs = branch ? a.residual_scale : 1.f;
-  const TX* px = static_cast<const TX*>(a.x);
-  const TU* pu = static_cast<const TU*>(a.branch);
-  const TU* pg = static_cast<const TU*>(a.gate);
-  const TX* pdy = static_cast<const TX*>(a.d_stream);
-  const TU* pdh = static_cast<const TU*>(a.d_normed);
-  auto fetch = [&](int64_t r, int s) {
-    if (r < t.end) {
+  uint32_t r = t.row;
+  const uint32_t parts = uint32_t(plan.parts);
+  const int rows = t.rows, depth = plan.depth;
+  // GATED: a gate of rows or elements; the columns' is in k
+  const bool full = GATED && a.gate_mode == kGateFull, by_row = GATED && a.gate_mode == kGateRow;
+  const uint32_t ld_x = uint32_t(a.ld_x * sizeof(TX)), ld_u = uint32_t(a.ld_branch * sizeof(TU));
+  const uint32_t ld_g = uint32_t(a.ld_gate * sizeof(TU)), out_x = uint32_t(cols * sizeof(TX)), out_u = uint32_t(cols * sizeof(TU));
+  auto x_row = [&](uint32_t row) { return row_at(static_cast<const TX*>(a.x), row, ld_x); };
+  auto u_row = [&](uint32_t row) { return row_at(static_cast<const TU*>(a.branch), row, ld_u); };
+  auto g_row = [&](uint32_t row) { return row_at(static_cast<const TU*>(a.gate), row, ld_g); };
+  const uint32_t ld_dy = uint32_t(a.ld_d_stream * sizeof(TX)), ld_dh = uint32_t(a.ld_d_normed * sizeof(TU));
+  auto dy_row = [&](uint32_t row) { return row_at(static_cast<const TX*>(a.d_stream), row, ld_dy); };
+  auto dh_row = [&](uint32_t row) { return row_at(static_cast<const TU*>(a.d_normed), row, ld_dh); };
+  auto fetch = [&](bool there, uint32_t row, uint32_t to) {
+    if (there) {
       if (normed) {
-        t.ahead.fetch(px + r * a.ld_x, S::x, s, tid, team, cols);
-        t.ahead.fetch(pdh + r * a.ld_d_normed, S::dh, s, tid, team, cols);
+        ahead.fetch(x_row(row), S::x, to);
+        ahead.fetch(dh_row(row), S::dh, to);
       }
-      if (branch) t.ahead.fetch(pu + r * a.ld_branch, S::u, s, tid, team, cols);
-      if (FULL) t.ahead.fetch(pg + r * a.ld_gate, S::gate, s, tid, team, cols);
-      if (pdy != nullptr) t.ahead.fetch(pdy + r * a.ld_d_stream, S::dy, s, tid, team, cols);
+      if (branch) ahead.fetch(u_row(row), S::u, to);
+      if (full) ahead.fetch(g_row(row), S::gate_b, to);
+      if (streamed) ahead.fetch(dy_row(row), S::dy, to);
     }
-    t.ahead.commit();
+    ahead.commit();
   };
-  int64_t r = t.group * plan.group_rows + t.id % plan.parts;
-  for (int s = 0; s < plan.depth; ++s) fetch(r + s * plan.parts, s);
-  for (; r < t.end; r += plan.parts) {
-    float2 st = make_float2(1.f, 1.f);
-    if (a.stats != nullptr) st = __ldg(reinterpret_cast<const float2*>(a.stats + 2 * r));
-    const float a1 = a.gate_mode == kGateRow ? act_of(load_f(a.gate, a.gate_dtype, r), a.gate_act) : 1.f;
-    const float ru = st.x, ry = st.y;
-    t.ahead.wait();
-    V8 z[NCH], uh[NCH], f[NCH];  // dz; u r_u; k with the row's or the element's gate
+  float2 st = make_float2(1.f, 1.f);
+  float g1 = 1.f;
+  auto scalars = [&](uint32_t row) {
+    if (a.stats != nullptr) st = __ldg(row_at(reinterpret_cast<const float2*>(a.stats), row, 8u));
+    if (by_row) g1 = load_f(a.gate, a.gate_dtype, row);
+  };
+  scalars(r);
+  for (int s = 0; s < depth; ++s) fetch(s < rows, r + s * parts, s * ahead.stage);
+  for (int n = 0; n < rows; ++n, r += parts) {
+    const float ru = st.x, ry = st.y, a1 = by_row ? act_of(g1, a.gate_act) : 1.f;
+    if (n + 1 < rows) scalars(r + parts);  // the next row's, a row ahead
+    ahead.wait();
+    V8 z[NCH], uh[NCH], act[NCH];  // dz; u r_u; the element's gate
     if (branch) {
 #pragma unroll
       for (int j = 0; j < NCH; ++j) {
-        uh[j] = mul(t.ahead.take(pu + r * a.ld_branch, S::u, j, tid, team, cols), ru);
-        f[j] = a.gate_mode == kGateRow ? mul(k[j], a1) : k[j];
-        if (FULL) {
-          const V8 g = t.ahead.take(pg + r * a.ld_gate, S::gate, j, tid, team, cols);
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            f[j].p[i] = fmul2(f[j].p[i], f2pack(act_of(g.get(2 * i), a.gate_act), act_of(g.get(2 * i + 1), a.gate_act)));
-        }
+        uh[j] = mul(ahead.take(u_row(r), S::u, j), ru);
+        if (full) act[j] = act8(ahead.take(g_row(r), S::gate_b, j), a.gate_act);
       }
     }
+    // k of a column with the row's or the element's gate
+    auto factor = [&](int j) {
+      V8 k = ahead.kept(2 * j);
+      if (by_row) k = mul(k, a1);
+      return full ? mul(k, act[j]) : k;
+    };
 #pragma unroll
     for (int j = 0; j < NCH; ++j) {
-      if (pdy != nullptr) z[j] = t.ahead.take(pdy + r * a.ld_d_stream, S::dy, j, tid, team, cols);
+      if (streamed) z[j] = ahead.take(dy_row(r), S::dy, j);
       else z[j].fill(0.f);
     }
     if (normed) {
@@ -454,51 +626,39 @@ __global__ void __launch_bounds__(NCH == 1 ? 256 : 512, NCH == 1 ? 2 : 1)
       float dot = 0.f;
 #pragma unroll
       for (int j = 0; j < NCH; ++j) {
-        const V8 x = mul(t.ahead.take(px + r * a.ld_x, S::x, j, tid, team, cols), rs);
-        yh[j] = mul(branch ? fma(f[j], uh[j], x) : x, ry);
-        const V8 d = t.ahead.take(pdh + r * a.ld_d_normed, S::dh, j, tid, team, cols);
+        const V8 v = mul(ahead.take(x_row(r), S::x, j), rs);
+        yh[j] = mul(branch ? fma(factor(j), uh[j], v) : v, ry);
+        const V8 d = ahead.take(dh_row(r), S::dh, j);
         acc_pre[j] = fma(d, yh[j], acc_pre[j]);
-        const V8 dw = mul(d, w[j]);
-        dot += total(mul(dw, yh[j]));
+        const V8 dw = mul(d, ahead.kept(2 * j + 1));
+        dot += dot8(dw, yh[j]);
         z[j] = fma(dw, ry, z[j]);
       }
       const float mean = t.sum.one(dot) * (inv * ry);
 #pragma unroll
       for (int j = 0; j < NCH; ++j) z[j] = fma(yh[j], -mean, z[j]);
     }
-    float dot_u = 0.f, dot_g = 0.f;
-    if (branch) {
-#pragma unroll
-      for (int j = 0; j < NCH; ++j) {
-        const V8 zu = mul(z[j], uh[j]);
-        if (post) dot_u += total(mul(f[j], zu));
-        if (a.gate_mode == kGateRow) dot_g += total(mul(k[j], zu));
-        if (FULL) {
-          const V8 g = t.ahead.take(pg + r * a.ld_gate, S::gate, j, tid, team, cols);
-          V8 dg = mul(k[j], zu), act;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float g0 = act_of(g.get(2 * i), a.gate_act), g1 = act_of(g.get(2 * i + 1), a.gate_act);
-            act.p[i] = f2pack(g0, g1);
-            dg.p[i] = fmul2(dg.p[i], f2pack(act_slope(g0, a.gate_act), act_slope(g1, a.gate_act)));
-          }
-          acc_s[j] = fma(act, zu, acc_s[j]);
-          if (a.d_gate != nullptr) store8<TU, VEC>(static_cast<TU*>(a.d_gate) + r * cols, dg, j, tid, team, cols);
-        } else {
-          acc_s[j] = fma(zu, a1, acc_s[j]);
-        }
-      }
-    }
-    fetch(r + plan.depth * plan.parts, t.ahead.slot);
-    t.ahead.next();
+    fetch(n + depth < rows, r + depth * parts, ahead.slot);
+    ahead.next();
     if (a.d_x != nullptr) {
 #pragma unroll
-      for (int j = 0; j < NCH; ++j)
-        store8<TX, VEC>(static_cast<TX*>(a.d_x) + r * cols, mul(z[j], rs), j, tid, team, cols);
+      for (int j = 0; j < NCH; ++j) store8<TX, LAY>(row_at(static_cast<TX*>(a.d_x), r, out_x), mul(z[j], rs), j, tid, team, cols);
     }
     if (!branch) continue;
+    float dot_u = 0.f, dot_g = 0.f;
+#pragma unroll
+    for (int j = 0; j < NCH; ++j) {
+      const V8 zu = mul(z[j], uh[j]);
+      if (by_row) dot_g += dot8(ahead.kept(2 * j), zu);
+      if (full && a.d_gate != nullptr)
+        store8<TU, LAY>(row_at(static_cast<TU*>(a.d_gate), r, out_u), mul(mul(ahead.kept(2 * j), zu), slope8(act[j], a.gate_act)), j, tid,
+                        team, cols);
+      acc_s[j] = full ? fma(act[j], zu, acc_s[j]) : by_row ? fma(zu, a1, acc_s[j]) : add(zu, acc_s[j]);
+      z[j] = mul(factor(j), z[j]);
+      if (post) dot_u += dot8(z[j], uh[j]);
+    }
     float mean_u = 0.f;
-    if (a.gate_mode == kGateRow) {
+    if (by_row) {
       const float2 s = t.sum.two(dot_u, dot_g);
       mean_u = s.x * inv;
       if (tid == 0 && a.d_gate != nullptr) static_cast<float*>(a.d_gate)[r] = act_slope(a1, a.gate_act) * s.y;
@@ -509,8 +669,7 @@ __global__ void __launch_bounds__(NCH == 1 ? 256 : 512, NCH == 1 ? 2 : 1)
       mean_u = post ? -mean_u * ru : 0.f;
 #pragma unroll
       for (int j = 0; j < NCH; ++j)
-        store8<TU, VEC>(static_cast<TU*>(a.d_branch) + r * cols, fma(uh[j], mean_u, mul(mul(f[j], z[j]), ru)), j, tid, team,
-                        cols);
+        store8<TU, LAY>(row_at(static_cast<TU*>(a.d_branch), r, out_u), fma(uh[j], mean_u, mul(z[j], ru)), j, tid, team, cols);
     }
   }
   if (partial == nullptr) return;
@@ -518,7 +677,7 @@ __global__ void __launch_bounds__(NCH == 1 ? 256 : 512, NCH == 1 ? 2 : 1)
   for (int j = 0; j < NCH; ++j)
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int c = col_of<VEC>(j, i, tid, team);
+      const int c = col_of<LAY>(j, i, tid, team);
       if (c >= cols) continue;
       partial[t.id * cols + c] = acc_pre[j].get(i);
       partial[(plan.teams + t.id) * cols + c] = acc_s[j].get(i);
@@ -721,7 +880,7 @@ int check_norm(const NormArgs* a, bool backward) {
       ((a->d_stream && a->ld_d_stream < a->cols) || (a->d_normed && (!a->pre_weight || a->ld_d_normed < a->cols)) ||
        (!a->stats && (a->post_weight || a->d_normed))))
     return MCL4MOE_ERR_INVALID;
-  if (a->cols > kMaxNormCols) return MCL4MOE_ERR_UNSUPPORTED;
+  if (a->cols > kMaxNormCols || a->rows > (int64_t(1) << 31) - 1) return MCL4MOE_ERR_UNSUPPORTED;
   return MCL4MOE_OK;
 }
 
@@ -736,15 +895,15 @@ struct NormShape {
   int64_t groups;
 };
 
-NormShape norm_shape(int64_t rows, int cols, int gate_mode, int64_t gate_rows, bool backward) {
+NormShape norm_shape(int64_t rows, int cols, int gate_mode, int64_t gate_rows, bool backward, bool wide) {
   NormShape s{};
-  s.wide = cols > 2048;
+  s.wide = wide;
   const int per = s.wide ? 16 : 8;
   const int need = (cols + per - 1) / per;
   s.threads = cols <= 256 ? 128 : (need + 31) / 32 * 32;
   s.rows_per_cta = cols <= 256 ? 4 : 1;
   if (cols > kTeamCols) s.threads = kNormThreads;
-  const int64_t per_sm = cols > kTeamCols ? 512 : s.wide ? 512 : backward ? 512 : 768;
+  const int64_t per_sm = cols > kTeamCols ? 512 : s.wide ? 512 : backward ? 256 * kBwdCtas : 768;
   s.ctas_per_sm = per_sm / s.threads > 0 ? int(per_sm / s.threads) : 1;
   const int64_t want = int64_t(s.ctas_per_sm) * num_sms() * s.rows_per_cta;
   s.groups = gate_mode == kGateChannel ? rows / gate_rows : 1;
@@ -776,6 +935,8 @@ bool norm_vectors(const NormArgs& a) {
 // element-wise gate.  Other mixes and wider rows go through the generic kernels.
 bool norm_in_registers(const NormArgs& a) {
   if (a.cols > kTeamCols || (a.branch && a.branch_dtype != a.norm_dtype)) return false;
+  const int64_t far = int64_t(1) << 30;  // byte strides in 32 bits
+  if (a.ld_x >= far || a.ld_branch >= far || a.ld_gate >= far || a.ld_d_stream >= far || a.ld_d_normed >= far) return false;
   if (a.gate_mode == kGateFull && a.gate_dtype != a.norm_dtype) return false;
   return a.x_dtype == a.norm_dtype || a.x_dtype == 1;
 }
@@ -783,41 +944,53 @@ bool norm_in_registers(const NormArgs& a) {
 // Rows ahead: up to four, as many as the CTAs that are resident at once have room for.
 constexpr int kAheadBytes = 200 * 1024;  // of an SM's shared memory
 
-template <typename TX, typename TU, int NCH, bool VEC, bool FULL>
+// 16 columns a thread: needed from 2049 columns on; from 1025 on where a row has more operands or
+// wider ones, so that the reductions weigh more than the warps in flight (32768 x 2048, forward /
+// backward in us, 8 against 16 columns a thread: bf16 96 / 161 against 103 / 168; float32 stream 149 / 232
+// against 138 / 215; element-wise gate 134 / 285 against 117 / 232). Single elements stay narrow
+// (32768 x 1001: 90 / 254 against 114 / 293).
+bool norm_wide(const NormArgs& a) {
+  if (a.cols > 2048 || a.cols <= 1024) return a.cols > 2048;
+  return norm_vectors(a) && (a.x_dtype == 1 || a.gate_mode >= kGateRow);
+}
+
+template <typename TX, typename TU, int NCH, int LAY, bool GATED>
 int launch_team(const NormArgs& a, NormShape s, bool backward, float* partial, cudaStream_t stream) {
   using S = Slots<TX, TU, NCH>;
-  const int stage = s.threads * 16 * int(backward ? S::backward : FULL ? S::forward : S::gate);
-  int depth = kAheadBytes / s.ctas_per_sm / stage;
+  const int stage = s.threads * 16 * int(backward ? (GATED ? S::backward : S::plain) : GATED ? S::forward : S::gate);
+  const int kept = backward ? s.threads * 16 * 4 * NCH : 0;
+  int depth = (kAheadBytes / s.ctas_per_sm - kept) / stage;
   depth = depth > 4 ? 4 : depth < 1 ? 1 : depth;
-  const int smem = VEC ? depth * stage : 0;
-  s.plan.depth = VEC ? depth : 0;
+  const int smem = kept + (LAY != kSingles ? depth * stage : 0);
+  s.plan.depth = LAY != kSingles ? depth : 0;
   const unsigned grid = unsigned((s.plan.teams + s.rows_per_cta - 1) / s.rows_per_cta);
   if (backward) {
     static std::atomic<uint64_t> raised{0};
-    if (VEC && !raise_smem_limit(residual_norm_team_bwd_kernel<TX, TU, NCH, VEC, FULL>, 220 * 1024, raised))
+    if (!raise_smem_limit(residual_norm_team_bwd_kernel<TX, TU, NCH, LAY, GATED>, 220 * 1024, raised))
       return MCL4MOE_ERR_CUDA;
-    residual_norm_team_bwd_kernel<TX, TU, NCH, VEC, FULL><<<grid, s.threads, smem, stream>>>(a, s.plan, partial);
+    residual_norm_team_bwd_kernel<TX, TU, NCH, LAY, GATED><<<grid, s.threads, smem, stream>>>(a, s.plan, partial);
   } else {
     static std::atomic<uint64_t> raised{0};
-    if (VEC && !raise_smem_limit(residual_norm_team_kernel<TX, TU, NCH, VEC, FULL>, 220 * 1024, raised))
+    if (LAY != kSingles && !raise_smem_limit(residual_norm_team_kernel<TX, TU, NCH, LAY, GATED>, 220 * 1024, raised))
       return MCL4MOE_ERR_CUDA;
-    residual_norm_team_kernel<TX, TU, NCH, VEC, FULL><<<grid, s.threads, smem, stream>>>(a, s.plan);
+    residual_norm_team_kernel<TX, TU, NCH, LAY, GATED><<<grid, s.threads, smem, stream>>>(a, s.plan);
   }
   return MCL4MOE_OK;
 }
-template <typename TX, typename TU, int NCH, bool VEC>
+template <typename TX, typename TU, int NCH, int LAY>
 int launch_team(const NormArgs& a, const NormShape& s, bool backward, float* partial, cudaStream_t stream) {
-  return a.gate_mode == kGateFull ? launch_team<TX, TU, NCH, VEC, true>(a, s, backward, partial, stream)
-                                  : launch_team<TX, TU, NCH, VEC, false>(a, s, backward, partial, stream);
+  return a.gate_mode >= kGateRow ? launch_team<TX, TU, NCH, LAY, true>(a, s, backward, partial, stream)
+                                 : launch_team<TX, TU, NCH, LAY, false>(a, s, backward, partial, stream);
 }
 template <typename TX, typename TU>
 int launch_team(const NormArgs& a, const NormShape& s, bool backward, float* partial, cudaStream_t stream) {
+  constexpr int kLay = sizeof(TX) == 4 ? kFours : kEights;
   const bool vec = norm_vectors(a);
   if (s.wide)
-    return vec ? launch_team<TX, TU, 2, true>(a, s, backward, partial, stream)
-               : launch_team<TX, TU, 2, false>(a, s, backward, partial, stream);
-  return vec ? launch_team<TX, TU, 1, true>(a, s, backward, partial, stream)
-             : launch_team<TX, TU, 1, false>(a, s, backward, partial, stream);
+    return vec ? launch_team<TX, TU, 2, kLay>(a, s, backward, partial, stream)
+               : launch_team<TX, TU, 2, kSingles>(a, s, backward, partial, stream);
+  return vec ? launch_team<TX, TU, 1, kLay>(a, s, backward, partial, stream)
+             : launch_team<TX, TU, 1, kSingles>(a, s, backward, partial, stream);
 }
 int launch_teams(const NormArgs& a, const NormShape& s, bool backward, float* partial, cudaStream_t stream) {
   if (a.x_dtype == 1) {
@@ -840,7 +1013,7 @@ int mcl4moe_residual_norm(const mcl4moe_norm_args* a, mcl4moe_stream_t stream) {
   const int st = check_norm(a, false);
   if (st != MCL4MOE_OK) return st;
   if (a->rows == 0) return MCL4MOE_OK;
-  const NormShape s = norm_shape(a->rows, a->cols, a->gate_mode, a->gate_rows, false);
+  const NormShape s = norm_shape(a->rows, a->cols, a->gate_mode, a->gate_rows, false, norm_wide(*a));
   if (s.plan.teams > (int64_t(1) << 30)) return MCL4MOE_ERR_UNSUPPORTED;
   if (norm_in_registers(*a)) {
     const int team = launch_teams(*a, s, false, nullptr, stream);
@@ -854,8 +1027,13 @@ int mcl4moe_residual_norm(const mcl4moe_norm_args* a, mcl4moe_stream_t stream) {
 
 size_t mcl4moe_residual_norm_workspace_size(int64_t rows, int cols, int gate_mode, int64_t gate_rows) {
   if (rows <= 0 || cols <= 0 || cols > kMaxNormCols || (gate_mode == kGateChannel && gate_rows <= 0)) return 0;
-  const NormShape s = norm_shape(rows, cols, gate_mode, gate_rows, true);
-  return size_t(2 * s.plan.teams + (s.groups > 1 ? s.groups : 0)) * size_t(cols) * sizeof(float);
+  int64_t teams = 0, groups = 0;  // of either width of the teams
+  for (int wide = cols > 2048; wide < 2; ++wide) {
+    const NormShape s = norm_shape(rows, cols, gate_mode, gate_rows, true, wide != 0);
+    teams = s.plan.teams > teams ? s.plan.teams : teams;
+    groups = s.groups;
+  }
+  return size_t(2 * teams + (groups > 1 ? groups : 0)) * size_t(cols) * sizeof(float);
 }
 
 int mcl4moe_residual_norm_backward(const mcl4moe_norm_args* a, void* workspace, size_t workspace_bytes,
@@ -869,7 +1047,7 @@ int mcl4moe_residual_norm_backward(const mcl4moe_norm_args* a, void* workspace, 
       return MCL4MOE_ERR_CUDA;
     return MCL4MOE_OK;
   }
-  const NormShape s = norm_shape(a->rows, a->cols, a->gate_mode, a->gate_rows, true);
+  const NormShape s = norm_shape(a->rows, a->cols, a->gate_mode, a->gate_rows, true, norm_wide(*a));
   if (s.plan.teams > (int64_t(1) << 30) || s.groups > 65533) return MCL4MOE_ERR_UNSUPPORTED;
   if (sums && (!workspace || workspace_bytes < mcl4moe_residual_norm_workspace_size(a->rows, a->cols, a->gate_mode,
                                                                                     a->gate_rows)))
