@@ -14,6 +14,7 @@
 // The noise is Philox4x32 with 7 rounds, counter (element / 4, tensor, step), key the seed: the
 // upper half of an element's word rounds m, the lower half v.
 #include <cmath>
+#include <type_traits>
 
 #include <cuda_fp16.h>
 
@@ -22,21 +23,22 @@
 namespace mcl4 {
 namespace {
 
-constexpr int kAdamBlock = 256;                 // elements that share a scale; one warp's share at a time
+constexpr int kAdamBlock = 256;    // elements that share a scale; one warp's share at a time
 constexpr int kAdamThreads = 256;
-constexpr int64_t kAdamChunk = 32 * kAdamBlock;  // elements of a CTA
+constexpr int kAdamPass = kAdamThreads / 32 * kAdamBlock;  // elements of a CTA's pass: a block for each warp
+constexpr int kAdamCtas = 3;                    // resident on an SM
 
 struct AdamHyper {
-  float beta1, beta2, one_minus_beta1, one_minus_beta2, eps, lr, weight_decay;
+  float beta1, beta2, one_minus_beta1, one_minus_beta2, eps;
   float step_size;  // lr / (1 - beta1^t)
   float decay;      // 1 - lr * weight_decay
   float inv_root;   // 1 / sqrt(1 - beta2^t)
-  double beta1_d, beta2_d;
+  double beta1_d, beta2_d, lr, weight_decay;
   const int64_t* step_dev;  // or nullptr: the values above hold
   const float* lr_dev;
   const float* grad_scale;
   uint32_t step;
-  uint32_t seed_lo, seed_hi;
+  uint32_t keys[14];  // Philox's key of each round
 };
 
 template <int N>
@@ -51,7 +53,9 @@ struct AdamTable {
   int64_t numel[N];
   int32_t first[N + 1];  // first chunk of each tensor
   int32_t index[N];      // the tensor's number in the noise counter
+  uint8_t wide[N];       // its arrays allow accesses of four elements
   int32_t n;
+  int32_t passes;        // of a CTA's turn
 };
 
 template <typename T>
@@ -72,67 +76,131 @@ __device__ __forceinline__ void from_f(float& d, float v) { d = v; }
 __device__ __forceinline__ void from_f(uint16_t& d, float v) { d = f32_to_bf16(v); }
 __device__ __forceinline__ void from_f(__half& d, float v) { d = __float2half_rn(v); }
 
-// Four consecutive elements: one vector access where all four exist and the address allows it.
+// Four consecutive elements, by one access or (`count` of them) singly.
 template <typename T>
 struct __align__(4 * sizeof(T)) Four {
   T v[4];
 };
-template <typename T>
-__device__ __forceinline__ Four<T> load4(const T* p, int count, bool wide) {
-  Four<T> r;
-  if (wide && count == 4) return *reinterpret_cast<const Four<T>*>(p);
+template <bool WHOLE, typename T>
+__device__ __forceinline__ Four<T> load4(const T* p, int count) {
+  if constexpr (WHOLE) {
+    return *reinterpret_cast<const Four<T>*>(p);
+  } else {
+    Four<T> r;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) r.v[i] = i < count ? p[i] : T(0);
-  return r;
-}
-template <typename T>
-__device__ __forceinline__ void store4(T* p, const Four<T>& r, int count, bool wide) {
-  if (wide && count == 4) {
-    *reinterpret_cast<Four<T>*>(p) = r;
-    return;
+    for (int i = 0; i < 4; ++i) r.v[i] = i < count ? p[i] : T(0);
+    return r;
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (i < count) p[i] = r.v[i];
 }
+template <bool WHOLE, typename T>
+__device__ __forceinline__ void store4(T* p, const Four<T>& r, int count) {
+  if constexpr (WHOLE) {
+    *reinterpret_cast<Four<T>*>(p) = r;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < count) p[i] = r.v[i];
+  }
+}
+
+template <int BYTES>
+__device__ __forceinline__ void copy_ahead(void* to, const void* from) {
+  const uint32_t at = uint32_t(__cvta_generic_to_shared(to));
+  if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(from) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(at), "l"(from), "n"(BYTES == 16 ? 4 : BYTES) : "memory");
+}
+
+__device__ __forceinline__ uint32_t word4(const Four<uint8_t>& b) { return *reinterpret_cast<const uint32_t*>(&b); }
+__device__ __forceinline__ Four<uint8_t> bytes4(uint32_t w) { return *reinterpret_cast<const Four<uint8_t>*>(&w); }
 
 // Philox4x32 (Salmon, Moraes, Dror, Shaw, "Parallel random numbers: as easy as 1, 2, 3", SC'11),
 // 7 rounds, the fewest that the paper found to pass BigCrush.
-__device__ __forceinline__ uint4 philox7(uint32_t c0, uint32_t c1, uint32_t c2, uint32_t c3, uint32_t k0, uint32_t k1) {
+__device__ __forceinline__ uint4 philox7(uint32_t c0, uint32_t c1, uint32_t c2, uint32_t c3, const uint32_t (&keys)[14]) {
 #pragma unroll
   for (int r = 0; r < 7; ++r) {
     const uint64_t a = uint64_t(0xD2511F53u) * c0, b = uint64_t(0xCD9E8D57u) * c2;
-    c0 = uint32_t(b >> 32) ^ c1 ^ k0;
+    c0 = uint32_t(b >> 32) ^ c1 ^ keys[2 * r];
     c1 = uint32_t(b);
-    c2 = uint32_t(a >> 32) ^ c3 ^ k1;
+    c2 = uint32_t(a >> 32) ^ c3 ^ keys[2 * r + 1];
     c3 = uint32_t(a);
-    k0 += 0x9E3779B9u;
-    k1 += 0xBB67AE85u;
   }
   return make_uint4(c0, c1, c2, c3);
 }
 
 __device__ __forceinline__ float pow2f(int e) { return __uint_as_float(uint32_t(e + 127) << 23); }
-__device__ __forceinline__ bool finite(float v) { return (__float_as_uint(v) & 0x7F800000u) != 0x7F800000u; }
 
 // 8-bit float with MANT mantissa bits and exponent bias BIAS of x * inv, rounded up where the
-// dropped part plus noise / 2^16 reaches a step; NaN where x is not finite.
-template <int MANT, int BIAS>
+// dropped part plus noise / 2^16 reaches a step; NaN where x is not finite.  A block's values lie
+// below 2^(TOP + 1).
+//   * In the type's normal range the bits themselves are the sum's fixed point: the noise goes onto
+//     the dropped bits and carries into the kept ones.  round8_normal returns that code less
+//     1 << MANT, and tells of values outside the range.
+//   * Below it (2^-13 of the block's largest for e4m3, 2^-28 for e5m2) the step is fixed and the
+//     sum is taken in float32: round8, for all.
+template <int MANT, int BIAS, int TOP>
+__device__ __forceinline__ uint32_t round8_normal(float x, float inv, uint32_t noise, bool& outside) {
+  constexpr uint32_t kLow = uint32_t(128 - BIAS) << 23, kRange = uint32_t(TOP + BIAS) << 23;
+  const uint32_t over = __float_as_uint(__fmul_rn(fabsf(x), inv)) - kLow;
+  outside |= over >= kRange;
+  return (over + (noise << (7 - MANT))) >> (23 - MANT);
+}
+template <int MANT, int BIAS, int TOP>
 __device__ __forceinline__ uint32_t round8(float x, float inv, uint32_t noise) {
-  const uint32_t sign = (__float_as_uint(x) >> 31) << 7;
-  if (!finite(x)) return 0x7Fu | sign;
+  bool outside = false;
+  const uint32_t code = round8_normal<MANT, BIAS, TOP>(x, inv, noise, outside) + (1u << MANT);
+  if (!outside) return code;
+  if ((__float_as_uint(x) & 0x7F800000u) == 0x7F800000u) return 0x7Fu;
   const float a = __fmul_rn(fabsf(x), inv);
-  int e = int(__float_as_uint(a) >> 23) - 127;  // binade; denormals and 0 end up below the smallest
-  e = e < 1 - BIAS ? 1 - BIAS : e;
-  const float steps = floorf(__fadd_rn(__fmul_rn(a, pow2f(MANT - e)), __fmul_rn(float(noise), 1.52587890625e-05f)));
-  return ((uint32_t(e + BIAS) << MANT) + uint32_t(steps) - (1u << MANT)) | sign;
+  return uint32_t(__fadd_rn(__fmul_rn(a, float(1 << (MANT + BIAS - 1))), __fmul_rn(float(noise), 1.52587890625e-05f)));
 }
-__device__ __forceinline__ float e4m3_value(uint32_t c) {
-  const float v = (c & 0x7Fu) == 0x7Fu ? __uint_as_float(0x7FC00000u) : e4m3_to_f32(c & 0x7Fu);
-  return c & 0x80u ? -v : v;
+
+__device__ __forceinline__ uint32_t pack4(const uint32_t (&b)[4]) {
+  return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
 }
-__device__ __forceinline__ float e5m2_value(uint32_t c) {  // the upper byte of a half
-  return __half2float(__ushort_as_half(static_cast<unsigned short>(c << 8)));
+
+// The codes of four moments of either kind where one of them is outside its type's normal range: rare,
+// so its registers stay out of the caller.
+__device__ __noinline__ uint2 round_any(float4 m, float4 v, float m_inv, float v_inv, uint4 word) {
+  const float mf[4] = {m.x, m.y, m.z, m.w}, vf[4] = {v.x, v.y, v.z, v.w};
+  const uint32_t w[4] = {word.x, word.y, word.z, word.w};
+  uint32_t mc[4], vc[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    mc[i] = round8<3, 7, 7>(mf[i], m_inv, w[i] >> 16);
+    vc[i] = round8<2, 15, 14>(vf[i], v_inv, w[i] & 0xFFFFu);
+  }
+  return make_uint2(pack4(mc), pack4(vc));
+}
+
+// Four e4m3 / e5m2 codes of one word, by the hardware's conversion to halves.
+__device__ __forceinline__ void e4m3x4(uint32_t w, float (&v)[4]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint32_t r;
+    asm("{ .reg .b16 t; cvt.u16.u32 t, %1; cvt.rn.f16x2.e4m3x2 %0, t; }" : "=r"(r) : "r"(w >> (16 * h)));
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r));
+    v[2 * h] = f.x;
+    v[2 * h + 1] = f.y;
+  }
+}
+__device__ __forceinline__ void e5m2x4(uint32_t w, float (&v)[4]) {  // a code is the upper byte of its half
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint32_t r = __byte_perm(w, 0u, h ? 0x3424 : 0x1404);
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r));
+    v[2 * h] = f.x;
+    v[2 * h + 1] = f.y;
+  }
+}
+
+// The update's m / (sqrt(v) inv_root + eps), within 2^-21: its rounding ends up far below the
+// parameter's own.
+__device__ __forceinline__ float adam_ratio(float m, float v, float inv_root, float eps) {
+  float root;
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(root) : "f"(v));
+  float inv;  // the flush to zero of a denormal denominator meets eps = 0 and v = 0 alone
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(root * inv_root + eps));
+  return m * inv;
 }
 
 // The power of two that puts the block's largest finite magnitude into binade TOP, and its inverse.
@@ -145,146 +213,326 @@ __device__ __forceinline__ void block_scale(uint32_t largest_bits, float& scale,
   inv = pow2f(TOP - e);
 }
 
-template <typename P, typename G, bool EIGHT, int N>
-__global__ void __launch_bounds__(kAdamThreads) adamw_kernel(const __grid_constant__ AdamTable<N> tab,
-                                                             const AdamHyper h0) {
-  AdamHyper h = h0;
-  if (h.step_dev != nullptr || h.lr_dev != nullptr) {
-    __shared__ float dev[4];
-    if (threadIdx.x == 0) {
-      const int64_t step = h.step_dev != nullptr ? *h.step_dev : int64_t(h.step);
-      const double lr = h.lr_dev != nullptr ? double(*h.lr_dev) : double(h.lr);
-      dev[0] = float(lr / (1.0 - pow(h.beta1_d, double(step))));
-      dev[1] = float(1.0 - lr * double(h.weight_decay));
-      dev[2] = float(1.0 / sqrt(1.0 - pow(h.beta2_d, double(step))));
-      dev[3] = __uint_as_float(uint32_t(step));
-    }
-    __syncthreads();
-    h.step_size = dev[0];
-    h.decay = dev[1];
-    h.inv_root = dev[2];
-    h.step = __float_as_uint(dev[3]);
-  }
-  int lo = 0, hi = tab.n - 1;  // the last tensor whose first chunk is not behind this one
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (tab.first[mid] <= int(blockIdx.x)) lo = mid;
-    else hi = mid - 1;
-  }
-  const int t = lo;
-  const int64_t numel = tab.numel[t];
-  const int64_t begin = int64_t(int(blockIdx.x) - tab.first[t]) * kAdamChunk;
-  const int64_t end = begin + kAdamChunk < numel ? begin + kAdamChunk : numel;
-  P* p = static_cast<P*>(tab.p[t]);
-  const G* g = static_cast<const G*>(tab.g[t]);
-  float* master = tab.master[t];
-  const bool wide_p = (reinterpret_cast<uintptr_t>(p) & (4 * sizeof(P) - 1)) == 0;
-  const bool wide_g = (reinterpret_cast<uintptr_t>(g) & (4 * sizeof(G) - 1)) == 0;
-  const bool wide_w = (reinterpret_cast<uintptr_t>(master) & 15) == 0;
-  const int state = EIGHT ? 1 : 4;
-  const bool wide_s =
-      ((reinterpret_cast<uintptr_t>(tab.m[t]) | reinterpret_cast<uintptr_t>(tab.v[t])) & (4 * state - 1)) == 0;
-  const float grad_scale = h.grad_scale != nullptr ? *h.grad_scale : 1.f;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int64_t base = begin + warp * kAdamBlock; base < end; base += kAdamThreads / 32 * kAdamBlock) {
-    float m[2][4], v[2][4];
-    uint32_t m_top = 0, v_top = 0;
-    float ms = 1.f, vs = 1.f;
-    if (EIGHT) {
-      ms = tab.ms[t][base / kAdamBlock];
-      vs = tab.vs[t][base / kAdamBlock];
-    }
+// What a warp needs of a tensor: its arrays from the CTA's first element of this turn on.
+template <typename P, typename G, bool EIGHT, bool MASTER>
+struct AdamTensor {
+  using S = typename std::conditional<EIGHT, uint8_t, float>::type;
+  P* p;
+  const G* g;
+  S* m;
+  S* v;
+  float* master;
+};
+
+// A lane's elements of a block, 2 x 4, as they were.
+template <typename P, typename G, bool EIGHT, bool MASTER>
+struct AdamRaw {
+  using S = typename AdamTensor<P, G, EIGHT, MASTER>::S;
+  Four<G> g[2];
+  Four<P> p[2];
+  Four<float> w[2];
+  Four<S> m[2], v[2];
+  float ms, vs;
+};
+
+template <bool WHOLE, typename P, typename G, bool EIGHT, bool MASTER>
+__device__ __forceinline__ AdamRaw<P, G, EIGHT, MASTER> adam_load(const AdamTensor<P, G, EIGHT, MASTER>& t, int off, int left,
+                                                                  const float* scale_m, const float* scale_v) {
+  const int lane = threadIdx.x & 31;
+  AdamRaw<P, G, EIGHT, MASTER> r;
+  r.ms = EIGHT ? *scale_m : 1.f;
+  r.vs = EIGHT ? *scale_v : 1.f;
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      const int64_t at = base + q * 128 + lane * 4;
-      const int count = at >= end ? 0 : end - at >= 4 ? 4 : int(end - at);
-      if (count == 0) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) m[q][i] = v[q][i] = 0.f;
-        continue;
+  for (int q = 0; q < 2; ++q) {
+    const int at = off + q * 128 + lane * 4;
+    const int count = WHOLE ? 4 : max(0, min(4, left - q * 128 - lane * 4));
+    r.g[q] = load4<WHOLE>(t.g + at, count);
+    if (MASTER) r.w[q] = load4<WHOLE>(t.master + at, count);
+    else r.p[q] = load4<WHOLE>(t.p + at, count);
+    r.m[q] = load4<WHOLE>(t.m + at, count);
+    r.v[q] = load4<WHOLE>(t.v + at, count);
+  }
+  return r;
+}
+
+// The step's factors: those of the launch, or taken from the device's step count and rate.
+struct AdamFactors {
+  float step_size, decay, inv_root, grad_scale;
+  uint32_t step;
+  __device__ __forceinline__ explicit AdamFactors(const AdamHyper& h) {
+    step_size = h.step_size;
+    decay = h.decay;
+    inv_root = h.inv_root;
+    step = h.step;
+    if (h.step_dev != nullptr || h.lr_dev != nullptr) {
+      __shared__ float dev[4];
+      if (threadIdx.x == 0) {
+        const int64_t now = h.step_dev != nullptr ? *h.step_dev : int64_t(h.step);
+        const double lr = h.lr_dev != nullptr ? double(*h.lr_dev) : h.lr;
+        dev[0] = float(lr / (1.0 - pow(h.beta1_d, double(now))));
+        dev[1] = float(1.0 - lr * h.weight_decay);
+        dev[2] = float(1.0 / sqrt(1.0 - pow(h.beta2_d, double(now))));
+        dev[3] = __uint_as_float(uint32_t(now));
       }
-      const Four<G> g4 = load4(g + at, count, wide_g);
-      Four<P> p4 = load4(p + at, count, wide_p);
-      Four<float> w4;
-      if (master != nullptr) w4 = load4(master + at, count, wide_w);
-      if (EIGHT) {
-        const Four<uint8_t> mc = load4(static_cast<const uint8_t*>(tab.m[t]) + at, count, wide_s);
-        const Four<uint8_t> vc = load4(static_cast<const uint8_t*>(tab.v[t]) + at, count, wide_s);
+      __syncthreads();
+      step_size = dev[0];
+      decay = dev[1];
+      inv_root = dev[2];
+      step = __float_as_uint(dev[3]);
+    }
+    grad_scale = h.grad_scale != nullptr ? *h.grad_scale : 1.f;
+  }
+};
+
+// One block of 256 elements.  WHOLE: all 256 are there and lie on vector addresses.
+template <bool WHOLE, typename P, typename G, bool EIGHT, bool MASTER>
+__device__ __forceinline__ void adam_block(const AdamTensor<P, G, EIGHT, MASTER>& t, AdamRaw<P, G, EIGHT, MASTER>& r, int off,
+                                           int left, float* scale_m, float* scale_v, int64_t element, int32_t index,
+                                           const AdamHyper& h, const AdamFactors& f) {
+  const int lane = threadIdx.x & 31;
+  int count[2] = {4, 4};
+  if (!WHOLE)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          m[q][i] = __fmul_rn(e4m3_value(mc.v[i]), ms);
-          v[q][i] = __fmul_rn(e5m2_value(vc.v[i]), vs);
-        }
+    for (int q = 0; q < 2; ++q) count[q] = max(0, min(4, left - q * 128 - lane * 4));
+  float m[2][4], v[2][4];
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const int at = off + q * 128 + lane * 4;
+    if constexpr (EIGHT) {
+      e4m3x4(word4(r.m[q]), m[q]);
+      e5m2x4(word4(r.v[q]), v[q]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float gr = __fmul_rn(to_f(r.g[q].v[i]), f.grad_scale);
+      if constexpr (EIGHT) {
+        m[q][i] = __fmul_rn(m[q][i], r.ms);
+        v[q][i] = __fmul_rn(v[q][i], r.vs);
       } else {
-        const Four<float> m4 = load4(static_cast<const float*>(tab.m[t]) + at, count, wide_s);
-        const Four<float> v4 = load4(static_cast<const float*>(tab.v[t]) + at, count, wide_s);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          m[q][i] = m4.v[i];
-          v[q][i] = v4.v[i];
-        }
+        m[q][i] = r.m[q].v[i];
+        v[q][i] = r.v[q].v[i];
       }
+      // each product and sum rounded by itself: the 8-bit codes' definition goes by it (packed pairs,
+      // mul and add.rn.f32x2, came out fused)
+      m[q][i] = __fadd_rn(__fmul_rn(m[q][i], h.beta1), __fmul_rn(gr, h.one_minus_beta1));
+      v[q][i] = __fadd_rn(__fmul_rn(v[q][i], h.beta2), __fmul_rn(__fmul_rn(gr, gr), h.one_minus_beta2));
+      const float w = MASTER ? r.w[q].v[i] : to_f(r.p[q].v[i]);
+      const float now = w * f.decay - adam_ratio(m[q][i], v[q][i], f.inv_root, h.eps) * f.step_size;
+      r.w[q].v[i] = now;
+      from_f(r.p[q].v[i], now);
+    }
+    store4<WHOLE>(t.p + at, r.p[q], count[q]);
+    if (MASTER) store4<WHOLE>(t.master + at, r.w[q], count[q]);
+    if constexpr (!EIGHT) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float gr = __fmul_rn(to_f(g4.v[i]), grad_scale);
-        m[q][i] = __fadd_rn(__fmul_rn(m[q][i], h.beta1), __fmul_rn(gr, h.one_minus_beta1));
-        v[q][i] = __fadd_rn(__fmul_rn(v[q][i], h.beta2), __fmul_rn(__fmul_rn(gr, gr), h.one_minus_beta2));
-        const float denom = sqrtf(v[q][i]) * h.inv_root + h.eps;
-        const float w = master != nullptr ? w4.v[i] : to_f(p4.v[i]);
-        const float now = w * h.decay - (m[q][i] / denom) * h.step_size;
-        w4.v[i] = now;
-        from_f(p4.v[i], now);
-        if (i < count) {
+        r.m[q].v[i] = m[q][i];
+        r.v[q].v[i] = v[q][i];
+      }
+      store4<WHOLE>(t.m + at, r.m[q], count[q]);
+      store4<WHOLE>(t.v + at, r.v[q], count[q]);
+    }
+  }
+  if constexpr (EIGHT) {
+    // The largest magnitudes; elements behind the end were loaded as zeros and stay 0, NaN is passed over.
+    float m_max = 0.f, v_max = 0.f;
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        m_max = fmaxf(m_max, fabsf(m[q][i]));
+        v_max = fmaxf(v_max, fabsf(v[q][i]));
+      }
+    uint32_t m_top = __reduce_max_sync(0xffffffffu, __float_as_uint(m_max));
+    uint32_t v_top = __reduce_max_sync(0xffffffffu, __float_as_uint(v_max));
+    if (m_top == 0x7F800000u || v_top == 0x7F800000u) {  // rare: the largest of the finite ones
+      m_top = v_top = 0;
+      for (int q = 0; q < 2; ++q)
+        for (int i = 0; i < 4; ++i) {
           const uint32_t mb = __float_as_uint(m[q][i]) & 0x7FFFFFFFu, vb = __float_as_uint(v[q][i]) & 0x7FFFFFFFu;
           if (mb < 0x7F800000u) m_top = max(m_top, mb);
           if (vb < 0x7F800000u) v_top = max(v_top, vb);
         }
-      }
-      store4(p + at, p4, count, wide_p);
-      if (master != nullptr) store4(master + at, w4, count, wide_w);
-      if (!EIGHT) {
-        Four<float> m4, v4;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          m4.v[i] = m[q][i];
-          v4.v[i] = v[q][i];
-        }
-        store4(static_cast<float*>(tab.m[t]) + at, m4, count, wide_s);
-        store4(static_cast<float*>(tab.v[t]) + at, v4, count, wide_s);
-      }
+      m_top = __reduce_max_sync(0xffffffffu, m_top);
+      v_top = __reduce_max_sync(0xffffffffu, v_top);
     }
-    if (!EIGHT) continue;
-    float m_inv, v_inv;
-    block_scale<7>(__reduce_max_sync(0xffffffffu, m_top), ms, m_inv);
-    block_scale<14>(__reduce_max_sync(0xffffffffu, v_top), vs, v_inv);
+    float ms, vs, m_inv, v_inv;
+    block_scale<7>(m_top, ms, m_inv);
+    block_scale<14>(v_top, vs, v_inv);
     if (lane == 0) {
-      tab.ms[t][base / kAdamBlock] = ms;
-      tab.vs[t][base / kAdamBlock] = vs;
+      *scale_m = ms;
+      *scale_v = vs;
     }
+    const int64_t quad = (element >> 2) + lane;
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
-      const int64_t at = base + q * 128 + lane * 4;
-      const int count = at >= end ? 0 : end - at >= 4 ? 4 : int(end - at);
-      if (count == 0) continue;
-      const uint4 word = philox7(uint32_t(at >> 2), uint32_t(at >> 34), uint32_t(tab.index[t]), h.step, h.seed_lo,
-                                 h.seed_hi);
+      if (!WHOLE && count[q] == 0) continue;
+      const uint4 word = philox7(uint32_t(quad + 32 * q), uint32_t(quad >> 32), uint32_t(index), f.step, h.keys);
       const uint32_t w[4] = {word.x, word.y, word.z, word.w};
-      Four<uint8_t> mc, vc;
+      uint32_t mc[4], vc[4];
+      bool outside = false;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        mc.v[i] = uint8_t(round8<3, 7>(m[q][i], m_inv, w[i] >> 16));
-        vc.v[i] = uint8_t(round8<2, 15>(v[q][i], v_inv, w[i] & 0xFFFFu));
+        mc[i] = round8_normal<3, 7, 7>(m[q][i], m_inv, w[i] >> 16, outside);
+        vc[i] = round8_normal<2, 15, 14>(v[q][i], v_inv, w[i] & 0xFFFFu, outside);
       }
-      store4(static_cast<uint8_t*>(tab.m[t]) + at, mc, count, wide_s);
-      store4(static_cast<uint8_t*>(tab.v[t]) + at, vc, count, wide_s);
+      uint32_t m_word = pack4(mc) + 0x08080808u, v_word = pack4(vc) + 0x04040404u;
+      if (outside) {
+        const uint2 both = round_any(make_float4(m[q][0], m[q][1], m[q][2], m[q][3]),
+                                     make_float4(v[q][0], v[q][1], v[q][2], v[q][3]), m_inv, v_inv, word);
+        m_word = both.x;
+        v_word = both.y;
+      }
+      uint32_t sign[4];  // of m; v is a sum of squares
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sign[i] = __float_as_uint(m[q][i]);
+      const uint32_t top = __byte_perm(__byte_perm(sign[0], sign[1], 0x0073), __byte_perm(sign[2], sign[3], 0x0073), 0x5410);
+      const int at = off + q * 128 + lane * 4;
+      store4<WHOLE>(t.m + at, bytes4(m_word | (top & 0x80808080u)), count[q]);
+      store4<WHOLE>(t.v + at, bytes4(v_word), count[q]);
     }
   }
 }
 
-template <typename P, typename G, bool EIGHT, int N>
+// The tensor of a turn: the last one whose first turn is not behind it.
+template <int N>
+__device__ __forceinline__ int adam_find(const AdamTable<N>& tab, int turn) {
+  int lo = 0, hi = tab.n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (tab.first[mid] <= turn) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+template <typename P, typename G, bool EIGHT, bool MASTER, int N>
+__device__ __forceinline__ AdamTensor<P, G, EIGHT, MASTER> adam_tensor(const AdamTable<N>& tab, int t, int64_t element) {
+  using S = typename AdamTensor<P, G, EIGHT, MASTER>::S;
+  return {static_cast<P*>(tab.p[t]) + element, static_cast<const G*>(tab.g[t]) + element, static_cast<S*>(tab.m[t]) + element,
+          static_cast<S*>(tab.v[t]) + element, MASTER ? tab.master[t] + element : nullptr};
+}
+
+// 32-bit moments: bound by HBM with one block after the other, one CTA a turn (403 M elements 1.65 ms,
+// 6.8 TB/s; persistent CTAs 1.80 ms).
+template <typename P, typename G, bool MASTER, int N>
+__global__ void __launch_bounds__(kAdamThreads, 4) adamw_kernel(const __grid_constant__ AdamTable<N> tab,
+                                                                const __grid_constant__ AdamHyper h) {
+  const AdamFactors f(h);
+  const int t = adam_find(tab, blockIdx.x);
+  const int chunk = tab.passes * kAdamPass;
+  const int64_t begin = int64_t(int(blockIdx.x) - tab.first[t]) * chunk;
+  const AdamTensor<P, G, false, MASTER> a = adam_tensor<P, G, false, MASTER>(tab, t, begin);
+  const int here = int(min(int64_t(chunk), tab.numel[t] - begin));
+  const bool wide = tab.wide[t] != 0;
+  for (int off = (threadIdx.x >> 5) * kAdamBlock; off < here; off += kAdamPass) {
+    if (here - off >= kAdamBlock && wide) {
+      auto raw = adam_load<true>(a, off, kAdamBlock, nullptr, nullptr);
+      adam_block<true>(a, raw, off, kAdamBlock, nullptr, nullptr, begin + off, 0, h, f);
+    } else {
+      const int left = min(kAdamBlock, here - off);
+      auto raw = adam_load<false>(a, off, left, nullptr, nullptr);
+      adam_block<false>(a, raw, off, left, nullptr, nullptr, begin + off, 0, h, f);
+    }
+  }
+}
+
+// 8-bit moments: half the bytes and more arithmetic (about 80 instructions an element, bound by their
+// issue and HBM together), so the loads have to run ahead of it.  Persistent CTAs take turns; each
+// lane copies its own elements of the blocks to come into shared memory (cp.async), kAdamAhead turns
+// ahead, and reads them back itself.  94 M elements: 291 us, 5.2 TB/s (loads into registers, no
+// turns ahead: 448 us).
+constexpr int kAdamAhead = 3;
+
+template <typename P, typename G, bool MASTER, int N>
+__global__ void __launch_bounds__(kAdamThreads, kAdamCtas) adamw8_kernel(const __grid_constant__ AdamTable<N> tab,
+                                                                         const __grid_constant__ AdamHyper h) {
+  using W = typename std::conditional<MASTER, float, P>::type;
+  struct Ahead {
+    Four<G> g[2][kAdamThreads];
+    Four<W> w[2][kAdamThreads];
+    uint32_t m[2][kAdamThreads], v[2][kAdamThreads];
+    float scales[kAdamThreads / 32][2];
+    int64_t element[kAdamThreads / 32];
+    int tensor[kAdamThreads / 32], left[kAdamThreads / 32];  // left < 256: the block is loaded when its time comes
+  };
+  extern __shared__ __align__(16) char smem[];
+  Ahead* ahead = reinterpret_cast<Ahead*>(smem);
+  const AdamFactors f(h);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  // the block to fetch next; where it lies goes into its slot with it
+  int t = adam_find(tab, blockIdx.x), turn = blockIdx.x;
+  const int turns = tab.first[tab.n];
+  auto fetch = [&](Ahead& s) {
+    if (turn < turns) {
+      while (turn >= tab.first[t + 1]) ++t;
+      const int64_t element = int64_t(turn - tab.first[t]) * kAdamPass + warp * kAdamBlock;
+      const int64_t rest = tab.numel[t] - element;
+      const bool whole = rest >= kAdamBlock && tab.wide[t] != 0;
+      if (lane == 0) {
+        s.element[warp] = element;
+        s.tensor[warp] = t;
+        s.left[warp] = whole ? kAdamBlock : rest <= 0 ? 0 : rest < kAdamBlock ? int(rest) : -kAdamBlock;
+      }
+      if (whole) {
+        const AdamTensor<P, G, true, MASTER> a = adam_tensor<P, G, true, MASTER>(tab, t, element);
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const int e = q * 128 + lane * 4;
+          copy_ahead<sizeof(Four<G>)>(&s.g[q][threadIdx.x], a.g + e);
+          if constexpr (MASTER) copy_ahead<16>(&s.w[q][threadIdx.x], a.master + e);
+          else copy_ahead<sizeof(Four<W>)>(&s.w[q][threadIdx.x], a.p + e);
+          copy_ahead<4>(&s.m[q][threadIdx.x], a.m + e);
+          copy_ahead<4>(&s.v[q][threadIdx.x], a.v + e);
+        }
+        if (lane < 2) copy_ahead<4>(&s.scales[warp][lane], (lane == 0 ? tab.ms : tab.vs)[t] + element / kAdamBlock);
+      }
+      turn += gridDim.x;
+    } else if (lane == 0) {
+      s.tensor[warp] = -1;
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  for (int s = 0; s < kAdamAhead; ++s) fetch(ahead[s]);
+  for (int stage = 0;; stage = stage + 1 == kAdamAhead ? 0 : stage + 1) {
+    Ahead& s = ahead[stage];
+    asm volatile("cp.async.wait_group %0;" ::"n"(kAdamAhead - 1) : "memory");
+    __syncwarp();  // place and scales come from other lanes
+    const int at = s.tensor[warp];
+    if (at < 0) break;
+    const int64_t element = s.element[warp];
+    const int left = s.left[warp];
+    AdamRaw<P, G, true, MASTER> raw;
+    if (left == kAdamBlock) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        raw.g[q] = s.g[q][threadIdx.x];
+        if constexpr (MASTER) raw.w[q] = s.w[q][threadIdx.x];
+        else raw.p[q] = s.w[q][threadIdx.x];
+        raw.m[q] = bytes4(s.m[q][threadIdx.x]);
+        raw.v[q] = bytes4(s.v[q][threadIdx.x]);
+      }
+      raw.ms = s.scales[warp][0];
+      raw.vs = s.scales[warp][1];
+    }
+    __syncwarp();  // the slot is read: the next copies may go over it
+    fetch(s);
+    const AdamTensor<P, G, true, MASTER> a = adam_tensor<P, G, true, MASTER>(tab, at, element);
+    float* ms = tab.ms[at] + element / kAdamBlock;
+    float* vs = tab.vs[at] + element / kAdamBlock;
+    if (left == kAdamBlock) {
+      adam_block<true>(a, raw, 0, kAdamBlock, ms, vs, element, tab.index[at], h, f);
+    } else if (left > 0 || left == -kAdamBlock) {
+      const int count = left > 0 ? left : kAdamBlock;
+      raw = adam_load<false>(a, 0, count, ms, vs);
+      adam_block<false>(a, raw, 0, count, ms, vs, element, tab.index[at], h, f);
+    }
+  }
+}
+
+template <typename P, typename G, bool EIGHT, bool MASTER, int N>
 int launch_table(const mcl4moe_adamw_args* a, int first, int count, const AdamHyper& h, cudaStream_t stream) {
   AdamTable<N> tab;
-  int64_t chunks = 0;
+  int64_t passes = 0;
   for (int i = 0; i < count; ++i) {
     const int t = first + i;
     tab.p[i] = a->params[t];
@@ -293,42 +541,65 @@ int launch_table(const mcl4moe_adamw_args* a, int first, int count, const AdamHy
     tab.v[i] = a->exp_avg_sqs[t];
     tab.ms[i] = EIGHT ? a->exp_avg_scales[t] : nullptr;
     tab.vs[i] = EIGHT ? a->exp_avg_sq_scales[t] : nullptr;
-    tab.master[i] = a->masters ? a->masters[t] : nullptr;
+    tab.master[i] = MASTER ? a->masters[t] : nullptr;
     tab.numel[i] = a->numels[t];
     tab.index[i] = a->indices ? a->indices[t] : t;
-    tab.first[i] = int32_t(chunks);
-    chunks += (a->numels[t] + kAdamChunk - 1) / kAdamChunk;
-    if (chunks > (int64_t(1) << 30)) return MCL4MOE_ERR_UNSUPPORTED;
+    const uintptr_t state = EIGHT ? 3 : 15;
+    tab.wide[i] = (reinterpret_cast<uintptr_t>(tab.p[i]) & (4 * sizeof(P) - 1)) == 0 &&
+                  (reinterpret_cast<uintptr_t>(tab.g[i]) & (4 * sizeof(G) - 1)) == 0 &&
+                  ((reinterpret_cast<uintptr_t>(tab.m[i]) | reinterpret_cast<uintptr_t>(tab.v[i])) & state) == 0 &&
+                  (reinterpret_cast<uintptr_t>(tab.master[i]) & 15) == 0;
+    passes += (a->numels[t] + kAdamPass - 1) / kAdamPass;
   }
-  tab.first[count] = int32_t(chunks);
+  // Turns of one pass (8-bit moments: all CTAs sweep one region; turns of four passes 320 us for 291
+  // at 94 M elements), with 32-bit moments of four once every SM has a few: 32 KB in a row of each array.
+  const int64_t most = int64_t(kAdamCtas) * num_sms();
+  tab.passes = EIGHT || passes <= 8 * most ? 1 : 4;
+  const int64_t chunk = int64_t(tab.passes) * kAdamPass;
+  int64_t turns = 0;
+  for (int i = 0; i < count; ++i) {
+    tab.first[i] = int32_t(turns);
+    turns += (tab.numel[i] + chunk - 1) / chunk;
+    if (turns > (int64_t(1) << 30)) return MCL4MOE_ERR_UNSUPPORTED;
+  }
+  tab.first[count] = int32_t(turns);
   tab.n = count;
-  if (chunks == 0) return MCL4MOE_OK;
-  adamw_kernel<P, G, EIGHT, N><<<unsigned(chunks), kAdamThreads, 0, stream>>>(tab, h);
+  if (turns == 0) return MCL4MOE_OK;
+  if constexpr (EIGHT) {
+    constexpr int kBytes = kAdamAhead * (kAdamThreads * 2 * (4 * (sizeof(G) + (MASTER ? 4 : sizeof(P))) + 8) + kAdamThreads / 32 * 24);
+    static std::atomic<uint64_t> raised{0};
+    if (!raise_smem_limit(adamw8_kernel<P, G, MASTER, N>, kBytes, raised)) return MCL4MOE_ERR_CUDA;
+    adamw8_kernel<P, G, MASTER, N><<<unsigned(turns < most ? turns : most), kAdamThreads, kBytes, stream>>>(tab, h);
+  } else {
+    adamw_kernel<P, G, MASTER, N><<<unsigned(turns), kAdamThreads, 0, stream>>>(tab, h);
+  }
   return cudaGetLastError() == cudaSuccess ? MCL4MOE_OK : MCL4MOE_ERR_CUDA;
 }
 
 // The tensors' pointers travel as kernel arguments (32764 bytes at most): a small table for few
 // tensors, full ones for the rest.
-template <typename P, typename G, bool EIGHT>
+template <typename P, typename G, bool EIGHT, bool MASTER>
 int launch_adamw(const mcl4moe_adamw_args* a, const AdamHyper& h, cudaStream_t stream) {
   for (int first = 0; first < a->n;) {
     const int left = a->n - first;
     const int count = left < 440 ? left : 440;
-    const int st = count <= 32 ? launch_table<P, G, EIGHT, 32>(a, first, count, h, stream)
-                               : launch_table<P, G, EIGHT, 440>(a, first, count, h, stream);
+    const int st = count <= 32 ? launch_table<P, G, EIGHT, MASTER, 32>(a, first, count, h, stream)
+                               : launch_table<P, G, EIGHT, MASTER, 440>(a, first, count, h, stream);
     if (st != MCL4MOE_OK) return st;
     first += count;
   }
   return MCL4MOE_OK;
 }
-
+template <typename P, typename G>
+int launch_adamw(const mcl4moe_adamw_args* a, const AdamHyper& h, cudaStream_t stream) {
+  if (a->masters) return a->bits == 8 ? launch_adamw<P, G, true, true>(a, h, stream) : launch_adamw<P, G, false, true>(a, h, stream);
+  return a->bits == 8 ? launch_adamw<P, G, true, false>(a, h, stream) : launch_adamw<P, G, false, false>(a, h, stream);
+}
 template <typename P>
-int launch_adamw_grad(const mcl4moe_adamw_args* a, const AdamHyper& h, cudaStream_t stream) {
-  if (a->grad_dtype == 0)
-    return a->bits == 8 ? launch_adamw<P, uint16_t, true>(a, h, stream) : launch_adamw<P, uint16_t, false>(a, h, stream);
-  if (a->grad_dtype == 1)
-    return a->bits == 8 ? launch_adamw<P, float, true>(a, h, stream) : launch_adamw<P, float, false>(a, h, stream);
-  return a->bits == 8 ? launch_adamw<P, __half, true>(a, h, stream) : launch_adamw<P, __half, false>(a, h, stream);
+int launch_adamw(const mcl4moe_adamw_args* a, const AdamHyper& h, cudaStream_t stream) {
+  if (a->grad_dtype == 0) return launch_adamw<P, uint16_t>(a, h, stream);
+  if (a->grad_dtype == 1) return launch_adamw<P, float>(a, h, stream);
+  return launch_adamw<P, __half>(a, h, stream);
 }
 
 }  // namespace
@@ -359,8 +630,8 @@ extern "C" int mcl4moe_adamw_step(const mcl4moe_adamw_args* a, mcl4moe_stream_t 
   h.one_minus_beta1 = float(1.0 - a->beta1);
   h.one_minus_beta2 = float(1.0 - a->beta2);
   h.eps = float(a->eps);
-  h.lr = float(a->lr);
-  h.weight_decay = float(a->weight_decay);
+  h.lr = a->lr;
+  h.weight_decay = a->weight_decay;
   h.decay = float(1.0 - a->lr * a->weight_decay);
   if (!a->step_dev) {
     h.step_size = float(a->lr / (1.0 - std::pow(a->beta1, double(a->step))));
@@ -372,9 +643,11 @@ extern "C" int mcl4moe_adamw_step(const mcl4moe_adamw_args* a, mcl4moe_stream_t 
   h.lr_dev = a->lr_dev;
   h.grad_scale = a->grad_scale;
   h.step = uint32_t(a->step);
-  h.seed_lo = uint32_t(a->seed);
-  h.seed_hi = uint32_t(a->seed >> 32);
-  if (a->param_dtype == 0) return launch_adamw_grad<uint16_t>(a, h, stream);
-  if (a->param_dtype == 1) return launch_adamw_grad<float>(a, h, stream);
-  return launch_adamw_grad<__half>(a, h, stream);
+  for (uint32_t r = 0; r < 7; ++r) {
+    h.keys[2 * r] = uint32_t(a->seed) + r * 0x9E3779B9u;
+    h.keys[2 * r + 1] = uint32_t(a->seed >> 32) + r * 0xBB67AE85u;
+  }
+  if (a->param_dtype == 0) return launch_adamw<uint16_t>(a, h, stream);
+  if (a->param_dtype == 1) return launch_adamw<float>(a, h, stream);
+  return launch_adamw<__half>(a, h, stream);
 }

@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 from array import array
+from operator import attrgetter
 from typing import Sequence
 
 import torch
@@ -22,17 +23,21 @@ from .routing import DTYPE_CODES, _launch
 STATE_BLOCK = 256  # elements of a tensor that share a scale of its 8-bit moments
 
 
-def _check_list(name: str, tensors: Sequence[Tensor], dtype: torch.dtype, device: int, sizes: list[int]) -> None:
+_dtype_of = attrgetter("dtype")
+
+
+def _check_list(name: str, tensors: Sequence[Tensor], dtype: torch.dtype, device: int, sizes: list[int]) -> array:
+    """The tensors' addresses, after the checks (C-level maps: an optimizer step has hundreds of tensors)."""
     if len(tensors) != len(sizes):
         raise ValueError(f"{name}: {len(tensors)} tensors for {len(sizes)} parameters")
-    want = {(dtype, device, True)}
-    if {(t.dtype, t.get_device(), t.is_contiguous()) for t in tensors} == want and \
-            [t.numel() for t in tensors] == sizes:
-        return
+    if (list(map(Tensor.numel, tensors)) == sizes and set(map(_dtype_of, tensors)) == {dtype}
+            and set(map(Tensor.get_device, tensors)) == {device} and all(map(Tensor.is_contiguous, tensors))):
+        return array("Q", list(map(Tensor.data_ptr, tensors)))
     for i, (t, n) in enumerate(zip(tensors, sizes)):
-        if (t.dtype, t.get_device(), t.is_contiguous()) not in want or t.numel() != n:
+        if t.dtype != dtype or t.get_device() != device or not t.is_contiguous() or t.numel() != n:
             raise ValueError(f"{name}[{i}] must be {n} contiguous {dtype} elements on the first parameter's device, got "
                              f"{t.numel()} of {t.dtype} on {t.device}")
+    raise AssertionError(name)
 
 
 @torch.no_grad()
@@ -78,25 +83,26 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
     dev = first.device
     if first.dtype not in DTYPE_CODES or grads[0].dtype not in DTYPE_CODES:
         raise ValueError(f"parameters and gradients must be bf16, fp16 or fp32, got {first.dtype} and {grads[0].dtype}")
-    index, sizes = first.get_device(), [p.numel() for p in params]
-    _check_list("params", params, first.dtype, index, sizes)
-    if not all(g.is_contiguous() for g in grads):
+    index, sizes = first.get_device(), list(map(Tensor.numel, params))
+    if not all(map(Tensor.is_contiguous, grads)):
         grads = [g.contiguous() for g in grads]
-    _check_list("grads", grads, grads[0].dtype, index, sizes)
-    _check_list("exp_avgs", exp_avgs, torch.float8_e4m3fn if eight else torch.float32, index, sizes)
-    _check_list("exp_avg_sqs", exp_avg_sqs, torch.float8_e5m2 if eight else torch.float32, index, sizes)
-    numels = array("q", sizes)
-    changed = [*params, *exp_avgs, *exp_avg_sqs]
+    moments = (torch.float8_e4m3fn, torch.float8_e5m2) if eight else (torch.float32, torch.float32)
+    written = dict(params=params, exp_avgs=exp_avgs, exp_avg_sqs=exp_avg_sqs)
+    at = dict(params=_check_list("params", params, first.dtype, index, sizes),
+              exp_avgs=_check_list("exp_avgs", exp_avgs, moments[0], index, sizes),
+              exp_avg_sqs=_check_list("exp_avg_sqs", exp_avg_sqs, moments[1], index, sizes))
     if eight:
         blocks = [-(-n // STATE_BLOCK) for n in sizes]
-        _check_list("exp_avg_scales", exp_avg_scales, torch.float32, index, blocks)
-        _check_list("exp_avg_sq_scales", exp_avg_sq_scales, torch.float32, index, blocks)
-        changed += [*exp_avg_scales, *exp_avg_sq_scales]
+        for name, tensors in (("exp_avg_scales", exp_avg_scales), ("exp_avg_sq_scales", exp_avg_sq_scales)):
+            at[name] = _check_list(name, tensors, torch.float32, index, blocks)
+            written[name] = tensors
     if masters is not None:
-        _check_list("masters", masters, torch.float32, index, sizes)
-        changed += list(masters)
-    if len({id(t) for t in changed}) != len(changed):
+        at["masters"] = _check_list("masters", masters, torch.float32, index, sizes)
+        written["masters"] = masters
+    places = [p for a in at.values() for p in a if p]  # an empty tensor has no address
+    if len(set(places)) != len(places):
         raise ValueError("a tensor is in the lists twice")
+    at["grads"] = _check_list("grads", grads, grads[0].dtype, index, sizes)
     for name, t, dtype in (("step", step, torch.int64), ("lr", lr, torch.float32), ("grad_scale", grad_scale, torch.float32)):
         if isinstance(t, Tensor) and (t.dtype != dtype or t.numel() != 1 or t.device != dev):
             raise ValueError(f"{name} as a tensor must be one {dtype} on {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
@@ -106,18 +112,12 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
     args = _lib.AdamwArgs(n=len(params), param_dtype=DTYPE_CODES[first.dtype],
                           grad_dtype=DTYPE_CODES[grads[0].dtype], bits=8 if eight else 32, beta1=beta1, beta2=beta2,
                           eps=eps, weight_decay=weight_decay, seed=int(seed) & 0xFFFFFFFFFFFFFFFF)
-    keep = [numels]
-    args.numels = numels.buffer_info()[0]
-    for name, tensors in (("params", params), ("grads", grads), ("exp_avgs", exp_avgs), ("exp_avg_sqs", exp_avg_sqs),
-                          ("exp_avg_scales", exp_avg_scales), ("exp_avg_sq_scales", exp_avg_sq_scales),
-                          ("masters", masters)):
-        if tensors is not None:
-            keep.append(array("Q", [t.data_ptr() for t in tensors]))
-            setattr(args, name, keep[-1].buffer_info()[0])
+    at["numels"] = array("q", sizes)
+    for name, a in at.items():
+        setattr(args, name, a.buffer_info()[0])
     if indices is not None:
-        a = array("i", indices)
-        keep.append(a)
-        args.indices = a.buffer_info()[0]
+        at["indices"] = array("i", indices)
+        args.indices = at["indices"].buffer_info()[0]
     if isinstance(step, Tensor):
         args.step_dev = step.data_ptr()
     else:
@@ -128,4 +128,4 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
         args.lr = float(lr)
     args.grad_scale = _ptr(grad_scale)
     _launch(dev, "mcl4moe_adamw_step", _lib.load().mcl4moe_adamw_step, ctypes.byref(args))
-    torch.autograd.graph.increment_version(changed)
+    torch.autograd.graph.increment_version([t for tensors in written.values() for t in tensors])
