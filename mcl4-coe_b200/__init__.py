@@ -10,7 +10,7 @@ through ``__graft_entry__.load_package()`` (registered as ``mcl4coe_b200``).
 
 from . import _lib, routing_variants
 from .expert_parallel import CudaEPOps, ExpertParallelMoE
-from .moe import MoEConfig, SparseMoE, SwiGLUExpert
+from .moe import MoEConfig, SparseMoE, SparseMoEBlock, SwiGLUExpert
 from .nvfp4 import (
     SPARSITY_MODES,
     GroupedNVFP4Cache,
@@ -26,7 +26,7 @@ from .nvfp4 import (
     quantize_nvfp4,
     reset_gemm_counts,
 )
-from .optim import adamw_step
+from .optim import AdamW, adamw_step
 from .norms import residual_norm
 from .routing import route_experts
 
@@ -49,6 +49,8 @@ __all__ = [
     "convert_linear_to_nvfp4",
     "nvfp4_mm",
     "quantize_activations",
+    "AdamW",
+    "SparseMoEBlock",
     "adamw_step",
     "residual_norm",
     "route_experts",

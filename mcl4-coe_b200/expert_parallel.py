@@ -485,7 +485,8 @@ class ExpertParallelMoE(nn.Module):
              or getattr(moe, "dense_subset_k", 0) > 0),
             ("the recurrent coverage penalty", getattr(moe, "recurrent_coverage_penalty", 0.0) > 0.0),
             ("sequence-diversity / mitotic-orthogonality losses", getattr(moe, "sequence_diversity_coef", 0.0) > 0.0
-             or getattr(moe, "mitotic_ortho_coef", 0.0) > 0.0)) if on]
+             or getattr(moe, "mitotic_ortho_coef", 0.0) > 0.0),
+            ("routing from scores", bool(getattr(moe, "_scored", bool)()))) if on]
         if variant:
             raise NotImplementedError(f"the expert-parallel layer routes plain top-k only; this layer uses {variant[0]}")
         E = len(moe.experts)

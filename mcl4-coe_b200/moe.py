@@ -32,6 +32,11 @@ and mitotic-orthogonality losses) compute the reference's selection on the
 library's router logits (``routing_variants.py``) and run the experts through
 ``mcl4moe_moe_forward_routed``.
 
+Routing from scores (``MoEConfig.score_function``, ``expert_groups``, ``balance_bias``,
+``routed_scale``; not in the reference) goes through ``route_experts`` and the same
+experts, forward and backward.  ``SparseMoEBlock`` is the layer with the norms and the
+residual around it.
+
 Training: under autograd (plain top-k routing) the forward keeps the gate / value
 rows, the permuted bf16 inputs, h and the unweighted down-projection rows, and the
 backward runs the reference's _NVFP4GroupedLinear.backward path
@@ -50,9 +55,14 @@ from typing import Any, Sequence
 
 import torch
 from torch import Tensor, nn
+from torch.autograd.function import once_differentiable
 
 from . import _lib
+from .norms import residual_norm
 from .nvfp4 import _stream_handle, get_or_build_grouped_cache, invalidate_cache, nvfp4_grouped_linear
+from .routing import GROUP_SCORES, SCORE_FUNCTIONS, route_experts
+
+RESIDUAL_GATES = ("none", "linear", "sigmoid", "tanh")
 
 
 @dataclass
@@ -72,6 +82,18 @@ class MoEConfig:
     dense_expert_indices: tuple[int, ...] = ()
     dense_subset_k: int = 0
     combine_dense_and_sparse: bool = False
+    # Routing from scores beyond the reference's plain softmax top-k (``route_experts``).
+    score_function: str = "softmax"      # or "sigmoid"
+    expert_groups: int = 1               # groups of consecutive experts ...
+    top_expert_groups: int = 0           # ... of which the best are searched (0: all)
+    group_score: str = "top2"            # a group's value: sum of its two best keys, or "max"
+    routed_scale: float = 1.0
+    balance_bias: bool = False           # a selection-only bias per expert (``SparseMoE.balance_bias``)
+    # The norms and the residual around the layer (``SparseMoEBlock``).
+    norm_eps: float = 1e-6
+    post_norm: bool = False
+    residual_gate: str = "none"          # "none", or a learned gate per channel: "linear", "sigmoid", "tanh"
+    branch_scale: float = 1.0
 
     def __post_init__(self) -> None:  # src/mcl4_coe/backbone.py:84-108
         for name in ("d_model", "expert_hidden_dim", "num_experts", "top_k"):
@@ -80,6 +102,15 @@ class MoEConfig:
                 raise ValueError(f"{name} must be a positive integer")
         if self.top_k > self.num_experts:
             raise ValueError("top_k cannot exceed num_experts")
+        if self.score_function not in SCORE_FUNCTIONS or self.group_score not in GROUP_SCORES:
+            raise ValueError(f"score_function must be one of {SCORE_FUNCTIONS}, group_score one of {GROUP_SCORES}")
+        groups, top = self.expert_groups, self.top_expert_groups or self.expert_groups
+        if groups < 1 or self.num_experts % groups != 0 or not 1 <= top <= groups:
+            raise ValueError("expert_groups must divide num_experts, top_expert_groups be at most expert_groups")
+        if self.top_k > top * (self.num_experts // groups):
+            raise ValueError("top_k cannot exceed the experts of the open groups")
+        if self.residual_gate not in RESIDUAL_GATES:
+            raise ValueError(f"residual_gate must be one of {RESIDUAL_GATES}")
 
 
 def _opt_ptr(t: Tensor | None) -> int | None:
@@ -109,10 +140,18 @@ class SparseMoE(nn.Module):
         self.dense_expert_indices: tuple[int, ...] = tuple(int(i) for i in getattr(config, "dense_expert_indices", ()))
         self.dense_subset_k = int(getattr(config, "dense_subset_k", 0))
         self.combine_dense_and_sparse = bool(getattr(config, "combine_dense_and_sparse", False))
+        self.score_function = str(getattr(config, "score_function", "softmax"))
+        self.expert_groups = int(getattr(config, "expert_groups", 1))
+        self.top_expert_groups = int(getattr(config, "top_expert_groups", 0))
+        self.group_score = str(getattr(config, "group_score", "top2"))
+        self.routed_scale = float(getattr(config, "routed_scale", 1.0))
         d_model = int(config.d_model)
         hidden = int(config.expert_hidden_dim)
         self.router = nn.Linear(d_model, self.num_experts, bias=False)
         self.experts = nn.ModuleList(SwiGLUExpert(d_model, hidden) for _ in range(self.num_experts))
+        # Selection-only bias [E] of routing from scores (None: off); see update_balance_bias().
+        self.register_buffer("balance_bias", torch.zeros(self.num_experts)
+                             if bool(getattr(config, "balance_bias", False)) else None)
         self.mitotic_pairs: list[tuple[int, int]] = []
         self.last_selected_mask: Tensor | None = None
         self.lineage_num_roots = 0
@@ -219,16 +258,26 @@ class SparseMoE(nn.Module):
 
     # ------------------------------------------------------------------ helpers
     def _routing_variant(self, prior_expert_mask, dense_expert_indices, dense_subset_k) -> str | None:
-        """Which routing variant this call needs (None: plain top-k, served by one library call)."""
+        """Which routing this call needs: None (plain top-k, served by one library call), "scored"
+        (``route_experts``), or one of the reference's variants ("sparse", "dense")."""
         if dense_expert_indices is not None and len(dense_expert_indices) > 0:
-            return "dense"
-        if self.dense_expert_indices or int(self.dense_subset_k if dense_subset_k is None else dense_subset_k) > 0:
-            return "dense"
-        if (self.mitotic_pairs or (self.lineage_top_families > 0 and self.lineage_root_ids is not None)
+            variant = "dense"
+        elif self.dense_expert_indices or int(self.dense_subset_k if dense_subset_k is None else dense_subset_k) > 0:
+            variant = "dense"
+        elif (self.mitotic_pairs or (self.lineage_top_families > 0 and self.lineage_root_ids is not None)
                 or (prior_expert_mask is not None and self.recurrent_coverage_penalty > 0.0)
                 or self.sequence_diversity_coef > 0.0 or self.mitotic_ortho_coef > 0.0):
-            return "sparse"
-        return None
+            variant = "sparse"
+        else:
+            return "scored" if self._scored() else None
+        if self._scored():
+            raise NotImplementedError("routing from scores does not combine with the reference's routing variants")
+        return variant
+
+    def _scored(self) -> bool:
+        """Whether the configuration routes through ``route_experts``: anything but plain softmax top-k."""
+        return (self.score_function != "softmax" or 0 < self.top_expert_groups < self.expert_groups
+                or self.routed_scale != 1.0 or self.balance_bias is not None)
 
     def _workspace(self, T: int, d: int, E: int, k: int, F: int, device: torch.device) -> Tensor:
         key = (T, d, E, k, F, str(device))
@@ -275,6 +324,8 @@ class SparseMoE(nn.Module):
         if flat.device.type != "cuda":
             raise ValueError("SparseMoE on B200 requires CUDA tensors (there is no CPU fallback)")
         variant = self._routing_variant(prior_expert_mask, dense_expert_indices, dense_subset_k)
+        if variant == "scored" and not details and static is None:
+            return self._forward_scored(x, valid)
         if torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in self.parameters())):
             if variant is not None or details or static is not None:
                 raise NotImplementedError("training (autograd) runs plain top-k routing through forward() only")
@@ -384,6 +435,76 @@ class SparseMoE(nn.Module):
         dns = [e.down_proj.weight for e in self.experts]
         out, aux, z, counts = _MoETrainFunction.apply(self, x, valid, self.router.weight, *ups, *dns)
         return dict(out=out, aux_loss=aux, router_z_loss=z, counts=counts)
+
+    # ------------------------------------------------------------------ routing from scores
+    def _forward_scored(self, x: Tensor, valid: Tensor | None) -> dict:
+        """Router logits, ``route_experts``, then the experts on that routing; under autograd with
+        the gradient of each.  ``aux_loss`` is the reference's E sum(load * mean score share), with
+        the sigmoid's shares s / sum(s); ``router_z_loss`` and the masked tokens as everywhere."""
+        E = len(self.experts)
+        if self.router.weight.shape[0] != E:
+            raise ValueError("router rows must match the number of experts")
+        if self.balance_bias is not None and self.balance_bias.numel() != E:
+            raise ValueError("balance_bias must have one entry per expert")
+        self.num_experts = E
+        flat = x.reshape(-1, x.shape[-1])
+        T = flat.shape[0]
+        dev = flat.device
+        vmask = None
+        if valid is not None:
+            vmask = valid.reshape(-1).to(device=dev).bool().contiguous()
+            if vmask.numel() != T:
+                raise ValueError("valid must have one entry per token")
+        if T == 0:
+            zero = torch.zeros((), dtype=torch.float32, device=dev)
+            self.last_selected_mask = torch.zeros((*x.shape[:-1], E), dtype=torch.float32, device=dev)
+            return dict(out=torch.zeros_like(x), aux_loss=zero, router_z_loss=zero,
+                        counts=torch.zeros(E, dtype=torch.float32, device=dev))
+        xb = flat.to(torch.bfloat16).contiguous()
+        bias = None
+        if self.router_logit_bias is not None:
+            bias = self.router_logit_bias.detach().to(device=dev, dtype=torch.float32).contiguous()
+        with torch.autocast(device_type=dev.type, enabled=False):
+            logits = _RouterLogitsFunction.apply(self, xb, self.router.weight, bias, vmask)
+            w, idx, slots = route_experts(
+                logits, self.top_k, score=self.score_function, bias=self.balance_bias, num_groups=self.expert_groups,
+                top_groups=self.top_expert_groups or self.expert_groups, group_score=self.group_score,
+                renormalize=self.norm_topk_prob, scale=self.routed_scale, valid=vmask)
+            if torch.is_grad_enabled() and (xb.requires_grad or w.requires_grad
+                                            or any(p.requires_grad for p in self.experts.parameters())):
+                out = _RoutedExpertsFunction.apply(self, xb, None if vmask is None else vmask.view(torch.uint8), idx, w,
+                                                   *[e.up_proj.weight for e in self.experts],
+                                                   *[e.down_proj.weight for e in self.experts])
+            else:
+                out = self._forward_routed(xb, None if vmask is None else vmask.view(torch.uint8), idx, w)
+            n_rows = float(T)
+            if vmask is not None:  # before the softmax: its gradient would spread what masked rows hold
+                logits = torch.where(vmask.unsqueeze(-1), logits, 0.0)
+            shares = (torch.softmax(logits, dim=-1) if self.score_function == "softmax"
+                      else torch.nn.functional.normalize(torch.sigmoid(logits), p=1.0, dim=-1))
+            z_rows = torch.logsumexp(logits, dim=-1).square()
+            if vmask is not None:
+                shares = torch.where(vmask.unsqueeze(-1), shares, 0.0)
+                z_rows = torch.where(vmask, z_rows, 0.0)
+                n_rows = vmask.sum().clamp_min(1)
+            load = slots.float() / slots.sum().clamp_min(1)
+            aux = E * (load * (shares.sum(dim=0) / n_rows)).sum()
+            z = z_rows.sum() / n_rows
+        mask = torch.zeros((T, E + 1), dtype=torch.float32, device=dev)
+        mask.scatter_(1, idx.long() % (E + 1), 1.0)  # id -1 falls into the column that is cut off
+        self.last_selected_mask = mask[:, :E].view(*x.shape[:-1], E)
+        return dict(out=out.to(x.dtype).view_as(x), aux_loss=aux, router_z_loss=z, counts=load.detach())
+
+    @torch.no_grad()
+    def update_balance_bias(self, counts: Tensor, rate: float = 1e-3) -> None:
+        """Moves ``balance_bias`` by ``rate`` towards an even load: up for experts below the mean of
+        ``counts`` (the forward's fourth result, or a sum of several), down for those above."""
+        if self.balance_bias is None:
+            raise ValueError("this layer has no balance_bias (MoEConfig.balance_bias)")
+        if counts.shape != self.balance_bias.shape:
+            raise ValueError("counts must have one entry per expert")
+        counts = counts.to(self.balance_bias)
+        self.balance_bias.add_(torch.sign(counts.mean() - counts), alpha=rate)
 
     # ------------------------------------------------------------------ routing variants
     def _router_logits(self, xb: Tensor, wr: Tensor, bias: Tensor | None) -> Tensor:
@@ -593,6 +714,133 @@ def _weight_grads(d_rows: Tensor, rows: Tensor, pad_start: Tensor, E: int) -> Te
     return dw
 
 
+def _experts_backward(d_out, slot_pos, topk_w, pad_start, counts, offs_start, y_save, up_save, up, dn, shape):
+    """``mcl4moe_moe_backward_experts`` on a training forward's saves: the gradients of the
+    down-projection rows, of the gate | value rows, of the permuted inputs and of the routing weights."""
+    lib = _lib.load()
+    T, d, E, k, F = shape
+    mcap = up_save.shape[0]
+    dev = up_save.device
+    d_out = d_out.reshape(T, d).to(torch.bfloat16).contiguous()
+    bf = dict(dtype=torch.bfloat16, device=dev)
+    d_y = torch.empty((mcap, d), **bf)
+    d_up = torch.empty((mcap, 2 * F), **bf)
+    d_rows = torch.empty((mcap, d), **bf)
+    d_w = torch.zeros((T, k), dtype=torch.float32, device=dev)
+    ws = torch.empty((max(lib.mcl4moe_moe_backward_workspace_size(T, d, E, k, F), 256),), dtype=torch.uint8, device=dev)
+    args = _lib.MoeBwdArgs(
+        T=T, d=d, E=E, k=k, F=F, d_out=d_out.data_ptr(), slot_pos=slot_pos.data_ptr(),
+        topk_w=topk_w.data_ptr(), pad_start=pad_start.data_ptr(), counts=counts.data_ptr(),
+        offs_start=offs_start.data_ptr(), y_save=y_save.data_ptr(), up_save=up_save.data_ptr(),
+        w_up_t=up.packed_t.data_ptr(), w_up_t_scales=up.scales_t.data_ptr(), w_up_g=up.g.data_ptr(),
+        w_dn_t=dn.packed_t.data_ptr(), w_dn_t_scales=dn.scales_t.data_ptr(), w_dn_g=dn.g.data_ptr(),
+        seed_down=random.getrandbits(31), seed_up=random.getrandbits(31),  # src/mcl4_coe/nvfp4.py:1140
+        d_y=d_y.data_ptr(), d_up=d_up.data_ptr(), d_rows=d_rows.data_ptr(), d_w=d_w.data_ptr(),
+        error_word=None, workspace=ws.data_ptr(), workspace_bytes=ws.numel())
+    if T > 0:
+        _lib.check(lib.mcl4moe_moe_backward_experts(args, _stream_handle()), "mcl4moe_moe_backward_experts")
+    return d_y, d_up, d_rows, d_w
+
+
+def _expert_parameter_grads(mod, d_y, d_up, h_save, x_rows, pad_start, shape, needed):
+    """The experts' weight gradients over the padded segments (padding rows are zero in d_y / d_up);
+    ``needed``: for each up projection, then each down projection."""
+    T, d, E, _, F = shape
+    n_exp = len(mod.experts)
+    f32 = dict(dtype=torch.float32, device=d_y.device)
+    if T > 0:
+        dw_dn = _weight_grads(d_y, h_save, pad_start, E)
+        dw_up = _weight_grads(d_up, x_rows, pad_start, E)
+    else:
+        dw_dn = torch.zeros((E, d, F), **f32)
+        dw_up = torch.zeros((E, 2 * F, d), **f32)
+    ups = [e.up_proj.weight for e in mod.experts]
+    dns = [e.down_proj.weight for e in mod.experts]
+    g_up = [dw_up[i].to(ups[i].dtype) if needed[i] else None for i in range(n_exp)]
+    g_dn = [dw_dn[i].to(dns[i].dtype) if needed[n_exp + i] else None for i in range(n_exp)]
+    return g_up, g_dn
+
+
+class _RouterLogitsFunction(torch.autograd.Function):
+    """fp32 router logits from the library's router; the gradient's two fp32 products as in
+    ``_MoETrainFunction`` (F.linear(x.float(), W) at src/mcl4_coe/backbone.py:790)."""
+
+    @staticmethod
+    def forward(ctx, mod, xb, wr_param, bias, vmask):
+        wr = wr_param.detach().to(torch.float32).contiguous()
+        ctx.save_for_backward(xb, wr, vmask)
+        ctx.wr_dtype = wr_param.dtype
+        return mod._router_logits(xb.detach(), wr, bias)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_logits):
+        xb, wr, vmask = ctx.saved_tensors
+        d_x = (d_logits @ wr).to(xb.dtype) if ctx.needs_input_grad[1] else None
+        d_wr = None
+        if ctx.needs_input_grad[2]:
+            x32 = xb.float()
+            if vmask is not None:
+                x32.masked_fill_(~vmask.unsqueeze(-1), 0.0)  # whatever masked rows hold
+            d_wr = (d_logits.t() @ x32).to(ctx.wr_dtype)
+        return None, d_x, d_wr, None, None
+
+
+class _RoutedExpertsFunction(torch.autograd.Function):
+    """The experts on a given routing under autograd: ``mcl4moe_moe_forward_routed`` with the training
+    saves, and the expert part of ``_MoETrainFunction``'s backward."""
+
+    @staticmethod
+    def forward(ctx, mod, xb, vmask, idx, w, *expert_weights):
+        lib = _lib.load()
+        T, d = xb.shape
+        E, k = len(mod.experts), idx.shape[1]
+        F = mod.experts[0].down_proj.weight.shape[1]
+        dev = xb.device
+        up = get_or_build_grouped_cache(mod.experts, "up_proj", with_bwd=True)
+        dn = get_or_build_grouped_cache(mod.experts, "down_proj", with_bwd=True)
+        mcap = lib.mcl4moe_padded_rows(T, E, k)
+        bf = dict(dtype=torch.bfloat16, device=dev)
+        out = torch.empty((T, d), **bf)
+        up_save = torch.empty((mcap, 2 * F), **bf)
+        x_rows = torch.empty((mcap, d), **bf)
+        y_save = torch.empty((mcap, d), **bf)
+        h_save = torch.empty((mcap, F), **bf)
+        ws = mod._workspace(T, d, E, k, F, dev)
+        args = _lib.MoeArgs(
+            x=xb.data_ptr(), router_w=None, logit_bias=None, valid=_opt_ptr(vmask),
+            w_up=up.packed.data_ptr(), w_up_scales=up.scales.data_ptr(), w_up_g=up.g.data_ptr(),
+            w_dn=dn.packed.data_ptr(), w_dn_scales=dn.scales.data_ptr(), w_dn_g=dn.g.data_ptr(),
+            T=T, d=d, E=E, k=k, F=F, norm_topk_prob=int(mod.norm_topk_prob),
+            out=out.data_ptr(), stats=None, sel_mask=None, topk_idx=idx.data_ptr(), topk_w=w.data_ptr(),
+            offs=None, perm=None, h_debug=h_save.data_ptr() if T > 0 else None, error_word=None,
+            workspace=ws.data_ptr(), workspace_bytes=ws.numel(), up_save=up_save.data_ptr() if T > 0 else None,
+            x_rows_save=x_rows.data_ptr() if T > 0 else None, y_save=y_save.data_ptr() if T > 0 else None)
+        _lib.check(lib.mcl4moe_moe_forward_routed(args, _stream_handle()), "mcl4moe_moe_forward_routed")
+        # the expert layout of this call (the workspace is reused by the next call)
+        layout = [_region(ws, r, 4 * n, T, d, E, k, F).view(torch.int32).clone()
+                  for r, n in ((6, T * k), (5, E + 1), (9, E), (10, E))]
+        ctx.mod, ctx.shape, ctx.caches = mod, (T, d, E, k, F), (up, dn)
+        ctx.save_for_backward(w, up_save, x_rows, y_save, h_save, *layout)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_out):
+        w, up_save, x_rows, y_save, h_save, slot_pos, pad_start, counts, offs_start = ctx.saved_tensors
+        T, d, E, k, F = ctx.shape
+        d_y, d_up, d_rows, d_w = _experts_backward(d_out, slot_pos, w, pad_start, counts, offs_start, y_save, up_save,
+                                                   *ctx.caches, ctx.shape)
+        d_x = None
+        if ctx.needs_input_grad[1]:
+            d_x = torch.empty((T, d), dtype=torch.bfloat16, device=d_rows.device)
+            _lib.check(_lib.load().mcl4moe_moe_backward_dx(d_rows.data_ptr(), slot_pos.data_ptr(), None, T, k, d,
+                                                           d_x.data_ptr(), _stream_handle()), "mcl4moe_moe_backward_dx")
+        g_up, g_dn = _expert_parameter_grads(ctx.mod, d_y, d_up, h_save, x_rows, pad_start, ctx.shape,
+                                             ctx.needs_input_grad[5:])
+        return (None, d_x, None, None, d_w, *g_up, *g_dn)
+
+
 class _MoETrainFunction(torch.autograd.Function):
     """The layer under autograd (src/mcl4_coe/backbone.py:787-911 with
     _NVFP4GroupedLinear, src/mcl4_coe/nvfp4.py:1051-1216).
@@ -673,33 +921,15 @@ class _MoETrainFunction(torch.autograd.Function):
         up, dn = ctx.caches
         T, d, E, k, F = ctx.shape
         dev = xb.device
-        mcap = up_save.shape[0]
-        n_exp = len(mod.experts)
         if d_out is None:
             d_out = torch.zeros((T, d), dtype=torch.bfloat16, device=dev)
-        d_out = d_out.reshape(T, d).to(torch.bfloat16).contiguous()
         f32 = dict(dtype=torch.float32, device=dev)
         d_aux = torch.zeros((), **f32) if d_aux is None else d_aux.detach().to(torch.float32).reshape(()).contiguous()
         d_z = torch.zeros((), **f32) if d_z is None else d_z.detach().to(torch.float32).reshape(()).contiguous()
         bf = dict(dtype=torch.bfloat16, device=dev)
-        d_y = torch.empty((mcap, d), **bf)
-        d_up = torch.empty((mcap, 2 * F), **bf)
-        d_rows = torch.empty((mcap, d), **bf)
-        d_w = torch.zeros((T, k), **f32)
-        ws = torch.empty((max(lib.mcl4moe_moe_backward_workspace_size(T, d, E, k, F), 256),), dtype=torch.uint8,
-                         device=dev)
-        args = _lib.MoeBwdArgs(
-            T=T, d=d, E=E, k=k, F=F, d_out=d_out.data_ptr(), slot_pos=slot_pos.data_ptr(),
-            topk_w=topk_w.data_ptr(), pad_start=pad_start.data_ptr(), counts=counts_i.data_ptr(),
-            offs_start=offs_start.data_ptr(), y_save=y_save.data_ptr(), up_save=up_save.data_ptr(),
-            w_up_t=up.packed_t.data_ptr(), w_up_t_scales=up.scales_t.data_ptr(), w_up_g=up.g.data_ptr(),
-            w_dn_t=dn.packed_t.data_ptr(), w_dn_t_scales=dn.scales_t.data_ptr(), w_dn_g=dn.g.data_ptr(),
-            seed_down=random.getrandbits(31), seed_up=random.getrandbits(31),  # src/mcl4_coe/nvfp4.py:1140
-            d_y=d_y.data_ptr(), d_up=d_up.data_ptr(), d_rows=d_rows.data_ptr(), d_w=d_w.data_ptr(),
-            error_word=None, workspace=ws.data_ptr(), workspace_bytes=ws.numel())
         stream = _stream_handle()
-        if T > 0:
-            _lib.check(lib.mcl4moe_moe_backward_experts(args, stream), "mcl4moe_moe_backward_experts")
+        d_y, d_up, d_rows, d_w = _experts_backward(d_out, slot_pos, topk_w, pad_start, counts_i, offs_start, y_save,
+                                                   up_save, up, dn, ctx.shape)
         d_logits = torch.empty((T, E), **f32)
         _lib.check(lib.mcl4moe_router_backward(logits.data_ptr(), topk_idx.data_ptr(), topk_w.data_ptr(),
                                                d_w.data_ptr(), _opt_ptr(vmask), stats.data_ptr(), d_aux.data_ptr(),
@@ -711,17 +941,44 @@ class _MoETrainFunction(torch.autograd.Function):
         d_x = torch.empty((T, d), **bf)
         _lib.check(lib.mcl4moe_moe_backward_dx(d_rows.data_ptr(), slot_pos.data_ptr(), d_x_router.data_ptr(), T, k, d,
                                                d_x.data_ptr(), stream), "mcl4moe_moe_backward_dx")
-        # expert weight gradients over the padded segments (padding rows are zero in d_y / d_up)
-        if T > 0:
-            dw_dn = _weight_grads(d_y, h_save, pad_start, E)
-            dw_up = _weight_grads(d_up, x_rows, pad_start, E)
-        else:
-            dw_dn = torch.zeros((E, d, F), **f32)
-            dw_up = torch.zeros((E, 2 * F, d), **f32)
-        ups = [e.up_proj.weight for e in mod.experts]
-        dns = [e.down_proj.weight for e in mod.experts]
-        g_up = [dw_up[i].to(ups[i].dtype) if ctx.needs_input_grad[4 + i] else None for i in range(n_exp)]
-        g_dn = [dw_dn[i].to(dns[i].dtype) if ctx.needs_input_grad[4 + n_exp + i] else None for i in range(n_exp)]
+        g_up, g_dn = _expert_parameter_grads(mod, d_y, d_up, h_save, x_rows, pad_start, ctx.shape,
+                                             ctx.needs_input_grad[4:])
         g_x = d_x.to(ctx.x_dtype).view(ctx.x_shape) if ctx.needs_input_grad[1] else None
         g_wr = d_wr.to(mod.router.weight.dtype) if ctx.needs_input_grad[3] else None
         return (None, g_x, None, g_wr, *g_up, *g_dn)
+
+
+class SparseMoEBlock(nn.Module):
+    """A layer's expert half: ``x + moe(moe_norm(x))`` (src/mcl4_coe/backbone.py:1269), with an
+    optional norm, gate and scale on the way back, the norms and the sum by ``residual_norm``::
+
+        y = x + branch_scale * act(gate) * post_norm(moe(moe_norm(x)))
+
+    ``forward(x, valid=None)`` returns ``(y, aux_loss, router_z_loss, counts)``; with
+    ``next_norm`` (the next block's norm weight) ``y`` becomes ``(y, next_norm(y))`` of the
+    same kernel, and ``normed`` takes such a norm in from the block before.
+    """
+
+    def __init__(self, config: Any, moe: SparseMoE | None = None) -> None:
+        super().__init__()
+        d_model = int(config.d_model)
+        self.eps = float(getattr(config, "norm_eps", 1e-6))
+        self.branch_scale = float(getattr(config, "branch_scale", 1.0))
+        self.residual_gate = str(getattr(config, "residual_gate", "none"))
+        if self.residual_gate not in RESIDUAL_GATES:
+            raise ValueError(f"residual_gate must be one of {RESIDUAL_GATES}")
+        self.moe = SparseMoE(config) if moe is None else moe
+        self.moe_norm = nn.Parameter(torch.ones(d_model))
+        self.post_norm = nn.Parameter(torch.ones(d_model)) if bool(getattr(config, "post_norm", False)) else None
+        self.gate = nn.Parameter(torch.ones(d_model)) if self.residual_gate != "none" else None
+
+    def forward(self, x: Tensor, valid: Tensor | None = None, *, normed: Tensor | None = None,
+                next_norm: Tensor | None = None):
+        if normed is None:
+            _, normed = residual_norm(x, pre_weight=self.moe_norm, eps=self.eps, norm_dtype=torch.bfloat16)
+        out, aux, z, counts = self.moe(normed, valid)
+        y, following = residual_norm(
+            x, out, post_weight=self.post_norm, gate=self.gate,
+            gate_activation="none" if self.residual_gate in ("none", "linear") else self.residual_gate,
+            pre_weight=next_norm, branch_scale=self.branch_scale, eps=self.eps)
+        return (y if next_norm is None else (y, following)), aux, z, counts

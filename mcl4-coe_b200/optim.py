@@ -129,3 +129,109 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
     args.grad_scale = _ptr(grad_scale)
     _launch(dev, "mcl4moe_adamw_step", _lib.load().mcl4moe_adamw_step, ctypes.byref(args))
     torch.autograd.graph.increment_version([t for tensors in written.values() for t in tensors])
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW whose step is one ``adamw_step`` call per parameter group, device and pair of types.
+
+    ``state_bits`` 8 keeps the moments in 8 bits (``adamw_step`` says how), which takes
+    2.03 instead of 8 bytes a parameter; ``master_weights`` gives bf16 / fp16 parameters
+    float32 masters.  ``step(grad_scale=t)`` multiplies the gradients by the device scalar
+    ``t`` (clipping).  ``lr`` may be a float32 tensor on the parameters' device.
+
+    ``capturable`` keeps one step count per group and device in device memory, so that a
+    captured step goes on counting when it is replayed; a replay does not go through torch,
+    so the parameters' versions stand still and an NVFP4 weight cache has to be told
+    (``invalidate_cache``).
+    """
+
+    def __init__(self, params, lr: float | Tensor = 1e-3, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
+                 weight_decay: float = 1e-2, *, state_bits: int = 32, master_weights: bool = False, seed: int = 0,
+                 capturable: bool = False) -> None:
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
+        if not isinstance(lr, Tensor) and not lr >= 0.0:
+            raise ValueError(f"lr must not be negative, got {lr}")
+        if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
+            raise ValueError(f"betas must be in [0, 1), got {betas}")
+        if not eps >= 0.0 or not weight_decay >= 0.0:
+            raise ValueError(f"eps and weight_decay must not be negative, got {eps} and {weight_decay}")
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay,
+                                      state_bits=state_bits, master_weights=master_weights, seed=int(seed),
+                                      capturable=bool(capturable)))
+
+    def _new_state(self, p: Tensor, group: dict) -> dict:
+        if not p.is_contiguous():
+            raise ValueError("AdamW takes contiguous parameters")
+        state: dict = {"step": 0}
+        if group["state_bits"] == 8:
+            blocks = -(-p.numel() // STATE_BLOCK)
+            state["exp_avg"] = torch.zeros_like(p, dtype=torch.float8_e4m3fn)
+            state["exp_avg_sq"] = torch.zeros_like(p, dtype=torch.float8_e5m2)
+            state["exp_avg_scale"] = torch.ones(blocks, dtype=torch.float32, device=p.device)
+            state["exp_avg_sq_scale"] = torch.ones(blocks, dtype=torch.float32, device=p.device)
+        else:
+            state["exp_avg"] = torch.zeros_like(p, dtype=torch.float32)
+            state["exp_avg_sq"] = torch.zeros_like(p, dtype=torch.float32)
+        if group["master_weights"] and p.dtype != torch.float32:
+            state["master"] = p.detach().to(torch.float32)
+        return state
+
+    @torch.no_grad()
+    def step(self, closure=None, *, grad_scale: Tensor | None = None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        place = 0  # a parameter's number in the optimizer keys its noise
+        for group in self.param_groups:
+            calls: dict = {}
+            for p in group["params"]:
+                place += 1
+                if p.grad is None:
+                    continue
+                if p.grad.is_sparse:
+                    raise ValueError("AdamW takes dense gradients")
+                state = self.state[p]
+                if not state:
+                    state.update(self._new_state(p, group))
+                if not group["capturable"]:
+                    state["step"] += 1
+                key = (p.device, p.dtype, p.grad.dtype, state["step"], "master" in state)
+                calls.setdefault(key, []).append((p, state, place - 1))
+            counts = self._device_counts(group, calls)
+            for (device, _, _, step, master), items in calls.items():
+                states = [s for _, s, _ in items]
+                eight = group["state_bits"] == 8
+                adamw_step([p for p, _, _ in items], [p.grad for p, _, _ in items],
+                           [s["exp_avg"] for s in states], [s["exp_avg_sq"] for s in states],
+                           step=counts[device] if counts else step, lr=group["lr"], betas=group["betas"],
+                           eps=group["eps"], weight_decay=group["weight_decay"],
+                           exp_avg_scales=[s["exp_avg_scale"] for s in states] if eight else None,
+                           exp_avg_sq_scales=[s["exp_avg_sq_scale"] for s in states] if eight else None,
+                           masters=[s["master"] for s in states] if master else None, grad_scale=grad_scale,
+                           seed=group["seed"], indices=[i for _, _, i in items])
+        return loss
+
+    def _device_counts(self, group: dict, calls: dict) -> dict | None:
+        """capturable: the group's step count on each device, moved on by one."""
+        if not group["capturable"]:
+            return None
+        counts = group.setdefault("step_counts", {})
+        for device in {key[0] for key in calls}:
+            if str(device) not in counts:
+                counts[str(device)] = torch.zeros((), dtype=torch.int64, device=device)
+            counts[str(device)] += 1
+        return {key[0]: counts[str(key[0])] for key in calls}
+
+    def load_state_dict(self, state_dict: dict) -> None:
+        """As ``torch.optim.Optimizer``'s, which would cast the moments to the parameters' type."""
+        super().load_state_dict(state_dict)
+        saved = [i for g in state_dict["param_groups"] for i in g["params"]]
+        for i, p in zip(saved, (p for g in self.param_groups for p in g["params"])):
+            for name, value in state_dict["state"].get(i, {}).items():
+                if isinstance(value, Tensor):
+                    self.state[p][name] = value.detach().to(p.device, copy=True)
+        for group in self.param_groups:
+            if "step_counts" in group:
+                group["step_counts"] = {d: t.detach().to(d, copy=True) for d, t in group["step_counts"].items()}

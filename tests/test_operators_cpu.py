@@ -141,3 +141,32 @@ def test_library_refuses(moe_pkg):
     numels, null = array("q", [5]), array("Q", [0])
     at = null.buffer_info()[0]
     assert adam(n=1, numels=numels.buffer_info()[0], params=at, grads=at, exp_avgs=at, exp_avg_sqs=at) == L.ERR_INVALID
+
+
+def test_config_of_scored_routing_and_block(moe_pkg):
+    base = dict(d_model=256, expert_hidden_dim=256, num_experts=8, top_k=2)
+    for bad in (dict(score_function="relu"), dict(group_score="sum"), dict(expert_groups=3), dict(expert_groups=0),
+                dict(expert_groups=4, top_expert_groups=5), dict(expert_groups=8, top_expert_groups=1),
+                dict(residual_gate="relu")):
+        with pytest.raises(ValueError):
+            moe_pkg.MoEConfig(**base, **bad)
+    layer = moe_pkg.SparseMoE(moe_pkg.MoEConfig(**base))
+    assert layer._routing_variant(None, None, None) is None and layer.balance_bias is None
+    for kw in (dict(score_function="sigmoid"), dict(expert_groups=4, top_expert_groups=2), dict(routed_scale=2.0),
+               dict(balance_bias=True)):
+        assert moe_pkg.SparseMoE(moe_pkg.MoEConfig(**base, **kw))._routing_variant(None, None, None) == "scored"
+    with pytest.raises(ValueError, match="balance_bias"):
+        layer.update_balance_bias(torch.zeros(8))
+    block = moe_pkg.SparseMoEBlock(moe_pkg.MoEConfig(**base))
+    assert {"moe_norm", "moe.router.weight"} <= set(block.state_dict())
+    assert block.post_norm is None and block.gate is None
+
+
+def test_optimizer_arguments(moe_pkg):
+    p = torch.nn.Parameter(torch.zeros(3))
+    for bad in (dict(state_bits=4), dict(lr=-1e-3), dict(betas=(1.0, 0.9)), dict(eps=-1.0), dict(weight_decay=-0.1)):
+        with pytest.raises(ValueError):
+            moe_pkg.AdamW([p], **bad)
+    opt = moe_pkg.AdamW([p])
+    opt.step()  # nothing has a gradient
+    assert not opt.state
