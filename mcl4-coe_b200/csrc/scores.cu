@@ -11,7 +11,13 @@
 //
 // The ids are those of exact arithmetic: the float32 keys carry an error bound, and a
 // row whose order hangs on less than that bound (neighbouring picks, or the border
-// between open and closed groups) is selected again in float64.
+// between open and closed groups) is selected again in float64, by a whole warp.
+//
+// A row is a few hundred bytes and a few hundred instructions, so issue slots bound it, not HBM:
+// a row gets 8, 16 or 32 lanes with up to 8 experts in each one's registers (16 above 256
+// experts), so that the butterflies and the pops of the k rounds serve up to four rows at once.
+#include <type_traits>
+
 #include <cuda_fp16.h>
 
 #include "kernels.cuh"
@@ -20,7 +26,8 @@ namespace mcl4 {
 namespace {
 
 constexpr unsigned kFull = 0xffffffffu;
-constexpr int kScoreWarps = 4;        // rows in flight per CTA, one warp each
+constexpr int kScoreWarps = 4;        // of a CTA
+constexpr int kScoreWarpsOne = 16;    // of the one CTA that a small batch fits into
 constexpr int kMaxScoreExperts = 512;
 
 enum { kSoftmax = 0, kSigmoid = 1 };
@@ -37,11 +44,16 @@ struct ScoreArgs {
   int32_t* idx;
   float* w;
   int32_t* counts;
+  int one;   // a single CTA: it writes the counts itself
+  int wide;  // rows allow 16-byte loads
 };
 
 __device__ __forceinline__ float load_logit(const float* p) { return __ldg(p); }
 __device__ __forceinline__ float load_logit(const uint16_t* p) { return bf16_to_f32(__ldg(p)); }
 __device__ __forceinline__ float load_logit(const __half* p) { return __half2float(__ldg(p)); }
+__device__ __forceinline__ float logit_value(float v) { return v; }
+__device__ __forceinline__ float logit_value(uint16_t v) { return bf16_to_f32(v); }
+__device__ __forceinline__ float logit_value(__half v) { return __half2float(v); }
 __device__ __forceinline__ void store_grad(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store_grad(uint16_t* p, float v) { *p = f32_to_bf16(v); }
 __device__ __forceinline__ void store_grad(__half* p, float v) { *p = __float2half_rn(v); }
@@ -61,157 +73,113 @@ __device__ __forceinline__ float value_of(uint32_t o) {
   return __uint_as_float(o & 0x80000000u ? o & 0x7FFFFFFFu : ~o);
 }
 
-__device__ __forceinline__ uint32_t warp_max(uint32_t v) { return __reduce_max_sync(kFull, v); }
-__device__ __forceinline__ uint64_t warp_max(uint64_t v) {
+// Butterflies over the LPT lanes of a row.
+template <int LPT, typename F, typename Op>
+__device__ __forceinline__ F lanes(F v, Op op) {
+#pragma unroll
+  for (int o = LPT / 2; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(kFull, v, o));
+  return v;
+}
+template <int LPT, typename F>
+__device__ __forceinline__ F lanes_sum(F v) {
+  return lanes<LPT>(v, [](F a, F b) { return a + b; });
+}
+template <int LPT>
+__device__ __forceinline__ float lanes_fmax(float v) {
+  return lanes<LPT>(v, [](float a, float b) { return fmaxf(a, b); });
+}
+template <int LPT>
+__device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
+  if (LPT == 32) return __reduce_max_sync(kFull, v);
+  return lanes<LPT>(v, [](uint32_t a, uint32_t b) { return max(a, b); });
+}
+__device__ __forceinline__ uint64_t warp_max64(uint64_t v) {
   const uint32_t hi = __reduce_max_sync(kFull, uint32_t(v >> 32));
   const uint32_t lo = __reduce_max_sync(kFull, uint32_t(v >> 32) == hi ? uint32_t(v) : 0u);
   return uint64_t(hi) << 32 | lo;
 }
-__device__ __forceinline__ uint64_t warp_min(uint64_t v) { return ~warp_max(~v); }
-__device__ __forceinline__ uint32_t warp_min(uint32_t v) { return __reduce_min_sync(kFull, v); }
 
-template <typename F>
-__device__ __forceinline__ F warp_sum(F v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
-  return v;
-}
-__device__ __forceinline__ float warp_fmax(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kFull, v, o));
-  return v;
-}
+__device__ __forceinline__ float minus_inf() { return __uint_as_float(0xFF800000u); }
 
-template <typename F>
-struct Order;
-template <>
-struct Order<float> {
-  using U = uint32_t;
+// What a warp keeps in shared memory for its rows (32 / LPT of them): values and group values of
+// rows whose groups do not fall on lanes, the picks, and the picks' keys.
+struct ScoreScratch {
+  double* val;     // [slots] (float32 values of the rows side by side, or one row's float64 values)
+  uint64_t* ord;   // [slots]
+  uint8_t* open;   // [slots]
+  int32_t* pick;   // [rows][32]
+  uint32_t* top;   // [rows][33]
 };
-template <>
-struct Order<double> {
-  using U = uint64_t;
-};
-
-template <typename F>
-__device__ __forceinline__ F minus_inf() {
-  return F(__int_as_float(0xFF800000));
+__host__ __device__ inline int score_slots(int E, int lpt) { return (32 / lpt * E + 15) / 16 * 16; }
+__host__ __device__ inline size_t score_scratch_bytes(int E, int lpt) {
+  return size_t(score_slots(E, lpt)) * 17 + size_t(32 / lpt) * 65 * 4 + 12;
 }
-__device__ __forceinline__ float exp_of(float v) { return expf(v); }
-__device__ __forceinline__ double exp_of(double v) { return exp(v); }
 
-// Selects the row's experts: lane j < k returns its pick (-1: none).  F = float: `close`
-// tells that the order is within the error bound of the keys.
-template <typename F, int NPL>
-__device__ __forceinline__ int select_row(const ScoreArgs& a, const float (&l)[NPL], float row_max, float bias_max,
-                                          char* smem, bool& close) {
-  using U = typename Order<F>::U;
+// One row by a whole warp in float64, straightforwardly: the picks (-1: none) go to `pick`.
+template <typename L>
+__device__ __noinline__ void select_exact(const ScoreArgs& a, const L* row, ScoreScratch s, int32_t* pick) {
   const int lane = threadIdx.x & 31;
   const int gsize = a.E / a.groups;
   const bool sums = a.groups > 1 && a.group_score == kGroupTop2 && gsize > 1;
-  const bool values = a.bias != nullptr || sums;  // else the logits alone give the order, exactly
-  // |key - exact key| <= rel * (|key| + bias) with rel = 2^-21.5 for the sigmoid (exp 2 ulp, sum and
-  // quotient half an ulp each) and 2^-17.2 for the softmax (l - max rounds to half an ulp of up to
-  // 104); twice that for a comparison, with room to spare; 1e-36 covers denormal scores.
-  const float rel = a.score == kSigmoid ? 9.5367431640625e-07f : 1.52587890625e-05f;
-  auto near = [&](U hi, U lo) {
-    if (sizeof(F) == 8 || !values || lo == 0) return false;
-    const float x = value_of(uint32_t(hi)), y = value_of(uint32_t(lo));
-    return x - y <= rel * (fabsf(x) + fabsf(y) + 8.f * bias_max) + 1e-36f;
-  };
-  F key[NPL];
-  F val[NPL];
-  F z = F(1);
-  if (values && a.score == kSoftmax) {
-    F part = F(0);
-#pragma unroll
-    for (int i = 0; i < NPL; ++i)
-      if (lane * NPL + i < a.E) part += exp_of(F(l[i]) - F(row_max));
-    z = warp_sum(part);
+  const double none = double(minus_inf());
+  double top = none, z = 1.0;
+  if (a.score == kSoftmax) {
+    for (int e = lane; e < a.E; e += 32) top = fmax(top, double(load_logit(row + e)));
+    top = lanes<32>(top, [](double x, double y) { return fmax(x, y); });
+    double part = 0.0;
+    for (int e = lane; e < a.E; e += 32) part += exp(double(load_logit(row + e)) - top);
+    z = lanes_sum<32>(part);
   }
-#pragma unroll
-  for (int i = 0; i < NPL; ++i) {
-    const int e = lane * NPL + i;
-    key[i] = val[i] = minus_inf<F>();
-    if (e >= a.E) continue;
-    key[i] = F(l[i]);
-    if (!values) continue;
-    const F s = a.score == kSigmoid ? F(1) / (F(1) + exp_of(-F(l[i]))) : exp_of(F(l[i]) - F(row_max)) / z;
-    const F b = a.bias != nullptr ? F(__ldg(a.bias + e)) : F(0);
-    if (l[i] != minus_inf<float>()) val[i] = a.bias != nullptr ? s + b : s;
-    if (a.bias != nullptr) key[i] = val[i];
+  __syncwarp();
+  for (int e = lane; e < a.E; e += 32) {
+    const float lf = load_logit(row + e);
+    const double l = double(lf), score = a.score == kSigmoid ? 1.0 / (1.0 + exp(-l)) : exp(l - top) / z;
+    const double v = lf == minus_inf() ? none : a.bias != nullptr ? score + double(__ldg(a.bias + e)) : score;
+    const double key = a.bias != nullptr ? v : l;
+    s.val[e] = sums ? v : key;
+    s.ord[e] = key == none ? 0 : ordered(key);
+    s.open[e] = 1;
   }
-  close = false;
-  U ord[NPL];
-#pragma unroll
-  for (int i = 0; i < NPL; ++i) ord[i] = key[i] == minus_inf<F>() ? U(0) : ordered(key[i]);
+  __syncwarp();
   if (a.groups > 1) {
-    F* sv = reinterpret_cast<F*>(smem);
-    U* so = reinterpret_cast<U*>(smem + 8 * a.E);
-    uint8_t* open = reinterpret_cast<uint8_t*>(smem + 16 * a.E);
-#pragma unroll
-    for (int i = 0; i < NPL; ++i)
-      if (lane * NPL + i < a.E) sv[lane * NPL + i] = sums ? val[i] : key[i];
-    __syncwarp();
+    // a group's value first: the key's order is kept beside it
     for (int g = lane; g < a.groups; g += 32) {
-      F first = minus_inf<F>(), second = minus_inf<F>();
+      double first = none, second = none;
       bool nan = false;
       for (int i = 0; i < gsize; ++i) {
-        const F v = sv[g * gsize + i];
+        const double v = s.val[g * gsize + i];
         nan |= v != v;
         second = v > first ? first : (v > second ? v : second);
         first = v > first ? v : first;
       }
-      if (sums && second != minus_inf<F>()) first += second;
-      so[g] = nan ? ~U(0) : first == minus_inf<F>() ? U(0) : ordered(first);
+      if (sums && second != none) first += second;
+      s.val[g * gsize] = __longlong_as_double((long long)(nan ? ~uint64_t(0) : first == none ? 0 : ordered(first)));
     }
     __syncwarp();
-    U lowest_open = ~U(0), highest_closed = 0;
+    auto value = [&](int g) { return uint64_t(__double_as_longlong(s.val[g * gsize])); };
     for (int g = lane; g < a.groups; g += 32) {
-      const U mine = so[g];
+      const uint64_t mine = value(g);
       int rank = 0;
-      for (int h = 0; h < a.groups; ++h) rank += so[h] > mine || (so[h] == mine && h < g);
-      open[g] = rank < a.top_groups;
-      if (rank < a.top_groups) lowest_open = mine < lowest_open ? mine : lowest_open;
-      else highest_closed = mine > highest_closed ? mine : highest_closed;
-    }
-    lowest_open = warp_min(lowest_open);
-    highest_closed = warp_max(highest_closed);
-    close = near(lowest_open, highest_closed);
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < NPL; ++i) {
-      const int e = lane * NPL + i;
-      if (e < a.E && !open[e / gsize]) ord[i] = 0;
+      for (int h = 0; h < a.groups; ++h) rank += value(h) > mine || (value(h) == mine && h < g);
+      if (rank >= a.top_groups)
+        for (int i = 0; i < gsize; ++i) s.open[g * gsize + i] = 0;
     }
     __syncwarp();
   }
-  int pick = -1;
-  U before = 0;
-  const int rounds = values && sizeof(F) == 4 ? a.k + 1 : a.k;  // one more: the best key left behind
-  for (int j = 0; j < rounds; ++j) {
-    U best = 0;
-    int at = 0;
-#pragma unroll
-    for (int i = 0; i < NPL; ++i)
-      if (ord[i] > best) {
-        best = ord[i];
-        at = i;
+  for (int j = 0; j < a.k; ++j) {
+    uint64_t best = 0;
+    int at = -1;
+    for (int e = lane; e < a.E; e += 32)
+      if (s.open[e] && s.ord[e] > best) {
+        best = s.ord[e];
+        at = e;
       }
-    const U top = warp_max(best);
-    if (j > 0 && near(before, top)) close = true;
-    if (top == 0) break;
-    const int owner = __ffs(__ballot_sync(kFull, best == top)) - 1;
-    const int e = __shfl_sync(kFull, lane * NPL + at, owner);
-    if (j < a.k && lane == j) pick = e;
-    if (lane == owner) {
-#pragma unroll
-      for (int i = 0; i < NPL; ++i)
-        if (i == at) ord[i] = 0;
-    }
-    before = top;
+    const uint64_t top_key = warp_max64(best);
+    const uint32_t first = __reduce_min_sync(kFull, best == top_key && at >= 0 ? uint32_t(at) : 0xFFFFFFFFu);
+    if (lane == 0) pick[j] = top_key == 0 ? -1 : int32_t(first);
+    if (top_key != 0 && uint32_t(at) == first) s.ord[at] = 0;
+    __syncwarp();
   }
-  return pick;
 }
 
 // exp(min(l, 0)) / (1 + e^-|l|): denormal, not zero, where 1 + e^-l would overflow.
@@ -223,28 +191,95 @@ __device__ __forceinline__ float sigmoid_ratio(float l, float m) {
   return expf(fminf(l, 0.f) - fminf(m, 0.f)) * (1.f + expf(-fabsf(m))) / (1.f + expf(-fabsf(l)));
 }
 
-// The chosen score relative to the chosen ones' sum (renorm) or as it is; lanes without a pick: 0.
-// `z`, `row_max`: the softmax's, where it is not renormalised.
-__device__ __forceinline__ float chosen_share(bool has, float l, int score, int renorm, float row_max, float z) {
-  if (!renorm) {
-    if (!has) return 0.f;
-    return score == kSigmoid ? sigmoid_of(l) : expf(l - row_max) / z;
+// Vector loads and stores of a lane's experts: NPL consecutive elements from e0 on.
+template <int NPL, typename L>
+__device__ __forceinline__ void load_lane(const L* row, int e0, int E, bool wide, float (&l)[NPL]) {
+  constexpr int kPer = 16 / int(sizeof(L));
+  if constexpr (NPL % kPer == 0) {
+    if (wide && e0 < E) {  // wide: E is a multiple of NPL, so a lane's experts are all there or none
+#pragma unroll
+      for (int q = 0; q < NPL / kPer; ++q) {
+        const uint4 w = __ldg(reinterpret_cast<const uint4*>(row + e0) + q);
+        const L* v = reinterpret_cast<const L*>(&w);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) l[q * kPer + i] = logit_value(v[i]);
+      }
+      return;
+    }
   }
-  // the largest chosen logit (fmaxf passes over NaN, which the ratios carry)
-  const float top = warp_fmax(has ? l : minus_inf<float>());
-  const float r = !has ? 0.f : score == kSigmoid ? sigmoid_ratio(l, top) : expf(l - top);
-  const float sum = warp_sum(r);
-  return has ? r / sum : 0.f;
+#pragma unroll
+  for (int i = 0; i < NPL; ++i) l[i] = e0 + i < E ? load_logit(row + e0 + i) : minus_inf();
+}
+template <int NPL, typename L>
+__device__ __forceinline__ void store_lane(L* row, int e0, int E, bool wide, const float (&v)[NPL]) {
+  constexpr int kPer = 16 / int(sizeof(L));
+  if constexpr (NPL % kPer == 0) {
+    if (wide && e0 < E) {
+#pragma unroll
+      for (int q = 0; q < NPL / kPer; ++q) {
+        uint4 w;
+        L* o = reinterpret_cast<L*>(&w);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) store_grad(o + i, v[q * kPer + i]);
+        reinterpret_cast<uint4*>(row + e0)[q] = w;
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < NPL; ++i)
+    if (e0 + i < E) store_grad(row + e0 + i, v[i]);
 }
 
-template <typename L, int NPL>
-__global__ void __launch_bounds__(kScoreWarps * 32) route_scores_kernel(ScoreArgs a) {
+// The chosen scores of a row's lanes, lane j % LPT holding pick j in slot j / LPT: relative to their
+// sum (renorm), or as they are.  Slots without a pick get 0.
+template <int LPT>
+__device__ __forceinline__ void chosen_shares(const bool (&has)[32 / LPT], const float (&l)[32 / LPT], int slots, int score,
+                                              int renorm, float row_max, float z, float (&share)[32 / LPT]) {
+  if (!renorm) {
+#pragma unroll
+    for (int q = 0; q < 32 / LPT; ++q) {
+      share[q] = 0.f;
+      if (q < slots && has[q]) share[q] = score == kSigmoid ? sigmoid_of(l[q]) : expf(l[q] - row_max) / z;
+    }
+    return;
+  }
+  float top = minus_inf();  // the largest chosen logit (fmaxf passes over NaN, which the ratios carry)
+#pragma unroll
+  for (int q = 0; q < 32 / LPT; ++q)
+    if (q < slots && has[q]) top = fmaxf(top, l[q]);
+  top = lanes_fmax<LPT>(top);
+  float sum = 0.f;
+#pragma unroll
+  for (int q = 0; q < 32 / LPT; ++q) {
+    share[q] = 0.f;
+    if (q < slots && has[q]) share[q] = score == kSigmoid ? sigmoid_ratio(l[q], top) : expf(l[q] - top);
+    sum += share[q];
+  }
+  sum = lanes_sum<LPT>(sum);
+#pragma unroll
+  for (int q = 0; q < 32 / LPT; ++q)
+    if (q < slots && has[q]) share[q] /= sum;
+}
+
+template <typename L, int LPT, int NPL>
+__global__ void __launch_bounds__(kScoreWarpsOne * 32) route_scores_kernel(ScoreArgs a) {
   extern __shared__ __align__(16) char smem[];
+  constexpr int kRows = 32 / LPT;  // of a warp
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const int seg = lane / LPT, sl = lane % LPT;
+  const unsigned seg_mask = LPT == 32 ? kFull : ((1u << LPT) - 1u);
   int32_t* hist = reinterpret_cast<int32_t*>(smem);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const size_t hist_bytes = (size_t(a.E) * 4 + 15) / 16 * 16;
-  const size_t warp_bytes = (size_t(a.E) * 17 + 15) / 16 * 16;
-  char* mine = smem + hist_bytes + warp * warp_bytes;
+  ScoreScratch s;
+  {
+    const int slots = score_slots(a.E, LPT);
+    char* at = smem + (size_t(a.E) * 4 + 15) / 16 * 16 + warp * ((score_scratch_bytes(a.E, LPT) + 15) / 16 * 16);
+    s.val = reinterpret_cast<double*>(at);
+    s.ord = reinterpret_cast<uint64_t*>(at + size_t(slots) * 8);
+    s.pick = reinterpret_cast<int32_t*>(at + size_t(slots) * 16);
+    s.top = reinterpret_cast<uint32_t*>(s.pick + kRows * 32);
+    s.open = reinterpret_cast<uint8_t*>(s.top + kRows * 33);
+  }
   if (a.counts != nullptr)
     for (int e = threadIdx.x; e < a.E; e += blockDim.x) hist[e] = 0;
   float bias_max = 0.f;
@@ -253,50 +288,208 @@ __global__ void __launch_bounds__(kScoreWarps * 32) route_scores_kernel(ScoreArg
       const float b = fabsf(__ldg(a.bias + e));
       if (b <= kFltMax) bias_max = fmaxf(bias_max, b);
     }
-    bias_max = warp_fmax(bias_max);
+    bias_max = lanes_fmax<32>(bias_max);
   }
   __syncthreads();
-  for (int64_t t = int64_t(blockIdx.x) * kScoreWarps + warp; t < a.T; t += int64_t(gridDim.x) * kScoreWarps) {
-    const L* row = static_cast<const L*>(a.logits) + t * a.ld;
-    int pick = -1;
-    float share = 0.f;
-    if (a.valid == nullptr || a.valid[t] != 0) {
-      float l[NPL];
-      float row_max = minus_inf<float>();
+  const int gsize = a.E / a.groups;
+  const bool sums = a.groups > 1 && a.group_score == kGroupTop2 && gsize > 1;
+  const bool values = a.bias != nullptr || sums;  // else the logits alone give the order, exactly
+  // groups of 1, 2, 4 .. whole lanes are valued by butterflies
+  const int glanes = gsize / NPL;
+  const bool on_lanes = a.groups > 1 && gsize % NPL == 0 && (glanes & (glanes - 1)) == 0;
+  const bool soft = a.score == kSoftmax && (values || !a.renorm);
+  const bool wide = a.wide && a.E % NPL == 0;
+  // |key - exact key| <= rel / 2 * (|key| + bias): sigmoid 2^-20.9 (exp 1 ulp, sum half an ulp, quotient
+  // 2 ulp), softmax 2^-17.2 (l - max rounds to half an ulp of up to 104); `near` adds both sides'
+  // bounds with room to spare, 1e-36 covers denormal scores.
+  const float rel = a.score == kSigmoid ? 1.9073486328125e-06f : 1.52587890625e-05f;
+  auto near = [&](uint32_t hi, uint32_t lo) {
+    if (!values || lo == 0) return false;
+    const float x = value_of(hi), y = value_of(lo);
+    return x - y <= rel * (fabsf(x) + fabsf(y) + 8.f * bias_max) + 1e-36f;
+  };
+  const int e0 = sl * NPL;
+  float bias[NPL];
+#pragma unroll
+  for (int i = 0; i < NPL; ++i) bias[i] = a.bias != nullptr && e0 + i < a.E ? __ldg(a.bias + e0 + i) : 0.f;
+  const int slots = (a.k + LPT - 1) / LPT;
+  int32_t* pick = s.pick + seg * 32;
+  uint32_t* tops = s.top + seg * 33;
+
+  for (int64_t base = (int64_t(blockIdx.x) * warps + warp) * kRows; base < a.T; base += int64_t(gridDim.x) * warps * kRows) {
+    const int64_t t = base + seg;
+    const bool live = t < a.T && (a.valid == nullptr || a.valid[t] != 0);
+    const L* row = static_cast<const L*>(a.logits) + (live ? t : 0) * a.ld;
+    float l[NPL];
+    if (live) {
+      load_lane(row, e0, a.E, wide, l);
+    }
+#pragma unroll
+    for (int i = 0; i < NPL; ++i)
+      if (!live) l[i] = minus_inf();
+    float row_max = 0.f, z = 1.f;
+    if (soft) {
+      row_max = l[0];
+#pragma unroll
+      for (int i = 1; i < NPL; ++i) row_max = fmaxf(row_max, l[i]);
+      row_max = lanes_fmax<LPT>(row_max);
+    }
+    float val[NPL];  // the scores, with the bias: what keys and group values are made of
+    if (values || soft) {
+      float part = 0.f;
 #pragma unroll
       for (int i = 0; i < NPL; ++i) {
-        const int e = lane * NPL + i;
-        l[i] = e < a.E ? load_logit(row + e) : minus_inf<float>();
-        row_max = fmaxf(row_max, l[i]);
+        if (a.score == kSigmoid) {
+          val[i] = __fdividef(1.f, 1.f + expf(-l[i]));
+        } else {
+          val[i] = e0 + i < a.E ? expf(l[i] - row_max) : 0.f;
+          part += val[i];
+        }
       }
-      row_max = warp_fmax(row_max);
-      bool close;
-      pick = select_row<float, NPL>(a, l, row_max, bias_max, mine, close);
-      if (close) {
-        bool ignored;
-        pick = select_row<double, NPL>(a, l, row_max, bias_max, mine, ignored);
-      }
-      float z = 1.f;
-      if (a.score == kSoftmax && !a.renorm) {
-        float part = 0.f;
+      if (soft) z = lanes_sum<LPT>(part);
+      const float scale = soft ? 1.f / z : 1.f;
+#pragma unroll
+      for (int i = 0; i < NPL; ++i) val[i] = l[i] == minus_inf() ? minus_inf() : val[i] * scale + bias[i];
+    }
+    uint32_t ord[NPL];
+#pragma unroll
+    for (int i = 0; i < NPL; ++i) {
+      const float key = a.bias != nullptr ? val[i] : l[i];
+      ord[i] = key == minus_inf() || e0 + i >= a.E ? 0u : ordered(key);
+    }
+    bool close = false;
+    if (a.groups > 1) {
+      bool open_all = true;
+      if (on_lanes) {
+        float first = minus_inf(), second = minus_inf();
+        bool nan = false;
+#pragma unroll
+        for (int i = 0; i < NPL; ++i) {
+          const float v = e0 + i < a.E ? (sums ? val[i] : a.bias != nullptr ? val[i] : l[i]) : minus_inf();
+          nan |= v != v;
+          second = fmaxf(second, fminf(first, v));
+          first = fmaxf(first, v);
+        }
+        for (int o = 1; o < glanes; o <<= 1) {
+          const float f2 = __shfl_xor_sync(kFull, first, o), s2 = __shfl_xor_sync(kFull, second, o);
+          nan = __shfl_xor_sync(kFull, int(nan), o) != 0 || nan;
+          second = fmaxf(fmaxf(second, s2), fminf(first, f2));
+          first = fmaxf(first, f2);
+        }
+        if (sums && second != minus_inf()) first += second;
+        const uint32_t mine = nan ? 0xFFFFFFFFu : first == minus_inf() ? 0u : ordered(first);
+        const int g = sl / glanes;
+        uint32_t below = 0;  // the best group behind this one
+        int rank = 0;
+        for (int h = 0; h < a.groups; ++h) {
+          const uint32_t o = __shfl_sync(kFull, mine, h * glanes, LPT);
+          const bool ahead = o > mine || (o == mine && h < g);
+          rank += ahead;
+          if (!ahead && h != g) below = max(below, o);
+        }
+        open_all = rank < a.top_groups;
+        close = rank == a.top_groups - 1 && near(mine, below);
 #pragma unroll
         for (int i = 0; i < NPL; ++i)
-          if (lane * NPL + i < a.E) part += expf(l[i] - row_max);
-        z = warp_sum(part);
+          if (!open_all) ord[i] = 0;
+      } else {
+        float* sv = reinterpret_cast<float*>(s.val) + seg * a.E;
+        uint32_t* so = reinterpret_cast<uint32_t*>(s.ord) + seg * a.E;
+        uint8_t* open = s.open + seg * a.E;
+#pragma unroll
+        for (int i = 0; i < NPL; ++i)
+          if (e0 + i < a.E) sv[e0 + i] = sums ? val[i] : a.bias != nullptr ? val[i] : l[i];
+        __syncwarp();
+        for (int g = sl; g < a.groups; g += LPT) {
+          float first = minus_inf(), second = minus_inf();
+          bool nan = false;
+          for (int i = 0; i < gsize; ++i) {
+            const float v = sv[g * gsize + i];
+            nan |= v != v;
+            second = fmaxf(second, fminf(first, v));
+            first = fmaxf(first, v);
+          }
+          if (sums && second != minus_inf()) first += second;
+          so[g] = nan ? 0xFFFFFFFFu : first == minus_inf() ? 0u : ordered(first);
+        }
+        __syncwarp();
+        for (int g = sl; g < a.groups; g += LPT) {
+          const uint32_t mine = so[g];
+          uint32_t below = 0;
+          int rank = 0;
+          for (int h = 0; h < a.groups; ++h) {
+            const uint32_t o = so[h];
+            const bool ahead = o > mine || (o == mine && h < g);
+            rank += ahead;
+            if (!ahead && h != g) below = max(below, o);
+          }
+          open[g] = rank < a.top_groups;
+          close |= rank == a.top_groups - 1 && near(mine, below);
+        }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < NPL; ++i)
+          if (e0 + i < a.E && !open[(e0 + i) / gsize]) ord[i] = 0;
       }
-      const float mine_l = pick >= 0 ? load_logit(row + pick) : 0.f;
-      share = chosen_share(pick >= 0, mine_l, a.score, a.renorm, row_max, z);
     }
-    if (lane < a.k) {
-      a.idx[t * a.k + lane] = pick;
-      a.w[t * a.k + lane] = pick >= 0 ? share * a.scale : 0.f;
-      if (a.counts != nullptr && pick >= 0) atomicAdd(hist + pick, 1);
+    __syncwarp();  // the last rows' picks are read
+    for (int j = sl; j < a.k; j += LPT) pick[j] = -1;
+    __syncwarp();
+    const int rounds = values ? a.k + 1 : a.k;  // one more: the best key left behind
+    for (int j = 0; j < rounds; ++j) {
+      uint32_t best = ord[0];
+#pragma unroll
+      for (int i = 1; i < NPL; ++i) best = max(best, ord[i]);
+      const uint32_t top = lanes_max<LPT>(best);
+      const unsigned held = __ballot_sync(kFull, best == top && top != 0) >> (seg * LPT) & seg_mask;
+      if (sl == 0) tops[j] = top;
+      if (held != 0 && sl == __ffs(held) - 1) {  // the lowest lane that has it: its first such expert goes
+        int at = 0;
+#pragma unroll
+        for (int i = NPL - 1; i >= 0; --i)
+          if (ord[i] == top) at = i;
+#pragma unroll
+        for (int i = 0; i < NPL; ++i)
+          if (i == at) ord[i] = 0;
+        if (j < a.k) pick[j] = e0 + at;
+      }
+    }
+    __syncwarp();
+    for (int j = sl; j + 1 < rounds; j += LPT) close |= near(tops[j], tops[j + 1]);
+    for (unsigned again = __ballot_sync(kFull, close); again != 0;) {  // rare: in float64, by the whole warp
+      const int which = (__ffs(again) - 1) / LPT;
+      again &= ~(seg_mask << (which * LPT));
+      select_exact(a, static_cast<const L*>(a.logits) + (base + which) * a.ld, s, s.pick + which * 32);
+    }
+    __syncwarp();
+    int id[kRows];
+    bool has[kRows];
+    float lc[kRows], share[kRows];
+#pragma unroll
+    for (int q = 0; q < kRows; ++q) {
+      const int j = q * LPT + sl;
+      id[q] = q < slots && j < a.k ? pick[j] : -1;
+      has[q] = id[q] >= 0;
+      lc[q] = has[q] ? load_logit(row + id[q]) : 0.f;
+    }
+    chosen_shares<LPT>(has, lc, slots, a.score, a.renorm, row_max, z, share);
+    if (t < a.T) {
+#pragma unroll
+      for (int q = 0; q < kRows; ++q) {
+        const int j = q * LPT + sl;
+        if (q >= slots || j >= a.k) continue;
+        a.idx[t * a.k + j] = id[q];
+        a.w[t * a.k + j] = has[q] ? share[q] * a.scale : 0.f;
+        if (a.counts != nullptr && has[q]) atomicAdd(hist + id[q], 1);
+      }
     }
   }
   if (a.counts == nullptr) return;
   __syncthreads();
-  for (int e = threadIdx.x; e < a.E; e += blockDim.x)
-    if (hist[e] != 0) atomicAdd(a.counts + e, hist[e]);  // whole numbers: the order does not matter
+  for (int e = threadIdx.x; e < a.E; e += blockDim.x) {
+    if (a.one) a.counts[e] = hist[e];
+    else if (hist[e] != 0) atomicAdd(a.counts + e, hist[e]);  // whole numbers: the order does not matter
+  }
 }
 
 struct ScoreBwdArgs {
@@ -305,45 +498,80 @@ struct ScoreBwdArgs {
   const int32_t* idx;
   const float* d_w;
   int T, E, k;
-  int score, renorm;
+  int score, renorm, wide;
   float scale;
   void* d_logits;
 };
 
-// One warp per row.  With r the weights before the scale, d = scale * d_w and c = sum r d:
+// With r the weights before the scale, d = scale * d_w and c = sum r d:
 //   renormalised:  dl = r (d - c) [* (1 - s) for the sigmoid] at the chosen, 0 elsewhere
 //   sigmoid:       dl = d s (1 - s) at the chosen
 //   softmax:       dl = p (d at the chosen - c) everywhere
-template <typename L>
+template <typename L, int LPT, int NPL>
 __global__ void __launch_bounds__(kScoreWarps * 32) route_scores_bwd_kernel(ScoreBwdArgs a) {
+  constexpr int kRows = 32 / LPT;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int64_t t = int64_t(blockIdx.x) * kScoreWarps + warp; t < a.T; t += int64_t(gridDim.x) * kScoreWarps) {
-    const L* row = static_cast<const L*>(a.logits) + t * a.ld;
-    L* out = static_cast<L*>(a.d_logits) + t * a.E;
-    const int pick = lane < a.k ? a.idx[t * a.k + lane] : -1;
-    const bool has = pick >= 0 && pick < a.E;
-    const bool any = __any_sync(kFull, has);
-    const bool dense = a.score == kSoftmax && !a.renorm && any;
-    float row_max = minus_inf<float>(), z = 1.f;
-    if (dense) {
-      for (int e = lane; e < a.E; e += 32) row_max = fmaxf(row_max, load_logit(row + e));
-      row_max = warp_fmax(row_max);
-      float part = 0.f;
-      for (int e = lane; e < a.E; e += 32) part += expf(load_logit(row + e) - row_max);
-      z = warp_sum(part);
+  const int seg = lane / LPT, sl = lane % LPT, e0 = sl * NPL;
+  const int slots = (a.k + LPT - 1) / LPT;
+  const bool wide = a.wide && a.E % NPL == 0;
+  for (int64_t base = (int64_t(blockIdx.x) * kScoreWarps + warp) * kRows; base < a.T;
+       base += int64_t(gridDim.x) * kScoreWarps * kRows) {
+    const int64_t t = base + seg;
+    const bool live = t < a.T;
+    const L* row = static_cast<const L*>(a.logits) + (live ? t : 0) * a.ld;
+    L* out = static_cast<L*>(a.d_logits) + (live ? t : 0) * a.E;
+    int id[kRows];
+    bool has[kRows];
+    float lc[kRows], d[kRows], share[kRows];
+    bool any = false;
+#pragma unroll
+    for (int q = 0; q < kRows; ++q) {
+      const int j = q * LPT + sl;
+      id[q] = live && q < slots && j < a.k ? a.idx[t * a.k + j] : -1;
+      has[q] = id[q] >= 0 && id[q] < a.E;
+      any |= has[q];
     }
-    const float l = has ? load_logit(row + pick) : 0.f;
-    const float d = has ? a.d_w[t * a.k + lane] * a.scale : 0.f;
-    const float r = any ? chosen_share(has, l, a.score, a.renorm, row_max, z) : 0.f;
-    const float c = warp_sum(has ? r * d : 0.f);
-    for (int e = lane; e < a.E; e += 32)
-      store_grad(out + e, dense ? -c * (expf(load_logit(row + e) - row_max) / z) : 0.f);
+#pragma unroll
+    for (int q = 0; q < kRows; ++q) {
+      lc[q] = has[q] ? load_logit(row + id[q]) : 0.f;
+      d[q] = has[q] ? a.d_w[t * a.k + q * LPT + sl] * a.scale : 0.f;
+    }
+    // the dense gradient reads the whole row; a row without picks keeps zeros whatever it holds
+    any = lanes<LPT>(int(any), [](int x, int y) { return x | y; }) != 0;
+    float g[NPL];
+    float row_max = 0.f, z = 1.f;
+    const bool dense = a.score == kSoftmax && !a.renorm;
+    if (dense) {
+      load_lane(row, e0, a.E, wide, g);
+      row_max = g[0];
+#pragma unroll
+      for (int i = 1; i < NPL; ++i) row_max = fmaxf(row_max, g[i]);
+      row_max = lanes_fmax<LPT>(row_max);
+      float part = 0.f;
+#pragma unroll
+      for (int i = 0; i < NPL; ++i) {
+        g[i] = e0 + i < a.E ? expf(g[i] - row_max) : 0.f;
+        part += g[i];
+      }
+      z = lanes_sum<LPT>(part);
+    }
+    chosen_shares<LPT>(has, lc, slots, a.score, a.renorm, row_max, z, share);
+    float c = 0.f;
+#pragma unroll
+    for (int q = 0; q < kRows; ++q)
+      if (has[q]) c += share[q] * d[q];
+    c = lanes_sum<LPT>(c);
+    const float factor = -c / z;
+#pragma unroll
+    for (int i = 0; i < NPL; ++i) g[i] = dense && any ? factor * g[i] : 0.f;
+    if (live) store_lane(out, e0, a.E, wide, g);
     __syncwarp();  // the chosen entries go over the row written above
-    if (has) {
-      float g;
-      if (a.score == kSoftmax) g = r * (d - c);
-      else g = (a.renorm ? r * (d - c) : r * d) * sigmoid_of(-l);  // 1 - sigmoid(l) = sigmoid(-l)
-      store_grad(out + pick, g);
+#pragma unroll
+    for (int q = 0; q < kRows; ++q) {
+      if (!has[q]) continue;
+      float v = a.score == kSoftmax || a.renorm ? share[q] * (d[q] - c) : share[q] * d[q];
+      if (a.score == kSigmoid) v *= sigmoid_of(-lc[q]);  // 1 - sigmoid(l) = sigmoid(-l)
+      store_grad(out + id[q], v);
     }
   }
 }
@@ -354,15 +582,59 @@ int check_scores(int64_t T, int E, int k, int dtype, int score) {
   return MCL4MOE_OK;
 }
 
+// Lanes of a row and experts of a lane: 8 lanes up to 64 experts, 16 up to 128, else 32.
+template <typename F>
+void score_shape(int E, F&& f) {
+  using std::integral_constant;
+  const auto pick = [&](auto lpt, auto npl) { f(lpt, npl); };
+  if (E <= 8) pick(integral_constant<int, 8>{}, integral_constant<int, 1>{});
+  else if (E <= 16) pick(integral_constant<int, 8>{}, integral_constant<int, 2>{});
+  else if (E <= 32) pick(integral_constant<int, 8>{}, integral_constant<int, 4>{});
+  else if (E <= 64) pick(integral_constant<int, 8>{}, integral_constant<int, 8>{});
+  else if (E <= 128) pick(integral_constant<int, 16>{}, integral_constant<int, 8>{});
+  else if (E <= 256) pick(integral_constant<int, 32>{}, integral_constant<int, 8>{});
+  else pick(integral_constant<int, 32>{}, integral_constant<int, 16>{});
+}
+
 template <typename L>
-cudaError_t launch_scores(const ScoreArgs& a, int grid, size_t smem, cudaStream_t s) {
-  const dim3 block(kScoreWarps * 32);
-  if (a.E <= 32) route_scores_kernel<L, 1><<<grid, block, smem, s>>>(a);
-  else if (a.E <= 64) route_scores_kernel<L, 2><<<grid, block, smem, s>>>(a);
-  else if (a.E <= 128) route_scores_kernel<L, 4><<<grid, block, smem, s>>>(a);
-  else if (a.E <= 256) route_scores_kernel<L, 8><<<grid, block, smem, s>>>(a);
-  else route_scores_kernel<L, 16><<<grid, block, smem, s>>>(a);
-  return cudaGetLastError();
+bool rows_wide(const void* p, int64_t ld) {
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld * int64_t(sizeof(L)) % 16 == 0;
+}
+
+template <typename L>
+int launch_scores(ScoreArgs a, cudaStream_t stream) {
+  int st = MCL4MOE_OK;
+  score_shape(a.E, [&](auto lpt, auto npl) {
+    constexpr int kLpt = decltype(lpt)::value, kNpl = decltype(npl)::value;
+    a.wide = rows_wide<L>(a.logits, a.ld);
+    // a batch that one CTA's warps hold in one pass: no counts to clear beforehand
+    a.one = a.T <= kScoreWarpsOne * (32 / kLpt);
+    const int warps = a.one ? (a.T + 32 / kLpt - 1) / (32 / kLpt) : kScoreWarps;
+    const int64_t blocks = (a.T + int64_t(warps) * (32 / kLpt) - 1) / (int64_t(warps) * (32 / kLpt));
+    const int64_t most = int64_t(8) * num_sms();
+    const size_t smem = (size_t(a.E) * 4 + 15) / 16 * 16 + warps * ((score_scratch_bytes(a.E, kLpt) + 15) / 16 * 16);
+    static std::atomic<uint64_t> raised{0};
+    if (!raise_smem_limit(route_scores_kernel<L, kLpt, kNpl>, 200 * 1024, raised) ||
+        (!a.one && a.counts != nullptr && cudaMemsetAsync(a.counts, 0, sizeof(int32_t) * a.E, stream) != cudaSuccess)) {
+      st = MCL4MOE_ERR_CUDA;
+      return;
+    }
+    route_scores_kernel<L, kLpt, kNpl><<<unsigned(blocks < most ? blocks : most), warps * 32, smem, stream>>>(a);
+    if (cudaGetLastError() != cudaSuccess) st = MCL4MOE_ERR_CUDA;
+  });
+  return st;
+}
+
+template <typename L>
+int launch_scores_bwd(ScoreBwdArgs a, cudaStream_t stream) {
+  a.wide = rows_wide<L>(a.logits, a.ld) && rows_wide<L>(a.d_logits, a.E);
+  score_shape(a.E, [&](auto lpt, auto npl) {
+    constexpr int kLpt = decltype(lpt)::value, kNpl = decltype(npl)::value;
+    const int64_t blocks = (a.T + int64_t(kScoreWarps) * (32 / kLpt) - 1) / (int64_t(kScoreWarps) * (32 / kLpt));
+    const int64_t most = int64_t(16) * num_sms();
+    route_scores_bwd_kernel<L, kLpt, kNpl><<<unsigned(blocks < most ? blocks : most), kScoreWarps * 32, 0, stream>>>(a);
+  });
+  return cudaGetLastError() == cudaSuccess ? MCL4MOE_OK : MCL4MOE_ERR_CUDA;
 }
 
 }  // namespace
@@ -381,18 +653,15 @@ int mcl4moe_route_scores(const void* logits, int dtype, int64_t ld, const float*
       int64_t(top_groups) * (E / groups) < k || (T > 0 && (!logits || !topk_idx || !topk_w)) || ld < E)
     return MCL4MOE_ERR_INVALID;
   if (st != MCL4MOE_OK) return st;
-  if (counts != nullptr && cudaMemsetAsync(counts, 0, sizeof(int32_t) * E, stream) != cudaSuccess)
-    return MCL4MOE_ERR_CUDA;
-  if (T == 0) return MCL4MOE_OK;
-  ScoreArgs a{logits, ld, bias, valid, int(T), E, k, score, groups, top_groups, group_score, renorm != 0, scale,
-              topk_idx, topk_w, counts};
-  const int64_t blocks = (T + kScoreWarps - 1) / kScoreWarps;
-  const int grid = int(blocks < int64_t(16) * num_sms() ? blocks : int64_t(16) * num_sms());
-  const size_t smem = (size_t(E) * 4 + 15) / 16 * 16 + kScoreWarps * ((size_t(E) * 17 + 15) / 16 * 16);
-  cudaError_t e = dtype == 0   ? launch_scores<uint16_t>(a, grid, smem, stream)
-                  : dtype == 1 ? launch_scores<float>(a, grid, smem, stream)
-                               : launch_scores<__half>(a, grid, smem, stream);
-  return e == cudaSuccess ? MCL4MOE_OK : MCL4MOE_ERR_CUDA;
+  if (T == 0) {
+    if (counts != nullptr && cudaMemsetAsync(counts, 0, sizeof(int32_t) * E, stream) != cudaSuccess)
+      return MCL4MOE_ERR_CUDA;
+    return MCL4MOE_OK;
+  }
+  const ScoreArgs a{logits, ld, bias, valid, int(T), E, k, score, groups, top_groups, group_score, renorm != 0, scale,
+                    topk_idx, topk_w, counts, 0, 0};
+  return dtype == 0 ? launch_scores<uint16_t>(a, stream)
+                    : dtype == 1 ? launch_scores<float>(a, stream) : launch_scores<__half>(a, stream);
 }
 
 int mcl4moe_route_scores_backward(const void* logits, int dtype, int64_t ld, const int32_t* topk_idx, const float* d_w,
@@ -403,14 +672,9 @@ int mcl4moe_route_scores_backward(const void* logits, int dtype, int64_t ld, con
   if (ld < E || (T > 0 && (!logits || !topk_idx || !d_w || !d_logits))) return MCL4MOE_ERR_INVALID;
   if (st != MCL4MOE_OK) return st;
   if (T == 0) return MCL4MOE_OK;
-  ScoreBwdArgs a{logits, ld, topk_idx, d_w, int(T), E, k, score, renorm != 0, scale, d_logits};
-  const int64_t blocks = (T + kScoreWarps - 1) / kScoreWarps;
-  const int grid = int(blocks < int64_t(16) * num_sms() ? blocks : int64_t(16) * num_sms());
-  const dim3 block(kScoreWarps * 32);
-  if (dtype == 0) route_scores_bwd_kernel<uint16_t><<<grid, block, 0, stream>>>(a);
-  else if (dtype == 1) route_scores_bwd_kernel<float><<<grid, block, 0, stream>>>(a);
-  else route_scores_bwd_kernel<__half><<<grid, block, 0, stream>>>(a);
-  return cudaGetLastError() == cudaSuccess ? MCL4MOE_OK : MCL4MOE_ERR_CUDA;
+  const ScoreBwdArgs a{logits, ld, topk_idx, d_w, int(T), E, k, score, renorm != 0, 0, scale, d_logits};
+  return dtype == 0 ? launch_scores_bwd<uint16_t>(a, stream)
+                    : dtype == 1 ? launch_scores_bwd<float>(a, stream) : launch_scores_bwd<__half>(a, stream);
 }
 
 }  // extern "C"
