@@ -30,6 +30,8 @@ constexpr int kScoreWarps = 4;        // of a CTA
 constexpr int kScoreWarpsOne = 16;    // of the one CTA that a small batch fits into
 constexpr int kMaxScoreExperts = 512;
 
+constexpr int32_t kUnsure = -2;
+
 enum { kSoftmax = 0, kSigmoid = 1 };
 enum { kGroupTop2 = 0, kGroupMax = 1 };
 
@@ -59,18 +61,10 @@ __device__ __forceinline__ void store_grad(uint16_t* p, float v) { *p = f32_to_b
 __device__ __forceinline__ void store_grad(__half* p, float v) { *p = __float2half_rn(v); }
 
 // Unsigned integers in the keys' order; 0 is "not there", NaN is above +inf, -0 equals 0.
-__device__ __forceinline__ uint32_t ordered(float v) {
-  if (v != v) return 0xFFFFFFFFu;
-  const uint32_t b = __float_as_uint(__fadd_rn(v, 0.f));
-  return b & 0x80000000u ? ~b : b | 0x80000000u;
-}
 __device__ __forceinline__ uint64_t ordered(double v) {
   if (v != v) return ~uint64_t(0);
   const uint64_t b = uint64_t(__double_as_longlong(__dadd_rn(v, 0.0)));
   return b >> 63 ? ~b : b | (uint64_t(1) << 63);
-}
-__device__ __forceinline__ float value_of(uint32_t o) {
-  return __uint_as_float(o & 0x80000000u ? o & 0x7FFFFFFFu : ~o);
 }
 
 // Butterflies over the LPT lanes of a row.
@@ -88,11 +82,61 @@ template <int LPT>
 __device__ __forceinline__ float lanes_fmax(float v) {
   return lanes<LPT>(v, [](float a, float b) { return fmaxf(a, b); });
 }
+// The largest of a row's lanes (no NaN).
 template <int LPT>
-__device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
-  if (LPT == 32) return __reduce_max_sync(kFull, v);
-  return lanes<LPT>(v, [](uint32_t a, uint32_t b) { return max(a, b); });
+__device__ __forceinline__ float lanes_top(float v) {
+  if constexpr (LPT == 32) {
+    float r;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+  } else {
+    return lanes_fmax<LPT>(v);
+  }
 }
+
+// Batcher's odd-even merge sort as a list of compare-exchange pairs.
+template <int N>
+struct SortPairs {
+  int n = 0;
+  int lo[64] = {}, hi[64] = {};
+  constexpr SortPairs() {
+    for (int p = 1; p < N; p *= 2)
+      for (int k = p; k >= 1; k /= 2)
+        for (int j = k % p; j + k < N; j += 2 * k)
+          for (int i = 0; i < k && i + j + k < N; ++i)
+            if ((i + j) / (2 * p) == (i + j + k) / (2 * p)) {
+              lo[n] = i + j;
+              hi[n] = i + j + k;
+              ++n;
+            }
+  }
+};
+// Sorts a lane's keys, falling, ties by place; returns the places, four bits each, best lowest.
+template <int N>
+using Places = typename std::conditional<(N > 8), uint64_t, uint32_t>::type;
+template <int N>
+__device__ __forceinline__ Places<N> sort_lane(float (&key)[N]) {
+  constexpr SortPairs<N> pairs;
+  int at[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) at[i] = i;
+#pragma unroll
+  for (int c = 0; c < pairs.n; ++c) {
+    const int i = pairs.lo[c], j = pairs.hi[c];
+    const float a = key[i], b = key[j];
+    const int x = at[i], y = at[j];
+    const bool swap = b > a || (b == a && y < x);
+    key[i] = swap ? b : a;
+    key[j] = swap ? a : b;
+    at[i] = swap ? y : x;
+    at[j] = swap ? x : y;
+  }
+  Places<N> places = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) places |= Places<N>(at[i]) << (4 * i);
+  return places;
+}
+
 __device__ __forceinline__ uint64_t warp_max64(uint64_t v) {
   const uint32_t hi = __reduce_max_sync(kFull, uint32_t(v >> 32));
   const uint32_t lo = __reduce_max_sync(kFull, uint32_t(v >> 32) == hi ? uint32_t(v) : 0u);
@@ -102,93 +146,25 @@ __device__ __forceinline__ uint64_t warp_max64(uint64_t v) {
 __device__ __forceinline__ float minus_inf() { return __uint_as_float(0xFF800000u); }
 
 // What a warp keeps in shared memory for its rows (32 / LPT of them): values and group values of
-// rows whose groups do not fall on lanes, the picks, and the picks' keys.
+// rows whose groups do not fall on lanes, and the picks (one more: the best key left behind).
 struct ScoreScratch {
   double* val;     // [slots] (float32 values of the rows side by side, or one row's float64 values)
   uint64_t* ord;   // [slots]
   uint8_t* open;   // [slots]
-  int32_t* pick;   // [rows][32]
-  uint32_t* top;   // [rows][33]
+  int32_t* pick;   // [rows][33]
 };
 __host__ __device__ inline int score_slots(int E, int lpt) { return (32 / lpt * E + 15) / 16 * 16; }
 __host__ __device__ inline size_t score_scratch_bytes(int E, int lpt) {
-  return size_t(score_slots(E, lpt)) * 17 + size_t(32 / lpt) * 65 * 4 + 12;
-}
-
-// One row by a whole warp in float64, straightforwardly: the picks (-1: none) go to `pick`.
-template <typename L>
-__device__ __noinline__ void select_exact(const ScoreArgs& a, const L* row, ScoreScratch s, int32_t* pick) {
-  const int lane = threadIdx.x & 31;
-  const int gsize = a.E / a.groups;
-  const bool sums = a.groups > 1 && a.group_score == kGroupTop2 && gsize > 1;
-  const double none = double(minus_inf());
-  double top = none, z = 1.0;
-  if (a.score == kSoftmax) {
-    for (int e = lane; e < a.E; e += 32) top = fmax(top, double(load_logit(row + e)));
-    top = lanes<32>(top, [](double x, double y) { return fmax(x, y); });
-    double part = 0.0;
-    for (int e = lane; e < a.E; e += 32) part += exp(double(load_logit(row + e)) - top);
-    z = lanes_sum<32>(part);
-  }
-  __syncwarp();
-  for (int e = lane; e < a.E; e += 32) {
-    const float lf = load_logit(row + e);
-    const double l = double(lf), score = a.score == kSigmoid ? 1.0 / (1.0 + exp(-l)) : exp(l - top) / z;
-    const double v = lf == minus_inf() ? none : a.bias != nullptr ? score + double(__ldg(a.bias + e)) : score;
-    const double key = a.bias != nullptr ? v : l;
-    s.val[e] = sums ? v : key;
-    s.ord[e] = key == none ? 0 : ordered(key);
-    s.open[e] = 1;
-  }
-  __syncwarp();
-  if (a.groups > 1) {
-    // a group's value first: the key's order is kept beside it
-    for (int g = lane; g < a.groups; g += 32) {
-      double first = none, second = none;
-      bool nan = false;
-      for (int i = 0; i < gsize; ++i) {
-        const double v = s.val[g * gsize + i];
-        nan |= v != v;
-        second = v > first ? first : (v > second ? v : second);
-        first = v > first ? v : first;
-      }
-      if (sums && second != none) first += second;
-      s.val[g * gsize] = __longlong_as_double((long long)(nan ? ~uint64_t(0) : first == none ? 0 : ordered(first)));
-    }
-    __syncwarp();
-    auto value = [&](int g) { return uint64_t(__double_as_longlong(s.val[g * gsize])); };
-    for (int g = lane; g < a.groups; g += 32) {
-      const uint64_t mine = value(g);
-      int rank = 0;
-      for (int h = 0; h < a.groups; ++h) rank += value(h) > mine || (value(h) == mine && h < g);
-      if (rank >= a.top_groups)
-        for (int i = 0; i < gsize; ++i) s.open[g * gsize + i] = 0;
-    }
-    __syncwarp();
-  }
-  for (int j = 0; j < a.k; ++j) {
-    uint64_t best = 0;
-    int at = -1;
-    for (int e = lane; e < a.E; e += 32)
-      if (s.open[e] && s.ord[e] > best) {
-        best = s.ord[e];
-        at = e;
-      }
-    const uint64_t top_key = warp_max64(best);
-    const uint32_t first = __reduce_min_sync(kFull, best == top_key && at >= 0 ? uint32_t(at) : 0xFFFFFFFFu);
-    if (lane == 0) pick[j] = top_key == 0 ? -1 : int32_t(first);
-    if (top_key != 0 && uint32_t(at) == first) s.ord[at] = 0;
-    __syncwarp();
-  }
+  return size_t(score_slots(E, lpt)) * 17 + size_t(32 / lpt) * 33 * 4 + 12;
 }
 
 // exp(min(l, 0)) / (1 + e^-|l|): denormal, not zero, where 1 + e^-l would overflow.
-__device__ __forceinline__ float sigmoid_of(float l) { return expf(fminf(l, 0.f)) / (1.f + expf(-fabsf(l))); }
+__device__ __forceinline__ float sigmoid_of(float l) { return __fdividef(expf(fminf(l, 0.f)), 1.f + expf(-fabsf(l))); }
 
 // exp(min(l, 0) - min(m, 0)) (1 + e^-|m|) / (1 + e^-|l|) = sigmoid(l) / sigmoid(m): no underflow
 // of the ratio where both scores underflow.
 __device__ __forceinline__ float sigmoid_ratio(float l, float m) {
-  return expf(fminf(l, 0.f) - fminf(m, 0.f)) * (1.f + expf(-fabsf(m))) / (1.f + expf(-fabsf(l)));
+  return __fdividef(expf(fminf(l, 0.f) - fminf(m, 0.f)) * (1.f + expf(-fabsf(m))), 1.f + expf(-fabsf(l)));
 }
 
 // Vector loads and stores of a lane's experts: NPL consecutive elements from e0 on.
@@ -259,7 +235,122 @@ __device__ __forceinline__ void chosen_shares(const bool (&has)[32 / LPT], const
   sum = lanes_sum<LPT>(sum);
 #pragma unroll
   for (int q = 0; q < 32 / LPT; ++q)
-    if (q < slots && has[q]) share[q] /= sum;
+    if (q < slots && has[q]) share[q] = __fdividef(share[q], sum);
+}
+
+// A row whose order float32 does not settle, by a whole warp in float64: N experts a lane.  It is
+// called behind the main loop: a call inside would cost every row its register spills (270 of 790
+// instructions a pass).  One row is one warp's latency, so its loops are unrolled for it.
+template <typename L, int N>
+__device__ __noinline__ void select_exact(const ScoreArgs& a, int64_t t, ScoreScratch s, int32_t* hist) {
+  const L* row = static_cast<const L*>(a.logits) + t * a.ld;
+  int32_t* pick = s.pick;
+  const int lane = threadIdx.x & 31, e0 = lane * N;
+  const int gsize = a.E / a.groups;
+  const bool sums = a.groups > 1 && a.group_score == kGroupTop2 && gsize > 1;
+  const double none = double(minus_inf());
+  float lf[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) lf[i] = e0 + i < a.E ? load_logit(row + e0 + i) : minus_inf();
+  double val[N], top = none;
+  if (a.score == kSigmoid) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) val[i] = 1.0 / (1.0 + exp(-double(lf[i])));
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) top = fmax(top, double(lf[i]));
+    top = lanes<32>(top, [](double x, double y) { return fmax(x, y); });
+    double part = 0.0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      val[i] = e0 + i < a.E ? exp(double(lf[i]) - top) : 0.0;
+      part += val[i];
+    }
+    const double z = lanes_sum<32>(part);
+#pragma unroll
+    for (int i = 0; i < N; ++i) val[i] /= z;
+  }
+  uint64_t ord[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (a.bias != nullptr && e0 + i < a.E) val[i] += double(__ldg(a.bias + e0 + i));
+    if (lf[i] == minus_inf()) val[i] = none;
+    const double key = a.bias != nullptr ? val[i] : double(lf[i]);
+    ord[i] = key == none ? 0 : ordered(key);
+    if (!sums) val[i] = key;
+  }
+  if (a.groups > 1) {
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (e0 + i < a.E) s.val[e0 + i] = val[i];
+    __syncwarp();
+    for (int g = lane; g < a.groups; g += 32) {
+      double first = none, second = none;
+      bool nan = false;
+#pragma unroll 4
+      for (int i = 0; i < gsize; ++i) {
+        const double v = s.val[g * gsize + i];
+        nan |= v != v;
+        second = v > first ? first : (v > second ? v : second);
+        first = v > first ? v : first;
+      }
+      if (sums && second != none) first += second;
+      s.ord[g] = nan ? ~uint64_t(0) : first == none ? 0 : ordered(first);
+    }
+    __syncwarp();
+    for (int g = lane; g < a.groups; g += 32) {
+      const uint64_t mine = s.ord[g];
+      int rank = 0;
+#pragma unroll 4
+      for (int h = 0; h < a.groups; ++h) rank += s.ord[h] > mine || (s.ord[h] == mine && h < g);
+      s.open[g] = rank < a.top_groups;
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (e0 + i < a.E && !s.open[(e0 + i) / gsize]) ord[i] = 0;
+  }
+  __syncwarp();
+  for (int j = 0; j < a.k; ++j) {
+    uint64_t best = ord[0];
+    int at = 0;
+#pragma unroll
+    for (int i = 1; i < N; ++i)
+      if (ord[i] > best) {
+        best = ord[i];
+        at = i;
+      }
+    const uint64_t top_key = warp_max64(best);
+    const unsigned held = __ballot_sync(kFull, best == top_key);
+    if (lane == __ffs(held) - 1) {  // the lowest lane that has it, and its first
+      pick[j] = top_key == 0 ? -1 : e0 + at;
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (i == at) ord[i] = 0;
+    }
+  }
+  __syncwarp();
+  float row_max = 0.f, sum = 1.f;
+  if (a.score == kSoftmax && !a.renorm) {
+    row_max = float(top);
+    float part = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (e0 + i < a.E) part += expf(lf[i] - row_max);
+    sum = lanes_sum<32>(part);
+  }
+  const int32_t id = lane < a.k ? pick[lane] : -1;
+  const bool has[1] = {id >= 0};
+  const float l[1] = {has[0] ? load_logit(row + id) : 0.f};
+  float share[1];
+  chosen_shares<32>(has, l, 1, a.score, a.renorm, row_max, sum, share);
+  if (lane < a.k) {
+    a.idx[t * a.k + lane] = id;
+    a.w[t * a.k + lane] = has[0] ? share[0] * a.scale : 0.f;
+    if (a.counts != nullptr && has[0]) atomicAdd(hist + id, 1);
+  }
+  __syncwarp();
 }
 
 template <typename L, int LPT, int NPL>
@@ -277,8 +368,7 @@ __global__ void __launch_bounds__(kScoreWarpsOne * 32) route_scores_kernel(Score
     s.val = reinterpret_cast<double*>(at);
     s.ord = reinterpret_cast<uint64_t*>(at + size_t(slots) * 8);
     s.pick = reinterpret_cast<int32_t*>(at + size_t(slots) * 16);
-    s.top = reinterpret_cast<uint32_t*>(s.pick + kRows * 32);
-    s.open = reinterpret_cast<uint8_t*>(s.top + kRows * 33);
+    s.open = reinterpret_cast<uint8_t*>(s.pick + kRows * 33);
   }
   if (a.counts != nullptr)
     for (int e = threadIdx.x; e < a.E; e += blockDim.x) hist[e] = 0;
@@ -299,22 +389,21 @@ __global__ void __launch_bounds__(kScoreWarpsOne * 32) route_scores_kernel(Score
   const bool on_lanes = a.groups > 1 && gsize % NPL == 0 && (glanes & (glanes - 1)) == 0;
   const bool soft = a.score == kSoftmax && (values || !a.renorm);
   const bool wide = a.wide && a.E % NPL == 0;
-  // |key - exact key| <= rel / 2 * (|key| + bias): sigmoid 2^-20.9 (exp 1 ulp, sum half an ulp, quotient
-  // 2 ulp), softmax 2^-17.2 (l - max rounds to half an ulp of up to 104); `near` adds both sides'
+  // |key - exact key| <= rel / 2 * (|key| + bias): sigmoid 2^-20.9 (exp 1 ulp, sum half an ulp, reciprocal
+  // 1 ulp), softmax 2^-17.2 (l - max rounds to half an ulp of up to 104); `near` adds both sides'
   // bounds with room to spare, 1e-36 covers denormal scores.
   const float rel = a.score == kSigmoid ? 1.9073486328125e-06f : 1.52587890625e-05f;
-  auto near = [&](uint32_t hi, uint32_t lo) {
-    if (!values || lo == 0) return false;
-    const float x = value_of(hi), y = value_of(lo);
-    return x - y <= rel * (fabsf(x) + fabsf(y) + 8.f * bias_max) + 1e-36f;
-  };
+  // (y <= x, and where |y| > |x| it is at most |x| + (x - y); false for an infinite x or y)
+  const float near_abs = values ? rel * 8.f * bias_max + 1e-36f : -1.f, near_rel = values ? 2.f * rel : 0.f;
+  auto near = [&](float x, float y) { return x - y <= near_rel * fminf(fabsf(x), kFltMax) + near_abs; };
   const int e0 = sl * NPL;
   float bias[NPL];
 #pragma unroll
   for (int i = 0; i < NPL; ++i) bias[i] = a.bias != nullptr && e0 + i < a.E ? __ldg(a.bias + e0 + i) : 0.f;
   const int slots = (a.k + LPT - 1) / LPT;
-  int32_t* pick = s.pick + seg * 32;
-  uint32_t* tops = s.top + seg * 33;
+  int32_t* pick = s.pick + seg * 33;
+  const unsigned lower = (1u << sl) - 1u;  // the row's lanes below this one
+  bool any_unsure = false;  // rows of this warp marked for float64
 
   for (int64_t base = (int64_t(blockIdx.x) * warps + warp) * kRows; base < a.T; base += int64_t(gridDim.x) * warps * kRows) {
     const int64_t t = base + seg;
@@ -340,7 +429,7 @@ __global__ void __launch_bounds__(kScoreWarpsOne * 32) route_scores_kernel(Score
 #pragma unroll
       for (int i = 0; i < NPL; ++i) {
         if (a.score == kSigmoid) {
-          val[i] = __fdividef(1.f, 1.f + expf(-l[i]));
+          asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(val[i]) : "f"(1.f + expf(-l[i])));
         } else {
           val[i] = e0 + i < a.E ? expf(l[i] - row_max) : 0.f;
           part += val[i];
@@ -351,77 +440,71 @@ __global__ void __launch_bounds__(kScoreWarpsOne * 32) route_scores_kernel(Score
 #pragma unroll
       for (int i = 0; i < NPL; ++i) val[i] = l[i] == minus_inf() ? minus_inf() : val[i] * scale + bias[i];
     }
-    uint32_t ord[NPL];
+    float key[NPL];  // -inf: not there
+    bool close = false;
 #pragma unroll
     for (int i = 0; i < NPL; ++i) {
-      const float key = a.bias != nullptr ? val[i] : l[i];
-      ord[i] = key == minus_inf() || e0 + i >= a.E ? 0u : ordered(key);
+      key[i] = e0 + i < a.E ? (a.bias != nullptr ? val[i] : l[i]) : minus_inf();
+      close |= key[i] != key[i];  // NaN ranks first: the float64 selection knows how
     }
-    bool close = false;
     if (a.groups > 1) {
-      bool open_all = true;
       if (on_lanes) {
         float first = minus_inf(), second = minus_inf();
-        bool nan = false;
 #pragma unroll
         for (int i = 0; i < NPL; ++i) {
-          const float v = e0 + i < a.E ? (sums ? val[i] : a.bias != nullptr ? val[i] : l[i]) : minus_inf();
-          nan |= v != v;
+          const float v = sums && e0 + i < a.E ? val[i] : key[i];
+          close |= v != v;
           second = fmaxf(second, fminf(first, v));
           first = fmaxf(first, v);
         }
         for (int o = 1; o < glanes; o <<= 1) {
           const float f2 = __shfl_xor_sync(kFull, first, o), s2 = __shfl_xor_sync(kFull, second, o);
-          nan = __shfl_xor_sync(kFull, int(nan), o) != 0 || nan;
           second = fmaxf(fmaxf(second, s2), fminf(first, f2));
           first = fmaxf(first, f2);
         }
-        if (sums && second != minus_inf()) first += second;
-        const uint32_t mine = nan ? 0xFFFFFFFFu : first == minus_inf() ? 0u : ordered(first);
+        const float mine = sums && second != minus_inf() ? first + second : first;
         const int g = sl / glanes;
-        uint32_t below = 0;  // the best group behind this one
+        float below = minus_inf();  // the best group behind this one
         int rank = 0;
         for (int h = 0; h < a.groups; ++h) {
-          const uint32_t o = __shfl_sync(kFull, mine, h * glanes, LPT);
+          const float o = __shfl_sync(kFull, mine, h * glanes, LPT);
           const bool ahead = o > mine || (o == mine && h < g);
           rank += ahead;
-          if (!ahead && h != g) below = max(below, o);
+          if (!ahead && h != g) below = fmaxf(below, o);
         }
-        open_all = rank < a.top_groups;
-        close = rank == a.top_groups - 1 && near(mine, below);
+        close |= rank == a.top_groups - 1 && near(mine, below);
+        if (rank >= a.top_groups) {
 #pragma unroll
-        for (int i = 0; i < NPL; ++i)
-          if (!open_all) ord[i] = 0;
+          for (int i = 0; i < NPL; ++i) key[i] = minus_inf();
+        }
       } else {
         float* sv = reinterpret_cast<float*>(s.val) + seg * a.E;
-        uint32_t* so = reinterpret_cast<uint32_t*>(s.ord) + seg * a.E;
+        float* so = reinterpret_cast<float*>(s.ord) + seg * a.E;
         uint8_t* open = s.open + seg * a.E;
 #pragma unroll
         for (int i = 0; i < NPL; ++i)
-          if (e0 + i < a.E) sv[e0 + i] = sums ? val[i] : a.bias != nullptr ? val[i] : l[i];
+          if (e0 + i < a.E) sv[e0 + i] = sums ? val[i] : key[i];
         __syncwarp();
         for (int g = sl; g < a.groups; g += LPT) {
           float first = minus_inf(), second = minus_inf();
-          bool nan = false;
           for (int i = 0; i < gsize; ++i) {
             const float v = sv[g * gsize + i];
-            nan |= v != v;
+            close |= v != v;
             second = fmaxf(second, fminf(first, v));
             first = fmaxf(first, v);
           }
-          if (sums && second != minus_inf()) first += second;
-          so[g] = nan ? 0xFFFFFFFFu : first == minus_inf() ? 0u : ordered(first);
+          so[g] = sums && second != minus_inf() ? first + second : first;
         }
         __syncwarp();
         for (int g = sl; g < a.groups; g += LPT) {
-          const uint32_t mine = so[g];
-          uint32_t below = 0;
+          const float mine = so[g];
+          float below = minus_inf();
           int rank = 0;
           for (int h = 0; h < a.groups; ++h) {
-            const uint32_t o = so[h];
+            const float o = so[h];
             const bool ahead = o > mine || (o == mine && h < g);
             rank += ahead;
-            if (!ahead && h != g) below = max(below, o);
+            if (!ahead && h != g) below = fmaxf(below, o);
           }
           open[g] = rank < a.top_groups;
           close |= rank == a.top_groups - 1 && near(mine, below);
@@ -429,39 +512,29 @@ __global__ void __launch_bounds__(kScoreWarpsOne * 32) route_scores_kernel(Score
         __syncwarp();
 #pragma unroll
         for (int i = 0; i < NPL; ++i)
-          if (e0 + i < a.E && !open[(e0 + i) / gsize]) ord[i] = 0;
+          if (e0 + i < a.E && !open[(e0 + i) / gsize]) key[i] = minus_inf();
       }
     }
+    Places<NPL> places = sort_lane(key);
     __syncwarp();  // the last rows' picks are read
-    for (int j = sl; j < a.k; j += LPT) pick[j] = -1;
-    __syncwarp();
     const int rounds = values ? a.k + 1 : a.k;  // one more: the best key left behind
+    float before = __uint_as_float(0x7F800000u);
     for (int j = 0; j < rounds; ++j) {
-      uint32_t best = ord[0];
+      const float top = lanes_top<LPT>(key[0]);
+      const bool mine = key[0] == top;
+      const unsigned held = __ballot_sync(kFull, mine) >> (seg * LPT) & seg_mask;
+      close |= near(before, top);
+      before = top;
+      const bool goes = mine && (held & lower) == 0;  // the lowest lane that has it: its best goes
+      if (goes) pick[j] = top == minus_inf() ? -1 : e0 + int(places & 15);
+      places = goes ? places >> 4 : places;
 #pragma unroll
-      for (int i = 1; i < NPL; ++i) best = max(best, ord[i]);
-      const uint32_t top = lanes_max<LPT>(best);
-      const unsigned held = __ballot_sync(kFull, best == top && top != 0) >> (seg * LPT) & seg_mask;
-      if (sl == 0) tops[j] = top;
-      if (held != 0 && sl == __ffs(held) - 1) {  // the lowest lane that has it: its first such expert goes
-        int at = 0;
-#pragma unroll
-        for (int i = NPL - 1; i >= 0; --i)
-          if (ord[i] == top) at = i;
-#pragma unroll
-        for (int i = 0; i < NPL; ++i)
-          if (i == at) ord[i] = 0;
-        if (j < a.k) pick[j] = e0 + at;
-      }
+      for (int i = 0; i + 1 < NPL; ++i) key[i] = goes ? key[i + 1] : key[i];
+      key[NPL - 1] = goes ? minus_inf() : key[NPL - 1];
     }
     __syncwarp();
-    for (int j = sl; j + 1 < rounds; j += LPT) close |= near(tops[j], tops[j + 1]);
-    for (unsigned again = __ballot_sync(kFull, close); again != 0;) {  // rare: in float64, by the whole warp
-      const int which = (__ffs(again) - 1) / LPT;
-      again &= ~(seg_mask << (which * LPT));
-      select_exact(a, static_cast<const L*>(a.logits) + (base + which) * a.ld, s, s.pick + which * 32);
-    }
-    __syncwarp();
+    const unsigned unsure = __ballot_sync(kFull, close) >> (seg * LPT) & seg_mask;
+    any_unsure |= __any_sync(kFull, close);
     int id[kRows];
     bool has[kRows];
     float lc[kRows], share[kRows];
@@ -473,7 +546,9 @@ __global__ void __launch_bounds__(kScoreWarpsOne * 32) route_scores_kernel(Score
       lc[q] = has[q] ? load_logit(row + id[q]) : 0.f;
     }
     chosen_shares<LPT>(has, lc, slots, a.score, a.renorm, row_max, z, share);
-    if (t < a.T) {
+    if (t < a.T && unsure != 0) {
+      if (sl == 0) a.idx[t * a.k] = kUnsure;
+    } else if (t < a.T) {
 #pragma unroll
       for (int q = 0; q < kRows; ++q) {
         const int j = q * LPT + sl;
@@ -484,6 +559,13 @@ __global__ void __launch_bounds__(kScoreWarpsOne * 32) route_scores_kernel(Score
       }
     }
   }
+  __syncwarp();
+  if (any_unsure)
+    for (int64_t base = (int64_t(blockIdx.x) * warps + warp) * kRows; base < a.T; base += int64_t(gridDim.x) * warps * kRows)
+      for (int r = 0; r < kRows && base + r < a.T; ++r) {
+        const int32_t mark = __shfl_sync(kFull, lane == 0 ? *const_cast<volatile int32_t*>(a.idx + (base + r) * a.k) : 0, 0);
+        if (mark == kUnsure) select_exact<L, (LPT * NPL + 31) / 32>(a, base + r, s, hist);
+      }
   if (a.counts == nullptr) return;
   __syncthreads();
   for (int e = threadIdx.x; e < a.E; e += blockDim.x) {
