@@ -240,7 +240,8 @@ __device__ __forceinline__ void chosen_shares(const bool (&has)[32 / LPT], const
 
 // A row whose order float32 does not settle, by a whole warp in float64: N experts a lane.  It is
 // called behind the main loop: a call inside would cost every row its register spills (270 of 790
-// instructions a pass).  One row is one warp's latency, so its loops are unrolled for it.
+// instructions a pass).  What it takes is one row's
+// latency, most of that the fetch of code that no other warp runs: hence the short loops.
 template <typename L, int N>
 __device__ __noinline__ void select_exact(const ScoreArgs& a, int64_t t, ScoreScratch s, int32_t* hist) {
   const L* row = static_cast<const L*>(a.logits) + t * a.ld;
@@ -249,46 +250,36 @@ __device__ __noinline__ void select_exact(const ScoreArgs& a, int64_t t, ScoreSc
   const int gsize = a.E / a.groups;
   const bool sums = a.groups > 1 && a.group_score == kGroupTop2 && gsize > 1;
   const double none = double(minus_inf());
-  float lf[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) lf[i] = e0 + i < a.E ? load_logit(row + e0 + i) : minus_inf();
-  double val[N], top = none;
-  if (a.score == kSigmoid) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) val[i] = 1.0 / (1.0 + exp(-double(lf[i])));
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) top = fmax(top, double(lf[i]));
+  double top = none, z = 1.0;
+  if (a.score == kSoftmax) {
+    for (int e = lane; e < a.E; e += 32) top = fmax(top, double(load_logit(row + e)));
     top = lanes<32>(top, [](double x, double y) { return fmax(x, y); });
     double part = 0.0;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      val[i] = e0 + i < a.E ? exp(double(lf[i]) - top) : 0.0;
-      part += val[i];
-    }
-    const double z = lanes_sum<32>(part);
-#pragma unroll
-    for (int i = 0; i < N; ++i) val[i] /= z;
+#pragma unroll 1
+    for (int e = lane; e < a.E; e += 32) part += exp(double(load_logit(row + e)) - top);
+    z = lanes_sum<32>(part);
   }
+  __syncwarp();
+#pragma unroll 1
+  for (int e = lane; e < a.E; e += 32) {
+    const float lf = load_logit(row + e);
+    const double l = double(lf), x = exp(a.score == kSigmoid ? -l : l - top);
+    const double score = (a.score == kSigmoid ? 1.0 : x) / (a.score == kSigmoid ? 1.0 + x : z);
+    const double v = lf == minus_inf() ? none : a.bias != nullptr ? score + double(__ldg(a.bias + e)) : score;
+    const double key = a.bias != nullptr ? v : l;
+    s.val[e] = sums ? v : key;
+    s.ord[e] = key == none ? 0 : ordered(key);
+  }
+  __syncwarp();
   uint64_t ord[N];
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    if (a.bias != nullptr && e0 + i < a.E) val[i] += double(__ldg(a.bias + e0 + i));
-    if (lf[i] == minus_inf()) val[i] = none;
-    const double key = a.bias != nullptr ? val[i] : double(lf[i]);
-    ord[i] = key == none ? 0 : ordered(key);
-    if (!sums) val[i] = key;
-  }
+  for (int i = 0; i < N; ++i) ord[i] = e0 + i < a.E ? s.ord[e0 + i] : 0;
+  __syncwarp();
   if (a.groups > 1) {
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (e0 + i < a.E) s.val[e0 + i] = val[i];
-    __syncwarp();
     for (int g = lane; g < a.groups; g += 32) {
       double first = none, second = none;
       bool nan = false;
-#pragma unroll 4
+#pragma unroll 1
       for (int i = 0; i < gsize; ++i) {
         const double v = s.val[g * gsize + i];
         nan |= v != v;
@@ -302,7 +293,7 @@ __device__ __noinline__ void select_exact(const ScoreArgs& a, int64_t t, ScoreSc
     for (int g = lane; g < a.groups; g += 32) {
       const uint64_t mine = s.ord[g];
       int rank = 0;
-#pragma unroll 4
+#pragma unroll 1
       for (int h = 0; h < a.groups; ++h) rank += s.ord[h] > mine || (s.ord[h] == mine && h < g);
       s.open[g] = rank < a.top_groups;
     }
@@ -312,6 +303,7 @@ __device__ __noinline__ void select_exact(const ScoreArgs& a, int64_t t, ScoreSc
       if (e0 + i < a.E && !s.open[(e0 + i) / gsize]) ord[i] = 0;
   }
   __syncwarp();
+#pragma unroll 1
   for (int j = 0; j < a.k; ++j) {
     uint64_t best = ord[0];
     int at = 0;
@@ -335,9 +327,7 @@ __device__ __noinline__ void select_exact(const ScoreArgs& a, int64_t t, ScoreSc
   if (a.score == kSoftmax && !a.renorm) {
     row_max = float(top);
     float part = 0.f;
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (e0 + i < a.E) part += expf(lf[i] - row_max);
+    for (int e = lane; e < a.E; e += 32) part += expf(load_logit(row + e) - row_max);
     sum = lanes_sum<32>(part);
   }
   const int32_t id = lane < a.k ? pick[lane] : -1;
@@ -353,8 +343,9 @@ __device__ __noinline__ void select_exact(const ScoreArgs& a, int64_t t, ScoreSc
   __syncwarp();
 }
 
-template <typename L, int LPT, int NPL>
-__global__ void __launch_bounds__(kScoreWarpsOne * 32) route_scores_kernel(ScoreArgs a) {
+// WARPS of a CTA at most: the one CTA of a small batch has many, the others stay at few and more registers.
+template <typename L, int LPT, int NPL, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32) route_scores_kernel(ScoreArgs a) {
   extern __shared__ __align__(16) char smem[];
   constexpr int kRows = 32 / LPT;  // of a warp
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
@@ -389,10 +380,11 @@ __global__ void __launch_bounds__(kScoreWarpsOne * 32) route_scores_kernel(Score
   const bool on_lanes = a.groups > 1 && gsize % NPL == 0 && (glanes & (glanes - 1)) == 0;
   const bool soft = a.score == kSoftmax && (values || !a.renorm);
   const bool wide = a.wide && a.E % NPL == 0;
-  // |key - exact key| <= rel / 2 * (|key| + bias): sigmoid 2^-20.9 (exp 1 ulp, sum half an ulp, reciprocal
-  // 1 ulp), softmax 2^-17.2 (l - max rounds to half an ulp of up to 104); `near` adds both sides'
-  // bounds with room to spare, 1e-36 covers denormal scores.
-  const float rel = a.score == kSigmoid ? 1.9073486328125e-06f : 1.52587890625e-05f;
+  // |key - exact key| <= u * (|key| + |bias|): sigmoid u = 2^-21.1 (exp 2 ulp, sum half an ulp, reciprocal
+  // 1 ulp, the key's own rounding), softmax 2^-17.2 (l - max rounds to half an ulp of up to 104).  Two keys
+  // are told apart if they differ by more than rel * (2 |larger| + 8 max|bias|), rel = 1.5 u and 2.3 u;
+  // 1e-36 covers denormal scores.
+  const float rel = a.score == kSigmoid ? 6.7e-07f : 1.52587890625e-05f;
   // (y <= x, and where |y| > |x| it is at most |x| + (x - y); false for an infinite x or y)
   const float near_abs = values ? rel * 8.f * bias_max + 1e-36f : -1.f, near_rel = values ? 2.f * rel : 0.f;
   auto near = [&](float x, float y) { return x - y <= near_rel * fminf(fabsf(x), kFltMax) + near_abs; };
@@ -696,12 +688,14 @@ int launch_scores(ScoreArgs a, cudaStream_t stream) {
     const int64_t most = int64_t(8) * num_sms();
     const size_t smem = (size_t(a.E) * 4 + 15) / 16 * 16 + warps * ((score_scratch_bytes(a.E, kLpt) + 15) / 16 * 16);
     static std::atomic<uint64_t> raised{0};
-    if (!raise_smem_limit(route_scores_kernel<L, kLpt, kNpl>, 200 * 1024, raised) ||
+    if (!raise_smem_limit(route_scores_kernel<L, kLpt, kNpl, kScoreWarpsOne>, 200 * 1024, raised) ||
         (!a.one && a.counts != nullptr && cudaMemsetAsync(a.counts, 0, sizeof(int32_t) * a.E, stream) != cudaSuccess)) {
       st = MCL4MOE_ERR_CUDA;
       return;
     }
-    route_scores_kernel<L, kLpt, kNpl><<<unsigned(blocks < most ? blocks : most), warps * 32, smem, stream>>>(a);
+    const unsigned grid = unsigned(blocks < most ? blocks : most);
+    if (a.one) route_scores_kernel<L, kLpt, kNpl, kScoreWarpsOne><<<grid, warps * 32, smem, stream>>>(a);
+    else route_scores_kernel<L, kLpt, kNpl, kScoreWarps><<<grid, warps * 32, smem, stream>>>(a);
     if (cudaGetLastError() != cudaSuccess) st = MCL4MOE_ERR_CUDA;
   });
   return st;
