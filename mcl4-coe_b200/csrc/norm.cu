@@ -943,6 +943,7 @@ bool norm_in_registers(const NormArgs& a) {
 
 // Rows ahead: up to four, as many as the CTAs that are resident at once have room for.
 constexpr int kAheadBytes = 200 * 1024;  // of an SM's shared memory
+constexpr int kTeamSmem = 224 * 1024;    // of a CTA: one float32 row of 8192 with an element-wise gate and the factors
 
 // 16 columns a thread: needed from 2049 columns on; from 1025 on where a row has more operands or
 // wider ones, so that the reductions weigh more than the warps in flight (32768 x 2048, forward /
@@ -966,12 +967,12 @@ int launch_team(const NormArgs& a, NormShape s, bool backward, float* partial, c
   const unsigned grid = unsigned((s.plan.teams + s.rows_per_cta - 1) / s.rows_per_cta);
   if (backward) {
     static std::atomic<uint64_t> raised{0};
-    if (!raise_smem_limit(residual_norm_team_bwd_kernel<TX, TU, NCH, LAY, GATED>, 220 * 1024, raised))
+    if (!raise_smem_limit(residual_norm_team_bwd_kernel<TX, TU, NCH, LAY, GATED>, kTeamSmem, raised))
       return MCL4MOE_ERR_CUDA;
     residual_norm_team_bwd_kernel<TX, TU, NCH, LAY, GATED><<<grid, s.threads, smem, stream>>>(a, s.plan, partial);
   } else {
     static std::atomic<uint64_t> raised{0};
-    if (LAY != kSingles && !raise_smem_limit(residual_norm_team_kernel<TX, TU, NCH, LAY, GATED>, 220 * 1024, raised))
+    if (LAY != kSingles && !raise_smem_limit(residual_norm_team_kernel<TX, TU, NCH, LAY, GATED>, kTeamSmem, raised))
       return MCL4MOE_ERR_CUDA;
     residual_norm_team_kernel<TX, TU, NCH, LAY, GATED><<<grid, s.threads, smem, stream>>>(a, s.plan);
   }

@@ -64,7 +64,9 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
     runs.  ``grad_scale`` (fp32 device scalar) is what clipping multiplies gradients
     with.  A moment that is not finite is NaN in 8 bits, its block's others stay.
     """
-    params, grads = list(params), list(grads)
+    params, grads, exp_avgs, exp_avg_sqs = list(params), list(grads), list(exp_avgs), list(exp_avg_sqs)
+    exp_avg_scales, exp_avg_sq_scales, masters = (None if t is None else list(t)
+                                                  for t in (exp_avg_scales, exp_avg_sq_scales, masters))
     if len(grads) != len(params):
         raise ValueError(f"{len(grads)} gradients for {len(params)} parameters")
     eight = exp_avg_scales is not None

@@ -223,6 +223,41 @@ def test_runs_are_equal_and_capture_replays(moe_pkg):
     assert torch.equal(out[3], torch.autograd.grad(moe_pkg.route_experts(leaf, 8, **kw)[0], leaf, d_w)[0])
 
 
+def test_large_batches_and_two_streams(moe_pkg):
+    """More rows than the CTAs that are resident, on two streams at once; strided, odd and masked rows
+    are compared with the definition row by row on a sample."""
+    wide = _logits(70001, 67, torch.bfloat16, 40)
+    logits = wide[:, 1:62]
+    valid = torch.rand(70001, generator=torch.Generator().manual_seed(3)).to(DEV) < 0.9
+    bias = (torch.arange(61, device=DEV) % 7) * 1e-3
+    kw = dict(score="sigmoid", bias=bias, valid=valid)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    outs = []
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            outs.append(moe_pkg.route_experts(logits, 6, **kw))
+    for s in streams:
+        torch.cuda.current_stream().wait_stream(s)
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
+    w, ids, counts = outs[0]
+    assert int(counts.sum()) == 6 * int(valid.sum())
+    assert torch.equal(torch.bincount(ids[ids >= 0].reshape(-1).long(), minlength=61), counts.long())
+    pick = torch.arange(0, 70001, 701)
+    want = ref.route(logits[pick], 6, score="sigmoid", bias=bias, valid=valid[pick])
+    assert torch.equal(ids[pick].cpu().long(), want[1])
+    torch.testing.assert_close(w[pick].cpu().double(), want[0], rtol=REL, atol=0)
+
+
+def test_second_differentiation_is_refused(moe_pkg):
+    logits = _logits(4, 16, torch.float32, 1).requires_grad_(True)
+    w, _, _ = moe_pkg.route_experts(logits, 4)
+    (g,) = torch.autograd.grad(w.square().sum(), logits, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
 def test_refusals_on_the_device(moe_pkg):
     logits = _logits(4, 16, torch.float32, 1)
     with pytest.raises(ValueError):

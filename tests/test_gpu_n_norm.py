@@ -159,6 +159,36 @@ def test_every_form(moe_pkg, post, pre, gate, act, T, d):
     _check(moe_pkg, t, dy, dh, act=act)
 
 
+@pytest.mark.parametrize("gate", ["token", "full"])
+@pytest.mark.parametrize("T,d", [(3, 8192), (5, 6000), (4, 2048), (300, 1032), (2, 1500), (2, 16384)])
+@pytest.mark.parametrize("xt,ut", [(F32, F32), (F32, BF), (BF, BF)])
+def test_gates_of_wide_rows(moe_pkg, gate, T, d, xt, ut):
+    t, dy, dh = _case(T, d, xt, ut, True, True, (T, 1) if gate == "token" else (T, d), 31)
+    _check(moe_pkg, t, dy, dh, act="sigmoid", bs=0.5)
+
+
+@pytest.mark.parametrize("T,d", [(9, 64), (4, 2049)])
+def test_mixed_types_outside_the_common_ones(moe_pkg, T, d):
+    """A float32 gate on bf16 rows, a norm in another type than the branch."""
+    t, dy, dh = _case(T, d, BF, BF, True, True, (T, d), 41)
+    t["gate"] = t["gate"].float()
+    _check(moe_pkg, t, dy, dh, act="tanh")
+    t, dy, dh = _case(T, d, BF, BF, True, True, (d,), 42)
+    dev = {n: v.to(DEV).requires_grad_(True) for n, v in t.items()}
+    out = moe_pkg.residual_norm(dev["x"], dev["branch"], post_weight=dev["post"], gate=dev["gate"], pre_weight=dev["pre"])
+    y, h = moe_pkg.residual_norm(dev["x"], dev["branch"], post_weight=dev["post"], gate=dev["gate"],
+                                 pre_weight=dev["pre"], norm_dtype=F32)
+    # two kernels add in another order: float32 values a few 2^-24 apart, which can round to neighbours in bf16
+    assert h.dtype == F32
+    assert ((h - out[1].float()).abs() <= (2.0 ** -8 + 2.0 ** -16) * h.abs()).all()
+    assert ((y.float() - out[0].float()).abs() <= 2.0 ** -7 * out[0].float().abs()).all()
+    got = torch.autograd.grad([y, h], list(dev.values()), [dy.to(DEV), dh.float().to(DEV)])
+    want = torch.autograd.grad(list(out), list(dev.values()), [dy.to(DEV), dh.to(DEV)])
+    for a, b in zip(got, want):  # the same sums in another order, rounded to the same type
+        scale = float(b.float().abs().max())
+        assert float((a.float() - b.float()).abs().max()) <= (2.0 ** -8 if b.dtype == BF else 2.0 ** -15) * scale
+
+
 @pytest.mark.parametrize("dy_on,dh_on", [(True, False), (False, True)])
 @pytest.mark.parametrize("d", [96, 37])
 def test_one_output_used(moe_pkg, dy_on, dh_on, d):
@@ -222,6 +252,32 @@ def test_half_precision_weights_get_their_own_gradient_type(moe_pkg):
     y, h = moe_pkg.residual_norm(t["x"].to(DEV), t["branch"].to(DEV), post_weight=post, pre_weight=pre)
     g = torch.autograd.grad([y, h], [post, pre], [dy.to(DEV), dh.to(DEV)])
     assert all(v.dtype == BF and torch.isfinite(v).all() for v in g)
+
+
+def test_only_some_inputs_need_gradients(moe_pkg):
+    t, dy, dh = _case(12, 96, BF, BF, True, True, (96,), 51)
+    full = {n: v.to(DEV).requires_grad_(True) for n, v in t.items()}
+
+    def run(leaves):
+        y, h = moe_pkg.residual_norm(leaves["x"], leaves["branch"], post_weight=leaves["post"], gate=leaves["gate"],
+                                     gate_activation="sigmoid", pre_weight=leaves["pre"])
+        wanted = [n for n in NAMES if leaves[n].requires_grad]
+        return dict(zip(wanted, torch.autograd.grad([y, h], [leaves[n] for n in wanted], [dy.to(DEV), dh.to(DEV)])))
+
+    want = run(full)
+    for n in NAMES:
+        got = run({m: v.detach().requires_grad_(m == n) for m, v in full.items()})
+        assert list(got) == [n] and torch.equal(got[n], want[n])
+    # one tensor as stream and as branch: both gradients reach it
+    both = full["x"].detach().clone().requires_grad_(True)
+    y, _ = moe_pkg.residual_norm(both, both, branch_scale=2.0)
+    (g,) = torch.autograd.grad(y, both, torch.ones_like(y))
+    assert torch.equal(g, torch.full_like(g, 3.0))
+    with pytest.raises(RuntimeError):  # differentiable once
+        x = full["x"].detach().float().requires_grad_(True)
+        _, h = moe_pkg.residual_norm(x, pre_weight=full["pre"].detach())
+        (g,) = torch.autograd.grad(h.sum(), x, create_graph=True)
+        g.sum().backward()
 
 
 def test_zero_rows_zero_values_and_non_finite_rows(moe_pkg):
