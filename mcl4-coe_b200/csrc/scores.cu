@@ -13,9 +13,11 @@
 // row whose order hangs on less than that bound (neighbouring picks, or the border
 // between open and closed groups) is selected again in float64, by a whole warp.
 //
-// A row is a few hundred bytes and a few hundred instructions, so issue slots bound it, not HBM:
-// a row gets 8, 16 or 32 lanes with up to 8 experts in each one's registers (16 above 256
-// experts), so that the butterflies and the pops of the k rounds serve up to four rows at once.
+// A row is a few hundred bytes and a few hundred instructions, so issue slots and latency bound it,
+// not HBM: a row gets 8, 16 or 32 lanes with up to 8 experts in each one's registers (16 above 256
+// experts), so that the butterflies and the pops of the k rounds serve up to four rows at once, on
+// lists that each lane has sorted.  32768 x 64, sigmoid, bias, 4 of 8 groups, top 8: 31 us (a warp a
+// row: 51 us); softmax without groups 20 us; 16383 x 256 with groups 47 us; gradients 10 to 12 us.
 #include <type_traits>
 
 #include <cuda_fp16.h>
@@ -685,7 +687,9 @@ int launch_scores(ScoreArgs a, cudaStream_t stream) {
     a.one = a.T <= kScoreWarpsOne * (32 / kLpt);
     const int warps = a.one ? (a.T + 32 / kLpt - 1) / (32 / kLpt) : kScoreWarps;
     const int64_t blocks = (a.T + int64_t(warps) * (32 / kLpt) - 1) / (int64_t(warps) * (32 / kLpt));
-    const int64_t most = int64_t(8) * num_sms();
+    // as many CTAs as are resident (32768 x 256 softmax 102 -> 90 us from 8 an SM), but the widest rows
+    // leave more of their latency to others (16384 x 512: 86 us, 96 with 5)
+    const int64_t most = int64_t(kLpt * kNpl > 256 ? 8 : 5) * num_sms();
     const size_t smem = (size_t(a.E) * 4 + 15) / 16 * 16 + warps * ((score_scratch_bytes(a.E, kLpt) + 15) / 16 * 16);
     static std::atomic<uint64_t> raised{0};
     if (!raise_smem_limit(route_scores_kernel<L, kLpt, kNpl, kScoreWarpsOne>, 200 * 1024, raised) ||
