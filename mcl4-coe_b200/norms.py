@@ -76,11 +76,11 @@ class _ResidualNorm(torch.autograd.Function):
     """Saves the inputs and the rows' two reciprocal root mean squares; the backward computes the rest again."""
 
     @staticmethod
-    def forward(ctx, x, branch, post, pre, gate, mode, gate_rows, act, norm_dtype, scales):
+    def forward(ctx, x, branch, post, pre, gate, form):
         stats = x.new_empty((x.shape[0], 2), dtype=torch.float32)
-        y, h = _norm_forward(x, branch, post, pre, gate, mode, gate_rows, act, norm_dtype, scales, stats)
+        y, h = _norm_forward(x, branch, post, pre, gate, *form, stats)
         ctx.save_for_backward(x, branch, post, pre, gate, stats)
-        ctx.args = (mode, gate_rows, act, norm_dtype, scales)
+        ctx.form = form
         ctx.set_materialize_grads(False)
         return y, h
 
@@ -98,16 +98,16 @@ class _ResidualNorm(torch.autograd.Function):
     @staticmethod
     def _gradients(ctx, d_y, d_h):
         if d_y is None and d_h is None:
-            return (None,) * 10
+            return (None,) * 6
         x, branch, post, pre, gate, stats = ctx.saved_tensors
-        mode, gate_rows, act, norm_dtype, scales = ctx.args
+        mode = ctx.form[0]
         need = ctx.needs_input_grad
         if x.shape[0] == 0:
             return tuple(torch.zeros_like(t) if n and t is not None else None
-                         for n, t in zip(need, (x, branch, post, pre, gate))) + (None,) * 5
+                         for n, t in zip(need, (x, branch, post, pre, gate))) + (None,)
         lib = _lib.load()
         dev = x.device
-        args = _fill(_lib.NormArgs(), x, branch, post, pre, gate, mode, gate_rows, act, norm_dtype, scales)
+        args = _fill(_lib.NormArgs(), x, branch, post, pre, gate, *ctx.form)
         args.stats = stats.data_ptr()
         if d_y is not None:
             d_y = _rows(d_y)
@@ -119,7 +119,8 @@ class _ResidualNorm(torch.autograd.Function):
         def out(wanted, like, attr, dtype=None):
             if like is None or not wanted:
                 return None
-            t = x.new_empty(like.shape, dtype=dtype or like.dtype)
+            t = torch.empty_like(like) if dtype is None and like.is_contiguous() else \
+                x.new_empty(like.shape, dtype=dtype or like.dtype)
             setattr(args, attr, t.data_ptr())
             return t
 
@@ -135,7 +136,7 @@ class _ResidualNorm(torch.autograd.Function):
         _launch(dev, "mcl4moe_residual_norm_backward", lib.mcl4moe_residual_norm_backward, args, _ptr(ws), nbytes)
         if d_gate is not None and d_gate.dtype != gate.dtype:
             d_gate = d_gate.to(gate.dtype)
-        return (d_x, d_branch, d_post, d_pre, d_gate) + (None,) * 5
+        return d_x, d_branch, d_post, d_pre, d_gate, None
 
 
 def residual_norm(x: Tensor, branch: Tensor | None = None, *, post_weight: Tensor | None = None,
@@ -185,12 +186,12 @@ def residual_norm(x: Tensor, branch: Tensor | None = None, *, post_weight: Tenso
         gate_2d, mode, gate_rows = _gate_form(gate, x)
     _require_cuda(x, "residual_norm")
     tensors = (_rows(x), None if branch is None else _rows(branch), _f32(post_weight), _f32(pre_weight), gate_2d)
-    rest = (mode, gate_rows, GATE_ACTIVATIONS.index(gate_activation), norm_dtype,
+    form = (mode, gate_rows, GATE_ACTIVATIONS.index(gate_activation), norm_dtype,
             (float(residual_scale), float(branch_scale), float(eps)))
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        y, h = _ResidualNorm.apply(*tensors, *rest)
+        y, h = _ResidualNorm.apply(*tensors, form)
     else:
-        y, h = _norm_forward(*tensors, *rest)
+        y, h = _norm_forward(*tensors, *form)
     if x.ndim != 2:
         y, h = (None if t is None else t.view(x.shape) for t in (y, h))
     return (x if branch is None else y), h

@@ -72,17 +72,20 @@ def _route_forward(logits, k, score, bias, groups, top_groups, group_score, reno
 
 
 class _RouteScores(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, k, score, bias, groups, top_groups, group_score, renorm, scale, valid):
-        w, idx, counts = _route_forward(logits, k, score, bias, groups, top_groups, group_score, renorm, scale, valid)
-        ctx.save_for_backward(logits, idx)
-        ctx.args = (k, score, renorm, scale)
-        ctx.mark_non_differentiable(idx, counts)
-        ctx.set_materialize_grads(False)
-        return w, idx, counts
+    """The weights as a function of the logits; the ids and counts leave through ``box`` (outputs that
+    autograd need not know of)."""
 
     @staticmethod
-    def backward(ctx, d_w, d_idx, d_counts):
+    def forward(ctx, logits, args, box):
+        w, idx, counts = _route_forward(logits, *args)
+        ctx.save_for_backward(logits, idx)
+        ctx.args = args
+        ctx.set_materialize_grads(False)
+        box += (idx, counts)
+        return w
+
+    @staticmethod
+    def backward(ctx, d_w):
         if torch.is_grad_enabled():  # create_graph: a second differentiation has to be refused
             return _RouteScores._once(ctx, d_w)
         return _RouteScores._gradients(ctx, d_w)
@@ -90,16 +93,16 @@ class _RouteScores(torch.autograd.Function):
     @staticmethod
     def _gradients(ctx, d_w):
         if d_w is None:
-            return (None,) * 10
+            return None, None, None
         logits, idx = ctx.saved_tensors
-        k, score, renorm, scale = ctx.args
+        k, score, _, _, _, _, renorm, scale, _ = ctx.args
         n, E = logits.shape
         d_w = _f32(d_w)
         d_logits = logits.new_empty((n, E))
         _launch(logits.device, "mcl4moe_route_scores_backward", _lib.load().mcl4moe_route_scores_backward,
                 logits.data_ptr(), DTYPE_CODES[logits.dtype], _ld(logits), idx.data_ptr(), d_w.data_ptr(), n, E, k,
                 score, renorm, scale, d_logits.data_ptr())
-        return (d_logits,) + (None,) * 9
+        return d_logits, None, None
 
     @staticmethod
     @once_differentiable
@@ -157,12 +160,15 @@ def route_experts(logits: Tensor, top_k: int, *, score: str = "softmax", bias: T
         valid = valid.contiguous()
     _require_cuda(logits, "route_experts")
     lead = logits.shape[:-1]
-    args = (_rows(logits), top_k, SCORE_FUNCTIONS.index(score), bias, num_groups, top_groups,
-            GROUP_SCORES.index(group_score), int(bool(renormalize)), float(scale), valid)
+    rows = _rows(logits)
+    args = (top_k, SCORE_FUNCTIONS.index(score), bias, num_groups, top_groups, GROUP_SCORES.index(group_score),
+            int(bool(renormalize)), float(scale), valid)
     if torch.is_grad_enabled() and logits.requires_grad:
-        w, idx, counts = _RouteScores.apply(*args)
+        box: list = []
+        w = _RouteScores.apply(rows, args, box)
+        idx, counts = box
     else:
-        w, idx, counts = _route_forward(*args)
+        w, idx, counts = _route_forward(rows, *args)
     if len(lead) != 1:
         w, idx = w.view(*lead, top_k), idx.view(*lead, top_k)
     return w, idx, counts

@@ -117,7 +117,7 @@ def test_masked_rows_may_hold_anything(moe_pkg):
     for p, q in zip(*results):
         assert torch.isfinite(p).all() and torch.equal(p, q)
     out, aux, z, load = layer(x, torch.zeros(40, dtype=torch.bool, device=DEV))
-    assert not out.any() and float(aux) == float(z) == 0.0 and not load.any()
+    assert not out.any() and float(aux.detach()) == float(z.detach()) == 0.0 and not load.any()
     empty = layer(x[:0])
     assert empty[0].shape == (0, 256)
 
