@@ -193,14 +193,23 @@ __device__ __forceinline__ void e5m2x4(uint32_t w, float (&v)[4]) {  // a code i
   }
 }
 
-// The update's m / (sqrt(v) inv_root + eps), within 2^-21: its rounding ends up far below the
+// The update's square root and reciprocal, within 2^-22 each: their rounding ends up far below the
 // parameter's own.
-__device__ __forceinline__ float adam_ratio(float m, float v, float inv_root, float eps) {
-  float root;
-  asm("sqrt.approx.f32 %0, %1;" : "=f"(root) : "f"(v));
-  float inv;  // the flush to zero of a denormal denominator meets eps = 0 and v = 0 alone
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(root * inv_root + eps));
-  return m * inv;
+__device__ __forceinline__ float root_of(float v) {
+  float r;
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float inverse_of(float d) {
+  float r;  // the flush to zero of a denormal denominator meets eps = 0 and v = 0 alone
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
+  return r;
+}
+__device__ __forceinline__ uint64_t both(float v) { return f2pack(v, v); }
+__device__ __forceinline__ uint64_t ffma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
 }
 
 // The power of two that puts the block's largest finite magnitude into binade TOP, and its inverse.
@@ -302,24 +311,39 @@ __device__ __forceinline__ void adam_block(const AdamTensor<P, G, EIGHT, MASTER>
       e4m3x4(word4(r.m[q]), m[q]);
       e5m2x4(word4(r.v[q]), v[q]);
     }
+// Two elements an instruction where a product stands alone.  The moments' sums are single: each
+    // product and sum is rounded by itself, which the 8-bit codes' definition goes by, and a packed
+    // product and a packed sum (mul and add.rn.f32x2) came out fused.
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float gr = __fmul_rn(to_f(r.g[q].v[i]), f.grad_scale);
+    for (int i = 0; i < 4; i += 2) {
+      const uint64_t gr = fmul2(f2pack(to_f(r.g[q].v[i]), to_f(r.g[q].v[i + 1])), both(f.grad_scale));
+      uint64_t mm, vv;
       if constexpr (EIGHT) {
-        m[q][i] = __fmul_rn(m[q][i], r.ms);
-        v[q][i] = __fmul_rn(v[q][i], r.vs);
+        mm = fmul2(f2pack(m[q][i], m[q][i + 1]), both(r.ms));
+        vv = fmul2(f2pack(v[q][i], v[q][i + 1]), both(r.vs));
       } else {
-        m[q][i] = r.m[q].v[i];
-        v[q][i] = r.v[q].v[i];
+        mm = f2pack(r.m[q].v[i], r.m[q].v[i + 1]);
+        vv = f2pack(r.v[q].v[i], r.v[q].v[i + 1]);
       }
-      // each product and sum rounded by itself: the 8-bit codes' definition goes by it (packed pairs,
-      // mul and add.rn.f32x2, came out fused)
-      m[q][i] = __fadd_rn(__fmul_rn(m[q][i], h.beta1), __fmul_rn(gr, h.one_minus_beta1));
-      v[q][i] = __fadd_rn(__fmul_rn(v[q][i], h.beta2), __fmul_rn(__fmul_rn(gr, gr), h.one_minus_beta2));
-      const float w = MASTER ? r.w[q].v[i] : to_f(r.p[q].v[i]);
-      const float now = w * f.decay - adam_ratio(m[q][i], v[q][i], f.inv_root, h.eps) * f.step_size;
-      r.w[q].v[i] = now;
-      from_f(r.p[q].v[i], now);
+      float m0, m1, v0, v1, g0, g1, h0, h1;
+      f2unpack(fmul2(mm, both(h.beta1)), m0, m1);
+      f2unpack(fmul2(gr, both(h.one_minus_beta1)), g0, g1);
+      f2unpack(fmul2(vv, both(h.beta2)), v0, v1);
+      f2unpack(fmul2(fmul2(gr, gr), both(h.one_minus_beta2)), h0, h1);
+      m[q][i] = __fadd_rn(m0, g0);
+      m[q][i + 1] = __fadd_rn(m1, g1);
+      v[q][i] = __fadd_rn(v0, h0);
+      v[q][i + 1] = __fadd_rn(v1, h1);
+      const uint64_t w = MASTER ? f2pack(r.w[q].v[i], r.w[q].v[i + 1]) : f2pack(to_f(r.p[q].v[i]), to_f(r.p[q].v[i + 1]));
+      const uint64_t denom = ffma2(f2pack(root_of(v[q][i]), root_of(v[q][i + 1])), both(f.inv_root), both(h.eps));
+      float d0, d1, now0, now1;
+      f2unpack(denom, d0, d1);
+      const uint64_t ratio = fmul2(f2pack(m[q][i], m[q][i + 1]), f2pack(inverse_of(d0), inverse_of(d1)));
+      f2unpack(ffma2(ratio, both(-f.step_size), fmul2(w, both(f.decay))), now0, now1);
+      r.w[q].v[i] = now0;
+      r.w[q].v[i + 1] = now1;
+      from_f(r.p[q].v[i], now0);
+      from_f(r.p[q].v[i + 1], now1);
     }
     store4<WHOLE>(t.p + at, r.p[q], count[q]);
     if (MASTER) store4<WHOLE>(t.master + at, r.w[q], count[q]);
@@ -436,10 +460,10 @@ __global__ void __launch_bounds__(kAdamThreads, 4) adamw_kernel(const __grid_con
   }
 }
 
-// 8-bit moments: half the bytes and more arithmetic (about 80 instructions an element, bound by their
+// 8-bit moments: half the bytes and more arithmetic (about 75 instructions an element, bound by their
 // issue and HBM together), so the loads have to run ahead of it.  Persistent CTAs take turns; each
 // lane copies its own elements of the blocks to come into shared memory (cp.async), kAdamAhead turns
-// ahead, and reads them back itself.  94 M elements: 291 us, 5.2 TB/s (loads into registers, no
+// ahead, and reads them back itself.  94 M elements: 281 us, 5.4 TB/s (loads into registers, no
 // turns ahead: 448 us).
 constexpr int kAdamAhead = 3;
 
