@@ -19,7 +19,7 @@
 //   S = sum over rows of dz uh:  dw_post = bs act(g) S,  dg = bs act'(g) w_post S.
 // 32768 x 2048 bf16 with both norms and a channel gate: forward 95 us (5.7 TB/s), backward 159 us
 // (5.1 TB/s) with the column sums; issue slots (60% busy) and the reductions' latency are what is
-// left.  Single elements (32768 x 1001, float32 stream): 90 and 254 us.
+// left.  Single elements (32768 x 1001, float32 stream): 92 and 230 us.
 #include <cuda_fp16.h>
 
 #include "kernels.cuh"
@@ -606,10 +606,23 @@ __global__ void __launch_bounds__(NCH == 1 ? 256 : 512, NCH == 1 ? kBwdCtas : 1)
     if (n + 1 < rows) scalars(r + parts);  // the next row's, a row ahead
     ahead.wait();
     V8 z[NCH], uh[NCH], act[NCH];  // dz; u r_u; the element's gate
+    // single elements come from memory: all of them are asked for before the first is used
+    V8 x1[NCH], dh1[NCH];
+    if constexpr (LAY == kSingles) {
+#pragma unroll
+      for (int j = 0; j < NCH; ++j) {
+        if (branch) uh[j] = ahead.take(u_row(r), S::u, j);
+        if (streamed) z[j] = ahead.take(dy_row(r), S::dy, j);
+        if (normed) {
+          x1[j] = ahead.take(x_row(r), S::x, j);
+          dh1[j] = ahead.take(dh_row(r), S::dh, j);
+        }
+      }
+    }
     if (branch) {
 #pragma unroll
       for (int j = 0; j < NCH; ++j) {
-        uh[j] = mul(ahead.take(u_row(r), S::u, j), ru);
+        uh[j] = mul(LAY == kSingles ? uh[j] : ahead.take(u_row(r), S::u, j), ru);
         if (full) act[j] = act8(ahead.take(g_row(r), S::gate_b, j), a.gate_act);
       }
     }
@@ -621,17 +634,17 @@ __global__ void __launch_bounds__(NCH == 1 ? 256 : 512, NCH == 1 ? kBwdCtas : 1)
     };
 #pragma unroll
     for (int j = 0; j < NCH; ++j) {
-      if (streamed) z[j] = ahead.take(dy_row(r), S::dy, j);
-      else z[j].fill(0.f);
+      if (!streamed) z[j].fill(0.f);
+      else if (LAY != kSingles) z[j] = ahead.take(dy_row(r), S::dy, j);
     }
     if (normed) {
       V8 yh[NCH];
       float dot = 0.f;
 #pragma unroll
       for (int j = 0; j < NCH; ++j) {
-        const V8 v = mul(ahead.take(x_row(r), S::x, j), rs);
+        const V8 v = mul(LAY == kSingles ? x1[j] : ahead.take(x_row(r), S::x, j), rs);
         yh[j] = mul(branch ? fma(factor(j), uh[j], v) : v, ry);
-        const V8 d = ahead.take(dh_row(r), S::dh, j);
+        const V8 d = LAY == kSingles ? dh1[j] : ahead.take(dh_row(r), S::dh, j);
         acc_pre[j] = fma(d, yh[j], acc_pre[j]);
         const V8 dw = mul(d, ahead.kept(2 * j + 1));
         dot += dot8(dw, yh[j]);
