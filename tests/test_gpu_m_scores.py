@@ -250,6 +250,24 @@ def test_large_batches_and_two_streams(moe_pkg):
     torch.testing.assert_close(w[pick].cpu().double(), want[0], rtol=REL, atol=0)
 
 
+def test_rows_far_apart(moe_pkg):
+    """Offsets that pass 32 bits."""
+    ld = (1 << 27) + 3
+    buf = torch.empty(20 * ld, dtype=torch.bfloat16, device=DEV)
+    far = buf.as_strided((20, 40), (ld, 1))
+    far.copy_(_logits(20, 40, torch.float32, 50))
+    near = far.contiguous()
+    d_w = _logits(20, 5, torch.float32, 51)
+    results = []
+    for t in (far, near):
+        leaf = t.detach().requires_grad_(True)
+        w, ids, counts = moe_pkg.route_experts(leaf, 5, renormalize=False)
+        results.append((w.detach(), ids, counts, torch.autograd.grad(w, leaf, d_w)[0]))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+    del buf, far
+    torch.cuda.empty_cache()
+
+
 def test_second_differentiation_is_refused(moe_pkg):
     logits = _logits(4, 16, torch.float32, 1).requires_grad_(True)
     w, _, _ = moe_pkg.route_experts(logits, 4)

@@ -224,6 +224,29 @@ def test_gates_that_broadcast(moe_pkg, shape):
         torch.testing.assert_close(a.cpu().double(), b, rtol=0, atol=4e-3 if a.numel() < 64 else 2e-4)
 
 
+@pytest.mark.parametrize("groups,rows,d", [(5, 64, 96), (700, 32, 40), (3, 33, 300), (2, 40, 8200), (4, 31, 64)])
+@pytest.mark.parametrize("act", ["none", "sigmoid"])
+def test_one_gate_row_for_each_sequence(moe_pkg, groups, rows, d, act):
+    """Column sums over groups of rows: each sequence's gate gradient, and the post norm's over all of them.
+    A sum of n terms is off by at most (n + 48 + d / 32) * 2^-24 of its terms' magnitudes."""
+    g = torch.Generator().manual_seed(groups)
+    x, u, dy = (torch.randn(groups, rows, d, generator=g) for _ in range(3))
+    gate, post = torch.randn(groups, 1, d, generator=g), torch.rand(d, generator=g) + 0.5
+    dev = [v.to(DEV).requires_grad_(True) for v in (gate, post)]
+    y, _ = moe_pkg.residual_norm(x.to(DEV), u.to(DEV), gate=dev[0], gate_activation=act, post_weight=dev[1], branch_scale=0.5)
+    got = torch.autograd.grad(y, dev, dy.to(DEV))
+    leaf = [v.double().requires_grad_(True) for v in (gate, post)]
+    want_y, _ = ref.norm(x.double(), u.double(), leaf[1], leaf[0], act, None, 1.0, 0.5)
+    want = torch.autograd.grad(want_y, leaf, dy.double())
+    uh = u.double() * torch.rsqrt(u.double().square().mean(-1, keepdim=True) + 1e-6)
+    terms = (0.5 * dy.double() * uh).abs()
+    a = gate.double() if act == "none" else torch.sigmoid(gate.double())
+    slope = torch.ones_like(a) if act == "none" else a * (1 - a)
+    sizes = [(terms * post.double()).sum(1, keepdim=True) * slope, (terms * a.abs()).sum((0, 1))]
+    for gg, wg, size, n in zip(got, want, sizes, (rows, groups * rows)):
+        assert ((gg.cpu().double() - wg).abs() <= (n + 48 + d / 32) * 2.0 ** -24 * size + 1e-30).all()
+
+
 def test_strides_and_offsets(moe_pkg):
     """Rows of a wider buffer, an odd first element, transposed and expanded inputs."""
     t, dy, dh = _case(20, 96, BF, BF, True, True, (20, 96), 9)
@@ -244,6 +267,26 @@ def test_strides_and_offsets(moe_pkg):
     x = t["x"][:1].to(DEV).expand(20, 96)
     y, h = moe_pkg.residual_norm(x, t["branch"][:1].to(DEV).expand(20, 96), pre_weight=t["pre"].to(DEV))
     assert torch.equal(y[0], y[19]) and torch.equal(h[0], h[19])
+
+
+@pytest.mark.parametrize("rows,ld", [(40, (1 << 26) + 8), (3, (1 << 30) + 8)])
+def test_rows_far_apart(moe_pkg, rows, ld):
+    """Offsets that pass 32 bits, and row strides that the fast kernels do not take."""
+    buf = torch.empty(rows * ld, dtype=BF, device=DEV)
+    x = buf.as_strided((rows, 64), (ld, 1))
+    g = torch.Generator().manual_seed(2)
+    x.copy_(torch.randn(rows, 64, generator=g))
+    u, w = torch.randn(rows, 64, generator=g).to(BF).to(DEV), torch.rand(64, generator=g).to(DEV)
+
+    def run(t):
+        leaf = t.detach().requires_grad_(True)
+        y, h = moe_pkg.residual_norm(leaf, u, pre_weight=w, post_weight=w)
+        return y.detach(), h.detach(), torch.autograd.grad([y, h], leaf, [u, u])[0]
+
+    for a, b in zip(run(x), run(x.contiguous())):  # another kernel may add in another order: one bf16 step
+        assert ((a.float() - b.float()).abs() <= 2.0 ** -6 * b.float().abs() + 2.0 ** -12).all()
+    del buf, x
+    torch.cuda.empty_cache()
 
 
 def test_half_precision_weights_get_their_own_gradient_type(moe_pkg):
