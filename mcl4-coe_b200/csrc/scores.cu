@@ -529,13 +529,15 @@ __global__ void __launch_bounds__(WARPS * 32) route_scores_kernel(ScoreArgs a) {
     __syncwarp();
     const unsigned unsure = __ballot_sync(kFull, close) >> (seg * LPT) & seg_mask;
     any_unsure |= __any_sync(kFull, close);
+    // An unsure row's picks are not read: where every lane's best is NaN, no lane equals the largest
+    // and a round writes none.  A NaN key makes its row unsure, so a settled row has all its picks.
     int id[kRows];
     bool has[kRows];
     float lc[kRows], share[kRows];
 #pragma unroll
     for (int q = 0; q < kRows; ++q) {
       const int j = q * LPT + sl;
-      id[q] = q < slots && j < a.k ? pick[j] : -1;
+      id[q] = unsure == 0 && q < slots && j < a.k ? pick[j] : -1;
       has[q] = id[q] >= 0;
       lc[q] = has[q] ? load_logit(row + id[q]) : 0.f;
     }

@@ -1,0 +1,78 @@
+"""Calls at the borders of ``route_experts``, ``residual_norm``, ``adamw_step`` and their users on B200:
+rows that are not finite, wrong lengths, captured and concurrent calls.  Routing is compared with its
+definition in float64, with the tolerances derived in ``test_gpu_m_scores.py``."""
+
+import pytest
+import torch
+
+import operators_ref as ref
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def _rows(T, E, seed, dtype=torch.float32):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randn(T, E, generator=g).to(dtype).to(DEV)
+
+
+def _ids(pkg, logits, k, **kw):
+    """ids and counts are those of the definition; returns the weights."""
+    w, ids, counts = pkg.route_experts(logits, k, **kw)
+    names = dict(num_groups="groups", renormalize="renorm")
+    want = ref.route(logits, k, **{names.get(n, n): v for n, v in kw.items()})
+    assert torch.equal(ids.cpu().long(), want[1])
+    assert torch.equal(counts.cpu().long(), want[2])
+    return w, want[0]
+
+
+# ------------------------------------------------------------------ rows of NaN
+@pytest.mark.parametrize("E", [1, 8, 64, 128, 256, 512])
+@pytest.mark.parametrize("T", [3, 700])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("with_bias", [False, True])
+def test_rows_of_nan_alone(moe_pkg, E, T, score, with_bias):
+    """Every lane's best key is NaN, in the first rows that a warp takes and in later ones."""
+    k = min(E, 8)
+    logits = _rows(T, E, E + T)
+    bad = torch.zeros(T, dtype=torch.bool)
+    bad[0] = bad[T // 2:T // 2 + 40] = True
+    logits[bad.to(DEV)] = float("nan")
+    bias = torch.linspace(-0.1, 0.1, E, device=DEV) if with_bias else None
+    for renorm in (True, False):
+        w, want = _ids(moe_pkg, logits, k, score=score, bias=bias, renormalize=renorm)
+        assert torch.isnan(w[bad.to(DEV)]).all()
+        torch.testing.assert_close(w.cpu().double()[~bad], want[~bad], rtol=2.0 ** -16, atol=0)
+    w, _ = _ids(moe_pkg, torch.full((T, E), float("nan"), device=DEV), k, score=score, bias=bias)
+    assert torch.isnan(w).all()
+
+
+@pytest.mark.parametrize("E", [8, 64, 128, 256, 512])
+@pytest.mark.parametrize("T", [3, 700])
+@pytest.mark.parametrize("spoil", [float("nan"), float("inf")])
+@pytest.mark.parametrize("groups", [1, 4])
+def test_one_logit_spoils_every_key_of_a_softmax(moe_pkg, E, T, spoil, groups):
+    """With a bias, or group sums, the keys are the softmax's: one NaN or +inf makes them all NaN."""
+    logits = _rows(T, E, 3 * E + T)
+    bad = torch.zeros(T, dtype=torch.bool)
+    bad[0] = bad[1] = bad[T // 2] = True
+    at = torch.arange(T) * 7 % E
+    logits[bad.to(DEV), at[bad].to(DEV)] = spoil
+    bias = torch.linspace(-0.1, 0.1, E, device=DEV)
+    for kw in (dict(bias=bias), dict(bias=bias, renormalize=False)):
+        w, want = _ids(moe_pkg, logits, min(E // groups, 6), num_groups=groups, top_groups=max(1, groups // 2), **kw)
+        torch.testing.assert_close(w.cpu().double()[~bad], want[~bad], rtol=2.0 ** -16, atol=0)
+
+
+@pytest.mark.parametrize("kw", [dict(score_function="sigmoid", balance_bias=True), dict(balance_bias=True)])
+@pytest.mark.parametrize("T", [40, 1500])
+def test_a_nan_token_leaves_the_other_tokens(moe_pkg, kw, T):
+    torch.manual_seed(0)
+    layer = moe_pkg.SparseMoE(moe_pkg.MoEConfig(d_model=256, expert_hidden_dim=256, num_experts=8, top_k=2, **kw)).to(DEV)
+    x = _rows(T, 256, 5, torch.bfloat16)
+    spoilt = x.clone()
+    spoilt[0] = float("nan")
+    with torch.no_grad():
+        a, b = layer(x)[0], layer(spoilt)[0]
+    assert torch.equal(a[1:], b[1:])
+    assert torch.isnan(b[0]).all()
