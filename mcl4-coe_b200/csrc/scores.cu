@@ -337,6 +337,8 @@ __device__ __noinline__ void select_exact(const ScoreArgs& a, int64_t t, ScoreSc
   const float l[1] = {has[0] ? load_logit(row + id) : 0.f};
   float share[1];
   chosen_shares<32>(has, l, 1, a.score, a.renorm, row_max, sum, share);
+  // a NaN or +inf logit makes every score of a softmax NaN, that of experts chosen by other keys too
+  if (a.score == kSoftmax && z != z) share[0] = __uint_as_float(0x7FFFFFFFu);
   if (lane < a.k) {
     a.idx[t * a.k + lane] = id;
     a.w[t * a.k + lane] = has[0] ? share[0] * a.scale : 0.f;

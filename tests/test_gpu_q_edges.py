@@ -64,6 +64,20 @@ def test_one_logit_spoils_every_key_of_a_softmax(moe_pkg, E, T, spoil, groups):
         torch.testing.assert_close(w.cpu().double()[~bad], want[~bad], rtol=2.0 ** -16, atol=0)
 
 
+@pytest.mark.parametrize("spoil", [float("nan"), float("inf")])
+@pytest.mark.parametrize("kw", [dict(bias=True), dict(num_groups=4, top_groups=1), dict(bias=True, num_groups=4, top_groups=2)])
+def test_a_spoilt_softmax_has_nan_weights(moe_pkg, spoil, kw):
+    """Every score of the row is NaN, so are its weights, whichever experts the order of NaN keys picks."""
+    for E in (8, 64, 256):
+        logits = _rows(5, E, E)
+        logits[1, E - 1] = logits[3, E // 2] = spoil
+        args = dict(kw, bias=torch.linspace(-0.1, 0.1, E, device=DEV)) if "bias" in kw else kw
+        for renorm in (True, False):
+            w, _, _ = moe_pkg.route_experts(logits, 2, renormalize=renorm, **args)
+            assert torch.isnan(w[[1, 3]]).all()
+            assert torch.isfinite(w[[0, 2, 4]]).all()
+
+
 @pytest.mark.parametrize("kw", [dict(score_function="sigmoid", balance_bias=True), dict(balance_bias=True)])
 @pytest.mark.parametrize("T", [40, 1500])
 def test_a_nan_token_leaves_the_other_tokens(moe_pkg, kw, T):
