@@ -650,6 +650,8 @@ class ExpertParallelMoE(nn.Module):
         bias = None
         if self.router_logit_bias is not None:
             bias = self.router_logit_bias.detach().to(device=xb.device, dtype=torch.float32).contiguous()
+            if bias.numel() != wr.shape[0]:
+                raise ValueError("router_logit_bias must have one entry per expert")
         vmask = None
         if valid is not None:
             vmask = valid.reshape(-1).to(device=xb.device, dtype=torch.uint8).contiguous()

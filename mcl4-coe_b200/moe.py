@@ -279,6 +279,15 @@ class SparseMoE(nn.Module):
         return (self.score_function != "softmax" or 0 < self.top_expert_groups < self.expert_groups
                 or self.routed_scale != 1.0 or self.balance_bias is not None)
 
+    def _logit_bias(self, device: torch.device, E: int) -> Tensor | None:
+        """``router_logit_bias`` as the library reads it: E contiguous fp32 values on ``device``."""
+        if self.router_logit_bias is None:
+            return None
+        bias = self.router_logit_bias.detach().to(device=device, dtype=torch.float32).contiguous()
+        if bias.numel() != E:
+            raise ValueError("router_logit_bias must have one entry per expert")
+        return bias
+
     def _workspace(self, T: int, d: int, E: int, k: int, F: int, device: torch.device) -> Tensor:
         key = (T, d, E, k, F, str(device))
         if self._ws is None or self._ws_key != key:
@@ -348,11 +357,7 @@ class SparseMoE(nn.Module):
         dn = get_or_build_grouped_cache(self.experts, "down_proj")
         xb = flat.to(torch.bfloat16).contiguous()
         wr = self.router.weight.detach().to(torch.float32).contiguous()
-        bias = None
-        if self.router_logit_bias is not None:
-            bias = self.router_logit_bias.detach().to(device=dev, dtype=torch.float32).contiguous()
-            if bias.numel() != E:
-                raise ValueError("router_logit_bias must have one entry per expert")
+        bias = self._logit_bias(dev, E)
         vmask = None
         if valid is not None:
             vmask = valid.reshape(-1).to(device=dev, dtype=torch.uint8).contiguous()
@@ -461,9 +466,7 @@ class SparseMoE(nn.Module):
             return dict(out=torch.zeros_like(x), aux_loss=zero, router_z_loss=zero,
                         counts=torch.zeros(E, dtype=torch.float32, device=dev))
         xb = flat.to(torch.bfloat16).contiguous()
-        bias = None
-        if self.router_logit_bias is not None:
-            bias = self.router_logit_bias.detach().to(device=dev, dtype=torch.float32).contiguous()
+        bias = self._logit_bias(dev, E)
         with torch.autocast(device_type=dev.type, enabled=False):
             logits = _RouterLogitsFunction.apply(self, xb, self.router.weight, bias, vmask)
             w, idx, slots = route_experts(
@@ -580,9 +583,7 @@ class SparseMoE(nn.Module):
                         counts=torch.zeros(E, dtype=torch.float32, device=dev))
         xb = flat.to(torch.bfloat16).contiguous()
         wr = self.router.weight.detach().to(device=dev, dtype=torch.float32).contiguous()
-        bias = None
-        if self.router_logit_bias is not None:
-            bias = self.router_logit_bias.detach().to(device=dev, dtype=torch.float32).contiguous()
+        bias = self._logit_bias(dev, E)
         logits = self._router_logits(xb, wr, bias).index_select(0, active)
         prior = None
         if prior_expert_mask is not None and self.recurrent_coverage_penalty > 0.0:
@@ -867,9 +868,7 @@ class _MoETrainFunction(torch.autograd.Function):
         dn = get_or_build_grouped_cache(mod.experts, "down_proj", with_bwd=True)
         xb = flat.detach().to(torch.bfloat16).contiguous()
         wr = wr_param.detach().to(torch.float32).contiguous()
-        bias = None
-        if mod.router_logit_bias is not None:
-            bias = mod.router_logit_bias.detach().to(device=dev, dtype=torch.float32).contiguous()
+        bias = mod._logit_bias(dev, E)
         vmask = None if valid is None else valid.reshape(-1).to(device=dev, dtype=torch.uint8).contiguous()
         mcap = lib.mcl4moe_padded_rows(T, E, k)
         bf = dict(dtype=torch.bfloat16, device=dev)

@@ -90,3 +90,23 @@ def test_a_nan_token_leaves_the_other_tokens(moe_pkg, kw, T):
         a, b = layer(x)[0], layer(spoilt)[0]
     assert torch.equal(a[1:], b[1:])
     assert torch.isnan(b[0]).all()
+
+
+# ------------------------------------------------------------------ wrong lengths
+def _layer(pkg, **kw):
+    torch.manual_seed(0)
+    return pkg.SparseMoE(pkg.MoEConfig(**{**dict(d_model=256, expert_hidden_dim=256, num_experts=8, top_k=2), **kw})).to(DEV)
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(score_function="sigmoid"), dict(dense_subset_k=2)])
+def test_a_logit_bias_of_another_length_is_refused(moe_pkg, kw):
+    layer, x = _layer(moe_pkg, **kw), _rows(20, 256, 1, torch.bfloat16)
+    layer.router_logit_bias = torch.zeros(7, device=DEV)
+    with pytest.raises(ValueError, match="router_logit_bias"), torch.no_grad():
+        layer(x)
+    if "dense_subset_k" not in kw:
+        with pytest.raises(ValueError, match="router_logit_bias"):
+            layer(x.requires_grad_(True))
+    layer.router_logit_bias = torch.zeros(8, device=DEV)
+    with torch.no_grad():
+        assert torch.isfinite(layer(x)[0]).all()
