@@ -655,6 +655,8 @@ class ExpertParallelMoE(nn.Module):
         vmask = None
         if valid is not None:
             vmask = valid.reshape(-1).to(device=xb.device, dtype=torch.uint8).contiguous()
+            if vmask.numel() != T:
+                raise ValueError("valid must have one entry per token")
 
         ev = self.stage_events
         mark = (lambda i: ev[i].record()) if ev is not None else (lambda i: None)

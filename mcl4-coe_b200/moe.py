@@ -658,10 +658,14 @@ class SparseMoE(nn.Module):
             w = expert_weights.to(device=dev, dtype=torch.float32).view(1, m).expand(T, m)
         else:
             w = expert_weights.to(device=dev, dtype=torch.float32).reshape(-1, m)
+        if w.shape[0] != T:
+            raise ValueError("expert_weights must have one row per token")
         order = sorted(range(m), key=lambda i: ids[i])
         idx = torch.tensor([ids[i] for i in order], dtype=torch.int32, device=dev).view(1, m).expand(T, m)
         w = w[:, order].contiguous()
         vmask = None if valid is None else valid.reshape(-1).to(device=dev, dtype=torch.uint8).contiguous()
+        if vmask is not None and vmask.numel() != T:
+            raise ValueError("valid must have one entry per token")
         out = self._forward_routed(flat.to(torch.bfloat16).contiguous(), vmask, idx.contiguous(), w)
         return out.to(x.dtype).view_as(x)
 
@@ -870,6 +874,8 @@ class _MoETrainFunction(torch.autograd.Function):
         wr = wr_param.detach().to(torch.float32).contiguous()
         bias = mod._logit_bias(dev, E)
         vmask = None if valid is None else valid.reshape(-1).to(device=dev, dtype=torch.uint8).contiguous()
+        if vmask is not None and vmask.numel() != T:
+            raise ValueError("valid must have one entry per token")
         mcap = lib.mcl4moe_padded_rows(T, E, k)
         bf = dict(dtype=torch.bfloat16, device=dev)
         out = torch.empty((T, d), **bf)

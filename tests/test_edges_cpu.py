@@ -1,8 +1,18 @@
 """Calls at the borders of the layer and of its operators that are refused, or decided on the host, checked
 without a GPU."""
 
+import os
+import sys
+from pathlib import Path
+
 import pytest
 import torch
+import torch.distributed as dist
+import torch.multiprocessing as mp
+
+from test_ep_cpu import _free_port
+
+HERE = Path(__file__).resolve().parent
 
 
 def _layer(pkg, **kw):
@@ -19,3 +29,27 @@ def test_logit_bias_has_one_entry_per_expert(moe_pkg):
             layer._logit_bias(cpu, 8)
     layer.router_logit_bias = torch.arange(8, dtype=torch.bfloat16)
     assert torch.equal(layer._logit_bias(cpu, 8), torch.arange(8, dtype=torch.float32))
+
+
+def _expert_parallel_worker(rank, port):
+    sys.path[:0] = [str(HERE.parent), str(HERE)]
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
+    dist.init_process_group("gloo", rank=rank, world_size=1)
+    try:
+        from __graft_entry__ import load_package
+        from ep_oracle_ops import OracleEPOps
+
+        ep = load_package().ExpertParallelMoE.from_dense(_layer(load_package(), num_experts=4), ops=OracleEPOps())
+        x = torch.zeros(6, 256, dtype=torch.bfloat16)
+        for n in (5, 7):
+            with pytest.raises(ValueError, match="valid"):
+                ep(x, torch.ones(n))
+        ep.router_logit_bias = torch.zeros(3)
+        with pytest.raises(ValueError, match="router_logit_bias"):
+            ep(x)
+    finally:
+        dist.destroy_process_group()
+
+
+def test_expert_parallel_refuses_wrong_lengths():
+    mp.spawn(_expert_parallel_worker, args=(_free_port(),), nprocs=1, join=True)

@@ -110,3 +110,20 @@ def test_a_logit_bias_of_another_length_is_refused(moe_pkg, kw):
     layer.router_logit_bias = torch.zeros(8, device=DEV)
     with torch.no_grad():
         assert torch.isfinite(layer(x)[0]).all()
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(score_function="sigmoid"), dict(dense_subset_k=2)])
+@pytest.mark.parametrize("n", [19, 21])
+def test_a_mask_of_another_length_is_refused(moe_pkg, kw, n):
+    layer, x = _layer(moe_pkg, **kw), _rows(20, 256, 1, torch.bfloat16)
+    valid = torch.ones(n, dtype=torch.bool, device=DEV)
+    with pytest.raises(ValueError, match="valid"), torch.no_grad():
+        layer(x, valid)
+    if "dense_subset_k" not in kw:
+        with pytest.raises(ValueError, match="valid"):
+            layer(x.requires_grad_(True), valid)
+    x = x.detach()
+    with pytest.raises(ValueError, match="valid"):
+        layer.forward_dense_subset(x, [0, 3], valid=valid)
+    with pytest.raises(ValueError, match="expert_weights"):
+        layer.forward_dense_subset(x, [0, 3], expert_weights=torch.ones(n, 2, device=DEV))
