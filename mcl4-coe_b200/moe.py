@@ -60,7 +60,7 @@ from torch.autograd.function import once_differentiable
 from . import _lib
 from .norms import residual_norm
 from .nvfp4 import _stream_handle, get_or_build_grouped_cache, invalidate_cache, nvfp4_grouped_linear
-from .routing import GROUP_SCORES, SCORE_FUNCTIONS, route_experts
+from .routing import GROUP_SCORES, SCORE_FUNCTIONS, _raw_stream, route_experts
 
 RESIDUAL_GATES = ("none", "linear", "sigmoid", "tanh")
 
@@ -167,8 +167,8 @@ class SparseMoE(nn.Module):
         # exist) recorded at the stage boundaries of the next forward calls.
         self.stage_events: Sequence[torch.cuda.Event] | None = None
         self.last_h: Tensor | None = None
-        self._ws: Tensor | None = None
-        self._ws_key: tuple | None = None
+        # the last call's workspace, its shape and the stream that may use it again (None: a captured call's)
+        self._ws_held: tuple[Tensor, tuple, int | None] | None = None
         self._graphs: dict | None = None  # CUDA-graph replay (enable_cuda_graph)
 
     @torch.no_grad()
@@ -289,14 +289,24 @@ class SparseMoE(nn.Module):
         return bias
 
     def _workspace(self, T: int, d: int, E: int, k: int, F: int, device: torch.device) -> Tensor:
-        key = (T, d, E, k, F, str(device))
-        if self._ws is None or self._ws_key != key:
-            nbytes = _lib.load().mcl4moe_moe_workspace_size(T, d, E, k, F)
-            if nbytes == 0 and T > 0:
-                raise ValueError(f"unsupported MoE shape T={T} d={d} E={E} k={k} F={F}")
-            self._ws = torch.empty((max(nbytes, 256),), dtype=torch.uint8, device=device)
-            self._ws_key = key
-        return self._ws
+        """Scratch memory of one call.  It is used again by the next call of its shape on its stream, which
+        runs behind it; calls on two streams would overwrite each other's operands.  A captured call's
+        belongs to its graph, whose replays go on using it."""
+        key = (T, d, E, k, F, device)
+        stream = None if torch.cuda.is_current_stream_capturing() else _raw_stream(device.index)
+        held = self._ws_held
+        if held is not None and stream is not None and held[1:] == (key, stream):
+            return held[0]
+        nbytes = _lib.load().mcl4moe_moe_workspace_size(T, d, E, k, F)
+        if nbytes == 0 and T > 0:
+            raise ValueError(f"unsupported MoE shape T={T} d={d} E={E} k={k} F={F}")
+        ws = torch.empty((max(nbytes, 256),), dtype=torch.uint8, device=device)
+        self._ws_held = (ws, key, stream)
+        return ws
+
+    @property
+    def _ws(self) -> Tensor | None:
+        return None if self._ws_held is None else self._ws_held[0]
 
     def _run_grouped_experts(self, gx: Tensor, offs: Tensor) -> Tensor:
         """The reference's operator seam (src/mcl4_coe/backbone.py:569-577)."""
@@ -673,12 +683,12 @@ class SparseMoE(nn.Module):
         """Synchronise and return the error word of the last forward (0 = every
         device-side wait completed; 1xx/2xx/3xx = TMA producer / MMA issuer /
         epilogue wait of a GEMM gave up after its time limit)."""
-        if self._ws is None or self._ws_key is None:
+        if self._ws_held is None:
             return 0
-        T, d, E, k, F, _ = self._ws_key
+        ws, (T, d, E, k, F, _), _ = self._ws_held
         lib = _lib.load()
-        off = lib.mcl4moe_workspace_region(self._ws.data_ptr(), 8, T, d, E, k, F) - self._ws.data_ptr()
-        return int(self._ws[off:off + 4].view(torch.int32).item())
+        off = lib.mcl4moe_workspace_region(ws.data_ptr(), 8, T, d, E, k, F) - ws.data_ptr()
+        return int(ws[off:off + 4].view(torch.int32).item())
 
     # ------------------------------------------------------------------ state dict
     def _save_to_state_dict(self, destination: dict, prefix: str, keep_vars: bool) -> None:

@@ -127,3 +127,71 @@ def test_a_mask_of_another_length_is_refused(moe_pkg, kw, n):
         layer.forward_dense_subset(x, [0, 3], valid=valid)
     with pytest.raises(ValueError, match="expert_weights"):
         layer.forward_dense_subset(x, [0, 3], expert_weights=torch.ones(n, 2, device=DEV))
+
+
+# ------------------------------------------------------------------ the layer's scratch memory
+SCORED = dict(score_function="sigmoid", balance_bias=True)
+
+
+@pytest.mark.parametrize("kw", [dict(), SCORED])
+def test_workspace_belongs_to_a_stream(moe_pkg, kw):
+    layer, x = _layer(moe_pkg, **kw), _rows(20, 256, 1, torch.bfloat16)
+    with torch.no_grad():
+        layer(x)
+        first = layer._ws
+        layer(x)
+        assert layer._ws is first
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            layer(x)
+        assert layer._ws is not first
+    torch.cuda.current_stream().wait_stream(side)
+
+
+@pytest.mark.parametrize("kw", [dict(), SCORED])
+def test_layer_on_two_streams_at_once(moe_pkg, kw):
+    layer = _layer(moe_pkg, **kw)
+    xs = [_rows(3000, 256, 7 + i, torch.bfloat16) for i in range(2)]
+    with torch.no_grad():
+        want = [layer(x)[0].clone() for x in xs]
+        streams = [torch.cuda.Stream() for _ in xs]
+        torch.cuda.synchronize()
+        got = [[], []]
+        for _ in range(20):
+            for s, x, g in zip(streams, xs, got):
+                with torch.cuda.stream(s):
+                    g.append(layer(x)[0])
+        torch.cuda.synchronize()
+    for w, g in zip(want, got):
+        assert all(torch.equal(w, o) for o in g)
+
+
+@pytest.mark.parametrize("kw", [dict(), SCORED])
+def test_captured_layer_keeps_its_workspace(moe_pkg, kw):
+    """Captured by hand; other calls of other sizes between the replays, and memory that takes what they freed."""
+    layer, x = _layer(moe_pkg, **kw), _rows(500, 256, 3, torch.bfloat16)
+    other = _rows(900, 256, 4, torch.bfloat16)
+    static = torch.empty_like(x)
+    with torch.no_grad():
+        want = [t.clone() for t in layer(x)]
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            layer(static.copy_(x))
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = layer(static)
+        captured = layer._ws
+        layer(x)
+        assert layer._ws is not captured
+        del captured
+        for _ in range(3):
+            layer(other)
+            taken = [torch.full((1 << 20,), 0xA5, dtype=torch.uint8, device=DEV) for _ in range(16)]
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(out, want))
+            assert all(bool((t == 0xA5).all()) for t in taken)
+            del taken
