@@ -235,5 +235,19 @@ class AdamW(torch.optim.Optimizer):
                 if isinstance(value, Tensor):
                     self.state[p][name] = value.detach().to(p.device, copy=True)
         for group in self.param_groups:
+            devices = {str(p.device): p.device for p in group["params"]}
             if "step_counts" in group:
-                group["step_counts"] = {d: t.detach().to(d, copy=True) for d, t in group["step_counts"].items()}
+                group["step_counts"] = _placed_counts(group["step_counts"], devices)
+            if isinstance(group["lr"], Tensor) and len(devices) == 1:
+                group["lr"] = group["lr"].to(*devices.values())
+
+
+def _placed_counts(saved: dict, devices: dict) -> dict:
+    """A group's saved step counts on the devices that its parameters have now: by name where every saved
+    device is among them, else (a checkpoint of another rank) the one value that all of them hold."""
+    if set(saved) <= set(devices):
+        return {d: t.detach().to(devices[d], copy=True) for d, t in saved.items()}
+    values = {int(t) for t in saved.values()}
+    if len(values) != 1:
+        raise ValueError(f"the saved step counts {saved} do not say which holds for parameters on {sorted(devices)}")
+    return {d: torch.full((), *values, dtype=torch.int64, device=device) for d, device in devices.items()}

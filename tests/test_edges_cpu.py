@@ -53,3 +53,42 @@ def _expert_parallel_worker(rank, port):
 
 def test_expert_parallel_refuses_wrong_lengths():
     mp.spawn(_expert_parallel_worker, args=(_free_port(),), nprocs=1, join=True)
+
+
+def _capturable(pkg, counts):
+    """(a fresh optimizer of two parameters, a checkpoint of such a one with ``counts``)"""
+    params = [torch.nn.Parameter(torch.zeros(5)), torch.nn.Parameter(torch.zeros(3))]
+    opt = pkg.AdamW(params, capturable=True)
+    saved = opt.state_dict()
+    saved["state"] = {i: dict(step=0, exp_avg=torch.ones(p.shape), exp_avg_sq=torch.ones(p.shape))
+                      for i, p in enumerate(params)}
+    saved["param_groups"][0]["step_counts"] = {d: torch.tensor(n) for d, n in counts.items()}
+    return opt, saved
+
+
+@pytest.mark.parametrize("counts", [{"cpu": 41}, {"cuda:0": 41}, {"cuda:0": 41, "cuda:1": 41}, {"cpu": 41, "cuda:1": 41}])
+def test_device_step_count_goes_on_after_loading(moe_pkg, counts):
+    """A checkpoint of one device loaded on another: the count goes where the moments go."""
+    opt, saved = _capturable(moe_pkg, counts)
+    opt.load_state_dict(saved)
+    group = opt.param_groups[0]
+    assert {d: int(t) for d, t in group["step_counts"].items()} == {"cpu": 41}
+    after = opt._device_counts(group, {(torch.device("cpu"), torch.float32): []})
+    assert int(after[torch.device("cpu")]) == 42
+    assert saved["param_groups"][0]["step_counts"] == {d: torch.tensor(41) for d in counts}
+
+
+def test_device_step_counts_that_differ_are_not_guessed(moe_pkg):
+    opt, saved = _capturable(moe_pkg, {"cuda:0": 41, "cuda:1": 40})
+    with pytest.raises(ValueError, match="step counts"):
+        opt.load_state_dict(saved)
+    opt, saved = _capturable(moe_pkg, {})
+    opt.load_state_dict(saved)
+    assert opt.param_groups[0]["step_counts"] == {}
+
+
+def test_learning_rate_tensor_follows_the_parameters(moe_pkg):
+    p = torch.nn.Parameter(torch.zeros(5))
+    opt = moe_pkg.AdamW([p], lr=torch.tensor(1e-3))
+    opt.load_state_dict(opt.state_dict())
+    assert opt.param_groups[0]["lr"].device == p.device and float(opt.param_groups[0]["lr"]) == pytest.approx(1e-3)

@@ -195,3 +195,30 @@ def test_captured_layer_keeps_its_workspace(moe_pkg, kw):
             assert all(torch.equal(a, b) for a, b in zip(out, want))
             assert all(bool((t == 0xA5).all()) for t in taken)
             del taken
+
+
+# ------------------------------------------------------------------ the optimizer
+@pytest.mark.parametrize("bits", [32, 8])
+def test_capturable_optimizer_resumes_from_another_device(moe_pkg, bits):
+    """A checkpoint whose count has another device's name: the next steps are those of going on."""
+    def make(values):
+        params = [torch.nn.Parameter(v.detach().clone()) for v in values]
+        return params, moe_pkg.AdamW(params, lr=1e-2, state_bits=bits, capturable=True, seed=4)
+
+    def steps(params, opt, n, first):
+        for i in range(first, first + n):
+            for j, p in enumerate(params):
+                p.grad = torch.full_like(p, 0.1 * (i + 1)) * torch.arange(1, p.numel() + 1, device=DEV)
+            opt.step()
+
+    params, opt = make([torch.linspace(-1, 1, n, device=DEV) for n in (300, 17)])
+    steps(params, opt, 3, 0)
+    saved = opt.state_dict()
+    counts = saved["param_groups"][0]["step_counts"]
+    assert list(counts) == ["cuda:0"] and int(counts["cuda:0"]) == 3
+    saved["param_groups"][0]["step_counts"] = {"cuda:7": counts["cuda:0"].cpu()}
+    again, resumed = make(params)
+    resumed.load_state_dict(saved)
+    steps(params, opt, 2, 3)
+    steps(again, resumed, 2, 3)
+    assert all(torch.equal(a, b) for a, b in zip(params, again))
