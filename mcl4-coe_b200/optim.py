@@ -142,7 +142,8 @@ class AdamW(torch.optim.Optimizer):
     ``t`` (clipping).  ``lr`` may be a float32 tensor on the parameters' device.
 
     ``capturable`` keeps one step count per group and device in device memory, so that a
-    captured step goes on counting when it is replayed; a replay does not go through torch,
+    captured step goes on counting when it is replayed.  A capture needs it, and an eager step
+    before, which makes the state.  A replay does not go through torch,
     so the parameters' versions stand still and an NVFP4 weight cache has to be told
     (``invalidate_cache``).
     """
@@ -185,6 +186,8 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        if torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
+            self._check_capture()
         place = 0  # a parameter's number in the optimizer keys its noise
         for group in self.param_groups:
             calls: dict = {}
@@ -214,6 +217,18 @@ class AdamW(torch.optim.Optimizer):
                            masters=[s["master"] for s in states] if master else None, grad_scale=grad_scale,
                            seed=group["seed"], indices=[i for _, _, i in items])
         return loss
+
+    def _check_capture(self) -> None:
+        """What a replay could not repeat: a step count on the host would stay at its value, and state made
+        during the capture would be made again by each replay."""
+        for group in self.param_groups:
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                if not group["capturable"]:
+                    raise RuntimeError("a captured AdamW step needs capturable=True")
+                if not self.state.get(p) or str(p.device) not in group.get("step_counts", {}):
+                    raise RuntimeError("an AdamW step can be captured once an eager one has made the parameters' state")
 
     def _device_counts(self, group: dict, calls: dict) -> dict | None:
         """capturable: the group's step count on each device, moved on by one."""

@@ -92,3 +92,19 @@ def test_learning_rate_tensor_follows_the_parameters(moe_pkg):
     opt = moe_pkg.AdamW([p], lr=torch.tensor(1e-3))
     opt.load_state_dict(opt.state_dict())
     assert opt.param_groups[0]["lr"].device == p.device and float(opt.param_groups[0]["lr"]) == pytest.approx(1e-3)
+
+
+def test_a_capture_needs_a_device_count_and_state(moe_pkg, monkeypatch):
+    monkeypatch.setattr(torch.cuda, "is_initialized", lambda: True)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    p = torch.nn.Parameter(torch.zeros(5))
+    opt = moe_pkg.AdamW([p])
+    opt.step()  # nothing has a gradient
+    p.grad = torch.ones(5)
+    with pytest.raises(RuntimeError, match="capturable"):
+        opt.step()
+    assert not opt.state
+    opt = moe_pkg.AdamW([p], capturable=True)
+    with pytest.raises(RuntimeError, match="eager"):
+        opt.step()
+    assert not opt.state and "step_counts" not in opt.param_groups[0]

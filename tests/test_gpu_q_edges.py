@@ -222,3 +222,24 @@ def test_capturable_optimizer_resumes_from_another_device(moe_pkg, bits):
     steps(params, opt, 2, 3)
     steps(again, resumed, 2, 3)
     assert all(torch.equal(a, b) for a, b in zip(params, again))
+
+
+def test_captures_that_could_not_replay_are_refused(moe_pkg):
+    params = [torch.nn.Parameter(torch.ones(n, device=DEV)) for n in (300, 17)]
+    for p in params:
+        p.grad = torch.ones_like(p)
+    eager, fresh = moe_pkg.AdamW(params), moe_pkg.AdamW(params, capturable=True)
+    eager.step()
+    torch.cuda.synchronize()
+    before = [p.detach().clone() for p in params]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="capturable"):
+            eager.step()
+        with pytest.raises(RuntimeError, match="eager"):
+            fresh.step()
+        params[0].detach().add_(1.0)
+    graph.replay()
+    eager.step()  # goes on eagerly, at step 2
+    assert eager.state[params[0]]["step"] == 2 and not fresh.state
+    assert not torch.equal(before[1], params[1])
