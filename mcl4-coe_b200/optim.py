@@ -191,6 +191,8 @@ class AdamW(torch.optim.Optimizer):
         place = 0  # a parameter's number in the optimizer keys its noise
         for group in self.param_groups:
             calls: dict = {}
+            if "step_counts" in group and not group["capturable"]:
+                self._host_counts(group)
             for p in group["params"]:
                 place += 1
                 if p.grad is None:
@@ -231,15 +233,26 @@ class AdamW(torch.optim.Optimizer):
                     raise RuntimeError("an AdamW step can be captured once an eager one has made the parameters' state")
 
     def _device_counts(self, group: dict, calls: dict) -> dict | None:
-        """capturable: the group's step count on each device, moved on by one."""
+        """capturable: the group's step count on each device, moved on by one.  A group whose ``capturable``
+        was changed (a checkpoint brings its own) goes on from where its other kind of count stood."""
         if not group["capturable"]:
             return None
         counts = group.setdefault("step_counts", {})
         for device in {key[0] for key in calls}:
             if str(device) not in counts:
-                counts[str(device)] = torch.zeros((), dtype=torch.int64, device=device)
+                before = {s["step"] for key, items in calls.items() if key[0] == device for _, s, _ in items}
+                if len(before) != 1:
+                    raise ValueError(f"capturable keeps one step count, these parameters have {sorted(before)}")
+                counts[str(device)] = torch.full((), *before, dtype=torch.int64, device=device)
             counts[str(device)] += 1
         return {key[0]: counts[str(key[0])] for key in calls}
+
+    def _host_counts(self, group: dict) -> None:
+        """Not capturable (any more): the counts that lived on the devices, for each parameter."""
+        counts = {d: int(t) for d, t in group.pop("step_counts").items()}
+        for p in group["params"]:
+            if self.state.get(p) and str(p.device) in counts:
+                self.state[p]["step"] = counts[str(p.device)]
 
     def load_state_dict(self, state_dict: dict) -> None:
         """As ``torch.optim.Optimizer``'s, which would cast the moments to the parameters' type."""

@@ -108,3 +108,19 @@ def test_a_capture_needs_a_device_count_and_state(moe_pkg, monkeypatch):
     with pytest.raises(RuntimeError, match="eager"):
         opt.step()
     assert not opt.state and "step_counts" not in opt.param_groups[0]
+
+
+def test_a_changed_kind_of_step_count_goes_on(moe_pkg):
+    params = [torch.nn.Parameter(torch.zeros(n)) for n in (5, 3)]
+    opt = moe_pkg.AdamW(params, capturable=True)
+    group, cpu = opt.param_groups[0], torch.device("cpu")
+    states = [opt.state[p] for p in params]
+    for s in states:
+        s.update(opt._new_state(params[0], group), step=4)
+    items = [(p, s, i) for i, (p, s) in enumerate(zip(params, states))]
+    assert int(opt._device_counts(group, {(cpu, 4): items})[cpu]) == 5
+    opt._host_counts(group)
+    assert [s["step"] for s in states] == [5, 5] and "step_counts" not in group
+    states[0]["step"] = 2
+    with pytest.raises(ValueError, match="step count"):
+        opt._device_counts(group, {(cpu, 2): items[:1], (cpu, 5): items[1:]})

@@ -243,3 +243,23 @@ def test_captures_that_could_not_replay_are_refused(moe_pkg):
     eager.step()  # goes on eagerly, at step 2
     assert eager.state[params[0]]["step"] == 2 and not fresh.state
     assert not torch.equal(before[1], params[1])
+
+
+def test_capturable_may_change_between_steps(moe_pkg):
+    """The step count goes on.  The factors of a step come from powers in double on the host or on the
+    device, at most one float32 rounding apart (2^-23 of an update of about lr), six times."""
+    def run(kinds):
+        p = torch.nn.Parameter(torch.linspace(-1, 1, 300, device=DEV))
+        opt = moe_pkg.AdamW([p], lr=1e-2, capturable=kinds[0])
+        for i, kind in enumerate(kinds):
+            opt.param_groups[0]["capturable"] = kind
+            p.grad = torch.full_like(p, 0.1 * (i + 1))
+            opt.step()
+        return p.detach(), opt
+
+    want, _ = run([False] * 6)
+    for kinds in ([False, False, False, True, True, True], [True, True, False, False, True, False]):
+        got, opt = run(kinds)
+        # the parameters round to 2^-24 of themselves with each update
+        torch.testing.assert_close(got, want, rtol=6 * 2.0 ** -23, atol=6 * 1e-2 * 2.0 ** -22)
+        assert ("step_counts" in opt.param_groups[0]) == kinds[-1]
