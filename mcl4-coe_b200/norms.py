@@ -11,7 +11,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .nvfp4 import _ptr, _require_cuda
-from .routing import DTYPE_CODES, _f32, _launch, _ld, _rows
+from .routing import DTYPE_CODES, _f32, _launch, _ld, _refuse_tangents, _rows
 
 GATE_ACTIVATIONS = ("none", "sigmoid", "tanh")
 MAX_COLS = 16384
@@ -157,7 +157,7 @@ def residual_norm(x: Tensor, branch: Tensor | None = None, *, post_weight: Tenso
     branch's, else ``x``'s).  The weights are ``[d]``; ``gate`` broadcasts to ``x``
     (one value for each channel, token or element, or one row for each sequence) and
     goes through ``gate_activation`` ("none", "sigmoid", "tanh").  Arithmetic is fp32,
-    each output is rounded once.  Every tensor gets its gradient; differentiable once.
+    each output is rounded once.  Every tensor gets its gradient; differentiable once, in reverse mode.
     """
     if gate_activation not in GATE_ACTIVATIONS:
         raise ValueError(f"gate_activation must be one of {GATE_ACTIVATIONS}, got {gate_activation!r}")
@@ -184,6 +184,7 @@ def residual_norm(x: Tensor, branch: Tensor | None = None, *, post_weight: Tenso
     mode, gate_rows, gate_2d = _NONE, 0, None
     if gate is not None:
         gate_2d, mode, gate_rows = _gate_form(gate, x)
+    _refuse_tangents("residual_norm", x, branch, post_weight, pre_weight, gate)
     _require_cuda(x, "residual_norm")
     tensors = (_rows(x), None if branch is None else _rows(branch), _f32(post_weight), _f32(pre_weight), gate_2d)
     form = (mode, gate_rows, GATE_ACTIVATIONS.index(gate_activation), norm_dtype,

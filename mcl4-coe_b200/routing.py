@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -47,6 +48,14 @@ def _rows(t: Tensor) -> Tensor:
     if (t.stride(1) != 1 and t.shape[1] > 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
         t = t.contiguous()
     return t
+
+
+def _refuse_tangents(what: str, *tensors: Tensor | None) -> None:
+    """Forward-mode derivatives, which the kernels would drop without a word."""
+    if getattr(forward_ad, "_current_level", 0) < 0:  # outside of a dual level no tensor has a tangent
+        return
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{what} has no forward-mode derivative")
 
 
 def _f32(t: Tensor | None) -> Tensor | None:
@@ -128,7 +137,7 @@ def route_experts(logits: Tensor, top_k: int, *, score: str = "softmax", bias: T
     runs out of experts has id -1 and weight 0 in its last slots, as have rows whose
     ``valid`` (``[..]``) is false.  NaN ranks first and makes its row's weights NaN.
     ids follow exact arithmetic on the given logits (near ties are decided in float64).
-    The gradient reaches the logits through the weights; differentiable once.
+    The gradient reaches the logits through the weights; differentiable once, in reverse mode.
     """
     if logits.ndim < 1 or logits.dtype not in DTYPE_CODES:
         raise ValueError(f"logits must be bf16, fp16 or fp32 rows, got {logits.dtype} {tuple(logits.shape)}")
@@ -158,6 +167,7 @@ def route_experts(logits: Tensor, top_k: int, *, score: str = "softmax", bias: T
         if valid.dtype != torch.bool:
             valid = valid != 0
         valid = valid.contiguous()
+    _refuse_tangents("route_experts", logits)
     _require_cuda(logits, "route_experts")
     lead = logits.shape[:-1]
     rows = _rows(logits)

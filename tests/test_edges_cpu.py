@@ -9,6 +9,7 @@ import pytest
 import torch
 import torch.distributed as dist
 import torch.multiprocessing as mp
+from torch.autograd import forward_ad
 
 from test_ep_cpu import _free_port
 
@@ -124,3 +125,19 @@ def test_a_changed_kind_of_step_count_goes_on(moe_pkg):
     states[0]["step"] = 2
     with pytest.raises(ValueError, match="step count"):
         opt._device_counts(group, {(cpu, 2): items[:1], (cpu, 5): items[1:]})
+
+
+def test_forward_mode_derivatives_are_refused(moe_pkg):
+    x, w = torch.zeros(3, 8), torch.ones(8)
+    with forward_ad.dual_level():
+        dx, dw = forward_ad.make_dual(x, torch.ones_like(x)), forward_ad.make_dual(w, torch.ones_like(w))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            moe_pkg.route_experts(dx, 2)
+        for args, kw in (((dx, x), {}), ((x, dx), {}), ((x, x), dict(gate=dw)), ((x, x), dict(post_weight=dw)),
+                         ((x,), dict(pre_weight=dw))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                moe_pkg.residual_norm(*args, **kw)
+        with pytest.raises(ValueError, match="CUDA"):  # nothing has a tangent
+            moe_pkg.residual_norm(x, x)
+    with pytest.raises((NotImplementedError, RuntimeError)):
+        torch.func.jvp(lambda t: moe_pkg.route_experts(t, 2)[0], (x,), (x,))
