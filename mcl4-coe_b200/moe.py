@@ -516,8 +516,19 @@ class SparseMoE(nn.Module):
             raise ValueError("this layer has no balance_bias (MoEConfig.balance_bias)")
         if counts.shape != self.balance_bias.shape:
             raise ValueError("counts must have one entry per expert")
-        counts = counts.to(self.balance_bias)
+        if self.balance_bias.dtype != torch.float32:  # a checkpoint's own buffer, taken over as it was
+            self.balance_bias = self.balance_bias.float()
+        counts = counts.to(device=self.balance_bias.device, dtype=torch.float64)
         self.balance_bias.add_(torch.sign(counts.mean() - counts), alpha=rate)
+
+    def _apply(self, fn, recurse: bool = True):
+        """``balance_bias`` stays in fp32 when the layer's type changes: in bf16 steps of 0.001 would be lost
+        from 0.5 on."""
+        bias = self.balance_bias
+        super()._apply(fn, recurse)
+        if bias is not None and self.balance_bias.dtype != torch.float32:
+            self.balance_bias = bias.to(device=self.balance_bias.device, dtype=torch.float32)
+        return self
 
     # ------------------------------------------------------------------ routing variants
     def _router_logits(self, xb: Tensor, wr: Tensor, bias: Tensor | None) -> Tensor:

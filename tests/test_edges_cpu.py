@@ -141,3 +141,33 @@ def test_forward_mode_derivatives_are_refused(moe_pkg):
             moe_pkg.residual_norm(x, x)
     with pytest.raises((NotImplementedError, RuntimeError)):
         torch.func.jvp(lambda t: moe_pkg.route_experts(t, 2)[0], (x,), (x,))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float64])
+def test_balance_bias_keeps_float32(moe_pkg, dtype):
+    start = torch.linspace(-0.9, 0.9, 8) + 1e-4
+    for make in (lambda m: m.to(dtype), lambda m: torch.nn.Sequential(m).to(dtype)[0]):
+        layer = _layer(moe_pkg, balance_bias=True)
+        layer.balance_bias.copy_(start)
+        layer = make(layer)
+        assert layer.router.weight.dtype == dtype
+        assert layer.balance_bias.dtype == torch.float32 and torch.equal(layer.balance_bias, start)
+        assert "balance_bias" in dict(layer.named_buffers())
+        # loads that 8 significant bits do not tell apart, 1000 times
+        counts = torch.tensor([1001, 1001, 1001, 1001, 999, 999, 999, 999])
+        for _ in range(1000):
+            layer.update_balance_bias(counts, rate=1e-3)
+        # each of the 1000 sums rounds to 2^-24 of at most 2
+        moved = torch.tensor([-1.0] * 4 + [1.0] * 4)
+        torch.testing.assert_close(layer.balance_bias, start + moved, rtol=0, atol=1000 * 2.0 ** -23)
+    assert _layer(moe_pkg).to(dtype).balance_bias is None
+
+
+def test_balance_bias_of_a_checkpoint_in_bf16(moe_pkg):
+    layer = _layer(moe_pkg, balance_bias=True)
+    state = {n: t.to(torch.bfloat16) for n, t in layer.state_dict().items()}
+    state["balance_bias"].fill_(0.75)
+    layer.load_state_dict(state, assign=True)
+    layer.update_balance_bias(torch.arange(8), rate=1e-3)
+    want = 0.75 + 1e-3 * torch.tensor([1.0] * 4 + [-1.0] * 4)
+    torch.testing.assert_close(layer.balance_bias, want, rtol=2.0 ** -23, atol=0)
