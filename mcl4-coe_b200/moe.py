@@ -50,6 +50,7 @@ from __future__ import annotations
 
 import ctypes
 import random
+import warnings
 from dataclasses import dataclass
 from typing import Any, Sequence
 
@@ -211,8 +212,12 @@ class SparseMoE(nn.Module):
         that dominates small decode batches.  While enabled the weights are not
         re-checked per call: call ``enable_cuda_graph()`` again after changing them
         (or growing / pruning experts) to capture afresh.  Forward only; no
-        ``forward_details``.
+        ``forward_details``.  Calls with another routing than plain softmax top-k (the
+        reference's variants, routing from scores) run eagerly all the same.
         """
+        if enabled and self._scored():
+            warnings.warn("enable_cuda_graph serves plain softmax top-k alone: this layer routes from scores and "
+                          "goes on running eagerly", stacklevel=2)
         self._graphs = {} if enabled else None
 
     def _graph_forward(self, flat: Tensor, valid: Tensor | None, x_shape, x_dtype):

@@ -171,3 +171,11 @@ def test_balance_bias_of_a_checkpoint_in_bf16(moe_pkg):
     layer.update_balance_bias(torch.arange(8), rate=1e-3)
     want = 0.75 + 1e-3 * torch.tensor([1.0] * 4 + [-1.0] * 4)
     torch.testing.assert_close(layer.balance_bias, want, rtol=2.0 ** -23, atol=0)
+
+
+def test_enable_cuda_graph_says_where_it_does_nothing(moe_pkg, recwarn):
+    _layer(moe_pkg).enable_cuda_graph()
+    _layer(moe_pkg, score_function="sigmoid").enable_cuda_graph(False)
+    assert not recwarn.list
+    with pytest.warns(UserWarning, match="routes from scores"):
+        _layer(moe_pkg, score_function="sigmoid").enable_cuda_graph()
