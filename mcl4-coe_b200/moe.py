@@ -465,7 +465,10 @@ class SparseMoE(nn.Module):
         if self.router.weight.shape[0] != E:
             raise ValueError("router rows must match the number of experts")
         if self.balance_bias is not None and self.balance_bias.numel() != E:
-            raise ValueError("balance_bias must have one entry per expert")
+            raise ValueError(f"balance_bias has {self.balance_bias.numel()} entries for {E} experts: give the layer one "
+                             "for each (0 for a new expert) when its experts change")
+        if E % self.expert_groups != 0:
+            raise ValueError(f"{E} experts do not form {self.expert_groups} groups: change expert_groups with the experts")
         self.num_experts = E
         flat = x.reshape(-1, x.shape[-1])
         T = flat.shape[0]

@@ -263,3 +263,42 @@ def test_capturable_may_change_between_steps(moe_pkg):
         # the parameters round to 2^-24 of themselves with each update
         torch.testing.assert_close(got, want, rtol=6 * 2.0 ** -23, atol=6 * 1e-2 * 2.0 ** -22)
         assert ("step_counts" in opt.param_groups[0]) == kinds[-1]
+
+
+# ------------------------------------------------------------------ experts that come and go
+def test_scored_layer_grows_and_prunes(moe_pkg):
+    """balance_bias and expert_groups change with the experts; until then the call is refused."""
+    layer = _layer(moe_pkg, score_function="sigmoid", balance_bias=True, expert_groups=4, top_expert_groups=2)
+    layer.update_balance_bias(torch.arange(8.0))
+    x = _rows(40, 256, 2, torch.bfloat16)
+
+    def experts(keep, new):
+        added = [moe_pkg.SwiGLUExpert(256, 256).to(DEV) for _ in range(new)]
+        layer.experts = torch.nn.ModuleList([layer.experts[i] for i in keep] + added)
+        router = torch.nn.Linear(256, len(keep) + new, bias=False).to(DEV)
+        router.weight[: len(keep)] = layer.router.weight[keep]
+        layer.router = router
+
+    def check(E):
+        out, _, _, load = layer(x)
+        logits = layer._router_logits(x, layer.router.weight.float().contiguous(), None)
+        _, ids, _ = ref.route(logits, 2, score="sigmoid", bias=layer.balance_bias, groups=layer.expert_groups, top_groups=2)
+        want = torch.zeros(40, E).scatter_(1, ids, 1.0)
+        assert torch.equal(layer.last_selected_mask.cpu(), want) and torch.isfinite(out).all() and load.shape == (E,)
+
+    with torch.no_grad():
+        check(8)
+        experts(list(range(8)), 2)
+        with pytest.raises(ValueError, match="balance_bias"):
+            layer(x)
+        layer.balance_bias = torch.cat([layer.balance_bias, torch.zeros(2, device=DEV)])
+        with pytest.raises(ValueError, match="expert_groups"):
+            layer(x)
+        layer.expert_groups = 5
+        check(10)
+        keep = [0, 1, 2, 4, 5, 7, 8, 9]
+        experts(keep, 0)
+        layer.balance_bias = layer.balance_bias[keep]
+        layer.expert_groups = 4
+        check(8)
+    assert layer.state_dict()["balance_bias"].shape == (8,)
