@@ -17,13 +17,16 @@ GATE_ACTIVATIONS = ("none", "sigmoid", "tanh")
 MAX_COLS = 16384
 _NONE, _CHANNEL, _ROW, _FULL = range(4)
 # Rows from which a gate shared by consecutive rows is summed inside the kernel (one partial
-# row of column sums per group); smaller groups are written out as one gate row per row.
+# row of column sums per group); smaller groups are written out as one gate row per row, unless a
+# 16-bit gate's gradient would be rounded for each row then.
 _MIN_GROUP_ROWS = 32
 _MAX_GROUPS = 65533
 
 
 def _gate_form(gate: Tensor, x: Tensor) -> tuple[Tensor, int, int]:
-    """(gate, mode, rows that share a gate row) for a gate that broadcasts to ``x``."""
+    """(gate, mode, rows that share a gate row) for a gate that broadcasts to ``x``.  A 16-bit gate's gradient
+    is rounded when its rows are added up, not before: where they are added here and not in the kernel, the
+    gate goes in as float32 (element-wise then through the kernels of mixed types)."""
     if gate.ndim == 1 and gate.shape[0] == x.shape[-1]:
         return gate.contiguous().view(1, -1), _CHANNEL, max(1, x.numel() // x.shape[-1])
     if gate.ndim > x.ndim or any(g != 1 and g != s for g, s in zip(gate.shape[::-1], x.shape[::-1])):
@@ -33,7 +36,10 @@ def _gate_form(gate: Tensor, x: Tensor) -> tuple[Tensor, int, int]:
     rows = x.numel() // max(1, d)
     if lead == x_lead and gate.shape[-1] == d and rows > 1:
         return _rows(gate), _FULL, 1
+    summed = gate.dtype != torch.float32 and gate.requires_grad and torch.is_grad_enabled()
     if gate.shape[-1] == 1 and d > 1:
+        if summed and gate.numel() != rows:
+            gate = gate.float()
         return gate.expand(*x_lead, 1).reshape(rows).contiguous(), _ROW, 1
     cut = max((i + 1 for i, s in enumerate(lead) if s != 1), default=0)
     groups = 1
@@ -41,8 +47,10 @@ def _gate_form(gate: Tensor, x: Tensor) -> tuple[Tensor, int, int]:
         groups *= s
     if lead[:cut] == x_lead[:cut]:
         share = max(1, rows // max(1, groups))
-        if groups == 1 or (share >= _MIN_GROUP_ROWS and groups <= _MAX_GROUPS):
+        if groups == 1 or ((share >= _MIN_GROUP_ROWS or summed) and 0 < groups <= _MAX_GROUPS):
             return gate.reshape(groups, d).contiguous(), _CHANNEL, share
+    if summed:
+        gate = gate.float()
     return gate.expand(x.shape).reshape(rows, d).contiguous(), _FULL, 1
 
 

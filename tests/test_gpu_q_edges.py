@@ -302,3 +302,38 @@ def test_scored_layer_grows_and_prunes(moe_pkg):
         layer.expert_groups = 4
         check(8)
     assert layer.state_dict()["balance_bias"].shape == (8,)
+
+
+# ------------------------------------------------------------------ gates that broadcast
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,shape", [((3, 40), shape) for shape in (
+    (3, 1, 64), (1, 40, 64), (1, 40, 1), (3, 1, 1), (1, 1, 64), (64,), (1,), (3, 40, 1), (3, 40, 64))] + [
+    ((12, 10), (12, 1, 64)), ((60, 2), (60, 1, 64)), ((60, 2), (60, 1, 1))])
+@pytest.mark.parametrize("branch", [torch.float32, None])
+def test_gradient_of_a_16_bit_gate_is_rounded_once(moe_pkg, dtype, rows, shape, branch):
+    """d gate = sum of dy act'(g) n over what the gate stands for.  Its terms cancel to a small rest, which
+    the rounding of single terms (2^-9 or 2^-12 of each) would bury; a sum of n float32 terms is off by
+    at most (n + 64) 2^-24 of their magnitudes, the result by half a step of its type."""
+    g = torch.Generator().manual_seed(5)
+    (B, S), d = rows, 64
+    kind = branch or dtype
+    x, u = torch.randn(B, S, d, generator=g).to(kind), (torch.rand(B, S, d, generator=g) + 0.5).to(kind)
+    dy = torch.randn(B, S, d, generator=g).sign() * (torch.rand(B, S, d, generator=g) + 0.5)
+    dy = (dy - (dy * u.float()).mean() / (u.float() ** 2).mean() * u.float()).to(kind)
+    gate = torch.randn(shape, generator=g).to(dtype)
+    leaf = gate.to(DEV).requires_grad_(True)
+    y, _ = moe_pkg.residual_norm(x.to(DEV), u.to(DEV), gate=leaf, gate_activation="sigmoid")
+    (got,) = torch.autograd.grad(y, leaf, dy.to(DEV))
+    assert got.dtype == dtype and got.shape == gate.shape
+    want_leaf = gate.double().requires_grad_(True)
+    want_y, _ = ref.norm(x.double(), u.double(), None, want_leaf, "sigmoid")
+    (want,) = torch.autograd.grad(want_y, want_leaf, dy.double())
+    s = torch.sigmoid(gate.double())
+    terms = (dy.double() * u.double() * s * (1 - s)).abs()
+    while terms.ndim > gate.ndim:
+        terms = terms.sum(0)
+    for i, size in enumerate(gate.shape):
+        terms = terms.sum(i, keepdim=True) if size == 1 else terms
+    n = B * S * d // max(1, gate.numel())
+    tol = (n + 64) * 2.0 ** -24 * terms + torch.finfo(dtype).eps / 2 * want.abs() + 2.0 ** -25
+    assert ((got.cpu().double() - want).abs() <= tol).all(), float(((got.cpu().double() - want).abs() / tol).max())
