@@ -479,10 +479,9 @@ class SparseMoE(nn.Module):
             if vmask.numel() != T:
                 raise ValueError("valid must have one entry per token")
         if T == 0:
-            zero = torch.zeros((), dtype=torch.float32, device=dev)
+            out, aux, z = _EmptyBatchFunction.apply(x, *self.parameters())
             self.last_selected_mask = torch.zeros((*x.shape[:-1], E), dtype=torch.float32, device=dev)
-            return dict(out=torch.zeros_like(x), aux_loss=zero, router_z_loss=zero,
-                        counts=torch.zeros(E, dtype=torch.float32, device=dev))
+            return dict(out=out, aux_loss=aux, router_z_loss=z, counts=torch.zeros(E, dtype=torch.float32, device=dev))
         xb = flat.to(torch.bfloat16).contiguous()
         bias = self._logit_bias(dev, E)
         with torch.autocast(device_type=dev.type, enabled=False):
@@ -793,6 +792,21 @@ def _expert_parameter_grads(mod, d_y, d_up, h_save, x_rows, pad_start, shape, ne
     g_up = [dw_up[i].to(ups[i].dtype) if needed[i] else None for i in range(n_exp)]
     g_dn = [dw_dn[i].to(dns[i].dtype) if needed[n_exp + i] else None for i in range(n_exp)]
     return g_up, g_dn
+
+
+class _EmptyBatchFunction(torch.autograd.Function):
+    """The layer without a token: an empty output and zero losses whose gradients are zeros, so that a
+    backward over them runs as for any batch."""
+
+    @staticmethod
+    def forward(ctx, x, *parameters):
+        ctx.save_for_backward(x, *parameters)
+        return torch.zeros_like(x), *(torch.zeros((), dtype=torch.float32, device=x.device) for _ in range(2))
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, *_):
+        return tuple(torch.zeros_like(t) if need else None for t, need in zip(ctx.saved_tensors, ctx.needs_input_grad))
 
 
 class _RouterLogitsFunction(torch.autograd.Function):

@@ -337,3 +337,21 @@ def test_gradient_of_a_16_bit_gate_is_rounded_once(moe_pkg, dtype, rows, shape, 
     n = B * S * d // max(1, gate.numel())
     tol = (n + 64) * 2.0 ** -24 * terms + torch.finfo(dtype).eps / 2 * want.abs() + 2.0 ** -25
     assert ((got.cpu().double() - want).abs() <= tol).all(), float(((got.cpu().double() - want).abs() / tol).max())
+
+
+# ------------------------------------------------------------------ no tokens
+@pytest.mark.parametrize("kw", [dict(), SCORED, dict(SCORED, expert_groups=4, top_expert_groups=2)])
+@pytest.mark.parametrize("block", [False, True])
+def test_training_step_without_tokens(moe_pkg, kw, block):
+    torch.manual_seed(0)
+    cfg = moe_pkg.MoEConfig(d_model=256, expert_hidden_dim=256, num_experts=8, top_k=2, **kw)
+    layer = (moe_pkg.SparseMoEBlock if block else moe_pkg.SparseMoE)(cfg).to(DEV)
+    x = torch.empty(2, 0, 256, dtype=torch.bfloat16, device=DEV).requires_grad_(True)
+    out, aux, z, load = layer(x)
+    assert out.shape == x.shape and float(aux.detach()) == float(z.detach()) == 0.0 and not load.any()
+    (out.float().sum() + aux + z).backward()
+    assert x.grad.shape == x.shape
+    for n, p in layer.named_parameters():
+        assert p.grad is not None and not p.grad.any(), n
+    with torch.no_grad():
+        assert layer(x)[0].shape == x.shape
