@@ -267,7 +267,9 @@ __device__ __noinline__ void select_exact(const ScoreArgs& a, int64_t t, ScoreSc
     const float lf = load_logit(row + e);
     const double l = double(lf), x = exp(a.score == kSigmoid ? -l : l - top);
     const double score = (a.score == kSigmoid ? 1.0 : x) / (a.score == kSigmoid ? 1.0 + x : z);
-    const double v = lf == minus_inf() ? none : a.bias != nullptr ? score + double(__ldg(a.bias + e)) : score;
+    const float b = a.bias != nullptr ? __ldg(a.bias + e) : 0.f;
+    // masked by its logit or by its bias, which a NaN score would swallow
+    const double v = lf == minus_inf() || b == minus_inf() ? none : score + double(b);
     const double key = a.bias != nullptr ? v : l;
     s.val[e] = sums ? v : key;
     s.ord[e] = key == none ? 0 : ordered(key);

@@ -78,6 +78,21 @@ def test_a_spoilt_softmax_has_nan_weights(moe_pkg, spoil, kw):
             assert torch.isfinite(w[[0, 2, 4]]).all()
 
 
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("E", [2, 24, 64, 300])
+@pytest.mark.parametrize("groups", [1, 2])
+def test_a_masked_expert_stays_masked_in_a_row_of_nan(moe_pkg, score, E, groups):
+    logits = _rows(6, E, E)
+    logits[0] = float("nan")
+    logits[2, E // 2] = float("nan")
+    logits[3, 0] = float("inf")
+    logits[4, E - 1] = float("-inf")
+    bias = torch.linspace(-0.1, 0.1, E, device=DEV)
+    bias[1::3] = float("-inf")
+    for kw in (dict(), dict(renormalize=False)):
+        _ids(moe_pkg, logits, min(8, E // groups), score=score, bias=bias, num_groups=groups, top_groups=1, **kw)
+
+
 @pytest.mark.parametrize("kw", [dict(score_function="sigmoid", balance_bias=True), dict(balance_bias=True)])
 @pytest.mark.parametrize("T", [40, 1500])
 def test_a_nan_token_leaves_the_other_tokens(moe_pkg, kw, T):
