@@ -544,10 +544,12 @@ int mcl4moe_copy_list_async(void* const* dst, const void* const* src, const uint
  * [T, E] (dtype 0 bf16, 1 fp32, 2 fp16; row stride ld elements), keys s + bias
  * (bias fp32 [E] or NULL; it selects only), and, with groups > 1, only the
  * top_groups groups (of E / groups consecutive experts) of the largest value: the
- * sum of the two best keys (group_score 0) or the best key (1).  topk_idx int32
+ * sum of the two best keys (group_score 0; a group with one unmasked expert counts
+ * that one) or the best key (1).  topk_idx int32
  * [T, k]: the k best keys in falling order, ties to the lower id; an expert whose
  * logit or bias is -inf is never chosen, slots without an expert are -1 with
- * weight 0, and so are the rows where valid (uint8 [T] or NULL) is 0.  topk_w
+ * weight 0, and so are the rows where valid (uint8 [T] or NULL) is 0.  NaN ranks
+ * first and makes the row's weights NaN, with softmax so does +inf.  topk_w
  * fp32 [T, k] = scale * s / (sum of the chosen s when renorm).  counts (int32 [E]
  * or NULL): slots of each expert.  E <= 512, k <= 32.
  * _backward: d_logits [T, E] (dtype of the logits, contiguous) for d_w fp32 [T, k].

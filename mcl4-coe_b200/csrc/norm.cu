@@ -47,6 +47,7 @@ __device__ __forceinline__ void store_f(void* p, int dtype, int64_t i, float v) 
   else static_cast<__half*>(p)[i] = __float2half_rn(v);
 }
 
+// The sigmoid's quotient is approximate (2 ulp): half a bf16 step is 2^15 times that.
 __device__ __forceinline__ float act_of(float g, int act) {
   return act == kActSigmoid ? __fdividef(1.f, 1.f + expf(-g)) : act == kActTanh ? tanhf(g) : g;
 }
@@ -962,10 +963,11 @@ constexpr int kAheadBytes = 200 * 1024;  // of an SM's shared memory
 constexpr int kTeamSmem = 224 * 1024;    // of a CTA: one float32 row of 8192 with an element-wise gate and the factors
 
 // 16 columns a thread: needed from 2049 columns on; from 1025 on where a row has more operands or
-// wider ones, so that the reductions weigh more than the warps in flight (32768 x 2048, forward /
-// backward in us, 8 against 16 columns a thread: bf16 96 / 161 against 103 / 168; float32 stream 149 / 232
-// against 138 / 215; element-wise gate 134 / 285 against 117 / 232). Single elements stay narrow
-// (32768 x 1001: 90 / 254 against 114 / 293).
+// wider ones, or a third reduction (a token gate's gradient), which then weigh more than the warps in
+// flight.  32768 x 2048, forward / backward in us, 8 against 16 columns a thread: bf16 97 / 162 against
+// 103 / 168; token gate 97 / 245 against 88 / 191; element-wise gate 120 / 261 against 120 / 208; float32
+// stream 149 / 234 against 138 / 215.  Single elements stay narrow: 32768 x 1501 with a float32 stream
+// 135 / 334 against 169 / 521, 32768 x 2047 bf16 204 / 456 against 206 / 730.
 bool norm_wide(const NormArgs& a) {
   if (a.cols > 2048 || a.cols <= 1024) return a.cols > 2048;
   return norm_vectors(a) && (a.x_dtype == 1 || a.gate_mode >= kGateRow);

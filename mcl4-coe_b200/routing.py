@@ -131,11 +131,13 @@ def route_experts(logits: Tensor, top_k: int, *, score: str = "softmax", bias: T
     int32 ``[E]`` slots of each expert.  ``bias`` (``[E]``) is added to the scores for
     the selection alone and gets no gradient.  With ``num_groups`` > 1 (groups of
     consecutive experts) only the ``top_groups`` groups with the best value are
-    searched: the sum of a group's two best keys (``"top2"``) or its best (``"max"``).
+    searched: the sum of a group's two best keys (``"top2"``; a group with one unmasked
+    expert counts that one) or its best (``"max"``).
 
     An expert whose logit or bias is ``-inf`` is masked: never chosen, and a row that
     runs out of experts has id -1 and weight 0 in its last slots, as have rows whose
-    ``valid`` (``[..]``) is false.  NaN ranks first and makes its row's weights NaN.
+    ``valid`` (``[..]``) is false.  NaN ranks first and makes its row's weights NaN; so
+    does +inf under a softmax.
     ids follow exact arithmetic on the given logits (near ties are decided in float64).
     The gradient reaches the logits through the weights; differentiable once, in reverse mode.
     """
