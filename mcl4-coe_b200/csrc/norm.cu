@@ -1045,7 +1045,9 @@ int mcl4moe_residual_norm(const mcl4moe_norm_args* a, mcl4moe_stream_t stream) {
 }
 
 size_t mcl4moe_residual_norm_workspace_size(int64_t rows, int cols, int gate_mode, int64_t gate_rows) {
-  if (rows <= 0 || cols <= 0 || cols > kMaxNormCols || (gate_mode == kGateChannel && gate_rows <= 0)) return 0;
+  if (rows <= 0 || cols <= 0 || cols > kMaxNormCols ||
+      (gate_mode == kGateChannel && (gate_rows <= 0 || rows % gate_rows != 0)))
+    return 0;
   int64_t teams = 0, groups = 0;  // of either width of the teams
   for (int wide = cols > 2048; wide < 2; ++wide) {
     const NormShape s = norm_shape(rows, cols, gate_mode, gate_rows, true, wide != 0);

@@ -2,6 +2,7 @@
 without a GPU."""
 
 import os
+import subprocess
 import sys
 from pathlib import Path
 
@@ -179,3 +180,19 @@ def test_enable_cuda_graph_says_where_it_does_nothing(moe_pkg, recwarn):
     assert not recwarn.list
     with pytest.warns(UserWarning, match="routes from scores"):
         _layer(moe_pkg, score_function="sigmoid").enable_cuda_graph()
+
+
+def _in_a_process(code):
+    """What ``code`` prints with the library as ``lib``; a signal that ends the process shows."""
+    run = subprocess.run([sys.executable, "-c", "from __graft_entry__ import load_package\npkg = load_package()\n"
+                          "lib = pkg.library()\n" + code], cwd=HERE.parent, capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0, (run.returncode, run.stderr[-500:])
+    return run.stdout.split()
+
+
+def test_norm_workspace_of_gates_that_do_not_fit(moe_pkg):
+    """Gate rows that do not divide the rows, as many as there are and more: the call that would use them
+    is refused, and so there is no workspace."""
+    got = _in_a_process("for rows in (3, 9, 10, 11, 20, 1 << 40):\n"
+                        "    print(lib.mcl4moe_residual_norm_workspace_size(10, 64, 1, rows))")
+    assert [int(n) > 0 for n in got] == [False, False, True, False, False, False]
