@@ -643,6 +643,7 @@ extern "C" int mcl4moe_adamw_step(const mcl4moe_adamw_args* a, mcl4moe_stream_t 
     return MCL4MOE_ERR_INVALID;
   for (int i = 0; i < a->n; ++i) {
     if (a->numels[i] < 0) return MCL4MOE_ERR_INVALID;
+    if (a->numels[i] > (int64_t(1) << 42)) return MCL4MOE_ERR_UNSUPPORTED;  // more turns than a grid has, at any size
     if (a->numels[i] > 0 && (!a->params[i] || !a->grads[i] || !a->exp_avgs[i] || !a->exp_avg_sqs[i] ||
                              (a->bits == 8 && (!a->exp_avg_scales[i] || !a->exp_avg_sq_scales[i])) ||
                              (a->masters && !a->masters[i])))

@@ -672,7 +672,7 @@ __global__ void __launch_bounds__(kScoreWarps * 32) route_scores_bwd_kernel(Scor
 
 int check_scores(int64_t T, int E, int k, int dtype, int score) {
   if (T < 0 || E <= 0 || k <= 0 || k > E || dtype < 0 || dtype > 2 || score < 0 || score > 1) return MCL4MOE_ERR_INVALID;
-  if (E > kMaxScoreExperts || k > kMaxTopK || T * k > kMaxRoutedSlots) return MCL4MOE_ERR_UNSUPPORTED;
+  if (E > kMaxScoreExperts || k > kMaxTopK || T > kMaxRoutedSlots / k) return MCL4MOE_ERR_UNSUPPORTED;
   return MCL4MOE_OK;
 }
 

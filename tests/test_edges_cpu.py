@@ -196,3 +196,30 @@ def test_norm_workspace_of_gates_that_do_not_fit(moe_pkg):
     got = _in_a_process("for rows in (3, 9, 10, 11, 20, 1 << 40):\n"
                         "    print(lib.mcl4moe_residual_norm_workspace_size(10, 64, 1, rows))")
     assert [int(n) > 0 for n in got] == [False, False, True, False, False, False]
+
+
+def test_sizes_whose_products_overflow_are_refused(moe_pkg):
+    """Counts of rows and elements near the end of 64 bits, with addresses that are never used."""
+    got = _in_a_process("""
+import ctypes
+from array import array
+L = pkg._lib
+at = 1 << 20
+for T in (1 << 62, (1 << 63) - 1, (1 << 30) + 1, 1 << 29):
+    for back in (False, True):
+        if back:
+            st = lib.mcl4moe_route_scores_backward(at, 1, 8, at, at, T, 8, 4, 0, 1, 1.0, at, None)
+        else:
+            st = lib.mcl4moe_route_scores(at, 1, 8, None, None, T, 8, 4, 0, 1, 1, 0, 1, 1.0, at, at, None, None)
+        print(st == L.ERR_UNSUPPORTED)
+pointers = array("Q", [at])
+p = pointers.buffer_info()[0]
+for n in ((1 << 63) - 1, (1 << 63) - 4000, 1 << 43):
+    for bits in (8, 32):
+        numels = array("q", [n])
+        a = L.AdamwArgs(n=1, param_dtype=1, grad_dtype=1, bits=bits, beta1=0.9, beta2=0.99, eps=1e-8, step=1, params=p,
+                        grads=p, exp_avgs=p, exp_avg_sqs=p, exp_avg_scales=p, exp_avg_sq_scales=p,
+                        numels=numels.buffer_info()[0])
+        print(lib.mcl4moe_adamw_step(ctypes.byref(a), None) == L.ERR_UNSUPPORTED)
+""")
+    assert got == ["True"] * 14
