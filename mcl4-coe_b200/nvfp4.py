@@ -358,10 +358,14 @@ def seed_grouped_cache(experts: nn.ModuleList, proj_name: str, filled: dict) -> 
 
 
 def invalidate_cache(experts: nn.ModuleList) -> None:
+    """Every expert is quantised again by the next call, whatever its weight's version says."""
     try:
         setattr(experts, CACHE_ATTR, None)
     except Exception:  # pragma: no cover
         pass
+    for expert in experts:  # or the next cache would carry their bytes over
+        for layer in expert.modules():
+            layer.__dict__.pop(SLOT_ATTR, None)
 
 
 @torch.no_grad()

@@ -223,3 +223,14 @@ for n in ((1 << 63) - 1, (1 << 63) - 4000, 1 << 43):
         print(lib.mcl4moe_adamw_step(ctypes.byref(a), None) == L.ERR_UNSUPPORTED)
 """)
     assert got == ["True"] * 14
+
+
+def test_invalidate_cache_leaves_no_bytes_to_carry_over(moe_pkg):
+    layer, nv = _layer(moe_pkg), moe_pkg.nvfp4
+    setattr(layer.experts, nv.CACHE_ATTR, {"up_proj": object()})
+    for e in layer.experts:
+        setattr(e.up_proj, nv.SLOT_ATTR, (object(), 0))
+        setattr(e.down_proj, nv.SLOT_ATTR, (object(), 0))
+    nv.invalidate_cache(layer.experts)
+    assert getattr(layer.experts, nv.CACHE_ATTR) is None
+    assert not any(hasattr(m, nv.SLOT_ATTR) for m in layer.modules())

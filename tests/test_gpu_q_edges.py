@@ -370,3 +370,18 @@ def test_training_step_without_tokens(moe_pkg, kw, block):
         assert p.grad is not None and not p.grad.any(), n
     with torch.no_grad():
         assert layer(x)[0].shape == x.shape
+
+
+# ------------------------------------------------------------------ the weights' NVFP4 copies
+@pytest.mark.parametrize("kw", [dict(), SCORED])
+def test_invalidated_cache_is_made_again(moe_pkg, kw):
+    """Weights that change without their version (a replayed optimizer step, ``.data``)."""
+    layer, x = _layer(moe_pkg, **kw), _rows(40, 256, 3, torch.bfloat16)
+    with torch.no_grad():
+        layer(x)
+        for p in layer.experts.parameters():
+            p.data.mul_(-1.5)
+        moe_pkg.nvfp4.invalidate_cache(layer.experts)
+        fresh = _layer(moe_pkg, **kw)
+        fresh.load_state_dict(layer.state_dict())
+        assert torch.equal(layer(x)[0], fresh(x)[0])
