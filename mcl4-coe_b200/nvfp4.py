@@ -227,9 +227,13 @@ def quantize_weight_slots(weights: list[Tensor], slots: list[int], cache: Groupe
 
 @torch.no_grad()
 def get_or_build_grouped_cache(experts: nn.ModuleList, proj_name: str, with_bwd: bool = False) -> GroupedNVFP4Cache:
-    """src/mcl4_coe/nvfp4.py:962-1048 on the B200 kernels (see module docstring)."""
+    """src/mcl4_coe/nvfp4.py:962-1048 on the B200 kernels (see module docstring).
+
+    A captured call whose cache is not current, and every captured training call, quantises
+    into a cache of its graph alone, in each replay: an update that a capture records has not
+    happened yet, and a captured optimizer step changes the weights between replays."""
     store = experts.__dict__.get(CACHE_ATTR)
-    if store:
+    if store and not (with_bwd and torch.cuda.is_current_stream_capturing()):
         entry = store.get(proj_name)
         if (entry is not None and (not with_bwd or entry.packed_t is not None)
                 and entry.still_current(experts, proj_name)):
@@ -256,6 +260,13 @@ def get_or_build_grouped_cache(experts: nn.ModuleList, proj_name: str, with_bwd:
         except Exception:  # pragma: no cover - ModuleList always accepts attributes
             pass
     entry = store.get(proj_name)
+    if torch.cuda.is_current_stream_capturing() and (with_bwd or entry is None or entry.versions != cur or
+                                                     entry.shape_key != (e_count, n, k, str(device))):
+        entry = GroupedNVFP4Cache(e_count, n, k, device)
+        if with_bwd:
+            entry.enable_transposed()
+        _quantize_dirty(entry, list(range(e_count)), weights, modes)
+        return entry
     if entry is None or entry.shape_key != (e_count, n, k, str(device)):
         entry = GroupedNVFP4Cache(e_count, n, k, device)
         if with_bwd:
@@ -268,8 +279,19 @@ def get_or_build_grouped_cache(experts: nn.ModuleList, proj_name: str, with_bwd:
         entry.remember_owners(experts, proj_name, layers, weights)
         return entry
     dirty = [i for i, (old, new) in enumerate(zip(entry.versions, cur)) if old != new]
+    _quantize_dirty(entry, dirty, weights, modes)
+    entry.versions = cur
+    for i in dirty:
+        setattr(layers[i], SLOT_ATTR, (entry, i))
+    entry.remember_owners(experts, proj_name, layers, weights)
+    return entry
+
+
+def _quantize_dirty(entry: GroupedNVFP4Cache, dirty: list[int], weights: list[Tensor], modes: list) -> None:
+    """The experts' weights into the slots ``dirty``; 2:4-sparse experts are masked before
+    (src/mcl4_coe/nvfp4.py:1017-1024)."""
     staged = []
-    for i in dirty:  # 2:4-sparse experts are masked before quantisation (src/mcl4_coe/nvfp4.py:1017-1024)
+    for i in dirty:
         if modes[i] == "none":
             entry.masks[i] = None
             staged.append(weights[i])
@@ -279,11 +301,6 @@ def get_or_build_grouped_cache(experts: nn.ModuleList, proj_name: str, with_bwd:
             staged.append(masked)
     quantize_weight_slots(staged, dirty, entry)
     CACHE_STATS["quantized"] += len(dirty)
-    entry.versions = cur
-    for i in dirty:
-        setattr(layers[i], SLOT_ATTR, (entry, i))
-    entry.remember_owners(experts, proj_name, layers, weights)
-    return entry
 
 
 def _carry_over(layers: list, cur: list, entry: GroupedNVFP4Cache) -> None:

@@ -385,3 +385,80 @@ def test_invalidated_cache_is_made_again(moe_pkg, kw):
         fresh = _layer(moe_pkg, **kw)
         fresh.load_state_dict(layer.state_dict())
         assert torch.equal(layer(x)[0], fresh(x)[0])
+
+
+# ------------------------------------------------------------------ captured calls and those copies
+def _side(fn):
+    """Runs ``fn`` on a side stream, as before a capture."""
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        result = fn()
+    torch.cuda.current_stream().wait_stream(side)
+    return result
+
+
+@pytest.mark.parametrize("kw", [dict(), SCORED])
+def test_capture_after_the_weights_changed(moe_pkg, kw):
+    """What a capture records has not run: an eager call behind it must not take its quantisation for done."""
+    layer, x = _layer(moe_pkg, **kw), _rows(60, 256, 3, torch.bfloat16)
+    static = x.clone()
+    with torch.no_grad():
+        old = layer(x)[0].clone()
+        _side(lambda: layer(static))
+        for p in layer.experts.parameters():
+            p.mul_(-1.5)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            captured = layer(static)[0]
+        eager = layer(x)[0].clone()
+        graph.replay()
+        fresh = _layer(moe_pkg, **kw)
+        fresh.load_state_dict(layer.state_dict())
+        want = fresh(x)[0]
+        assert torch.equal(eager, want) and torch.equal(captured, want) and not torch.equal(want, old)
+        for p in layer.experts.parameters():  # once more, behind the capture
+            p.mul_(2.0)
+        fresh.load_state_dict(layer.state_dict())
+        assert torch.equal(layer(x)[0], fresh(x)[0])
+
+
+@pytest.mark.parametrize("kw", [dict(), SCORED])
+@pytest.mark.parametrize("fresh_cache", [False, True])
+def test_captured_training_step(moe_pkg, kw, fresh_cache):
+    """Forward, gradients and optimizer step in one graph, replayed: the weights are those of eager steps
+    (the same seeds of the stochastic rounding)."""
+    import random
+
+    x = _rows(200, 256, 6, torch.bfloat16)
+
+    def make():
+        layer = _layer(moe_pkg, **kw)
+        return layer, list(layer.parameters()), moe_pkg.AdamW(layer.parameters(), lr=1e-2, capturable=True)
+
+    def step(layer, params, opt, inp):
+        random.seed(11)
+        out, aux, z, _ = layer(inp)
+        ones = [torch.ones_like(t) for t in (out, aux, z)]
+        for p, g in zip(params, torch.autograd.grad([out, aux, z], params, ones)):
+            p.grad = g
+        opt.step()
+
+    one, two = make(), make()
+    for _ in range(5):
+        step(*one, x)
+    static = x.clone()
+    _side(lambda: [step(*two, static) for _ in range(2)])
+    if fresh_cache:  # an eager forward between the last step and the capture
+        two[0](static)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(*two, static)
+    for _ in range(3):
+        two[0](_rows(333, 256, 9, torch.bfloat16))  # other calls between the replays
+        graph.replay()
+    for (n, p), q in zip(one[0].named_parameters(), two[1]):
+        assert torch.equal(p, q), n
+    moe_pkg.nvfp4.invalidate_cache(two[0].experts)
+    with torch.no_grad():
+        assert torch.equal(one[0](x)[0], two[0](x)[0])
