@@ -60,8 +60,8 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .norms import residual_norm
-from .nvfp4 import _stream_handle, get_or_build_grouped_cache, invalidate_cache, nvfp4_grouped_linear
-from .routing import GROUP_SCORES, SCORE_FUNCTIONS, _raw_stream, route_experts
+from .nvfp4 import _raw_stream, _stream_handle, get_or_build_grouped_cache, invalidate_cache, nvfp4_grouped_linear
+from .routing import GROUP_SCORES, SCORE_FUNCTIONS, route_experts
 
 RESIDUAL_GATES = ("none", "linear", "sigmoid", "tanh")
 

@@ -50,6 +50,11 @@ SLOT_ATTR = "_mcl4_b200_nvfp4_slot"
 CACHE_STATS = {"quantized": 0, "carried": 0}
 
 
+# The raw handle of a device's current stream; the public route builds a Stream object first.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _stream_handle() -> int:
     return torch.cuda.current_stream().cuda_stream
 
@@ -141,6 +146,25 @@ class GroupedNVFP4Cache:
         self.packed_t: Tensor | None = None
         self.scales_t: Tensor | None = None
         self._owners: tuple | None = None  # what ``versions`` was read from (see still_current)
+        self._written: tuple | None = None  # (event behind the kernels that wrote the bytes, their stream)
+
+    def bytes_written(self) -> None:
+        """Called behind the kernels that write the bytes."""
+        if self.packed.is_cuda and not torch.cuda.is_current_stream_capturing():  # a graph has its own order
+            event = torch.cuda.Event() if self._written is None else self._written[0]
+            event.record()
+            self._written = (event, _raw_stream(self.packed.device.index))
+
+    def await_bytes(self) -> None:
+        """Called before the bytes are used: another stream than the one that wrote them waits."""
+        written = self._written
+        if (written is not None and written[1] != _raw_stream(self.packed.device.index)
+                and not torch.cuda.is_current_stream_capturing()):
+            torch.cuda.current_stream(self.packed.device).wait_event(written[0])
+
+    def __getstate__(self) -> dict:  # copies and pickles: an event is neither
+        self.await_bytes()
+        return {**self.__dict__, "_written": None}
 
     def remember_owners(self, experts: nn.ModuleList, proj_name: str, layers: list, weights: list) -> None:
         """Record the module dicts, Parameters, versions and storages ``versions`` was read
@@ -237,6 +261,7 @@ def get_or_build_grouped_cache(experts: nn.ModuleList, proj_name: str, with_bwd:
         entry = store.get(proj_name)
         if (entry is not None and (not with_bwd or entry.packed_t is not None)
                 and entry.still_current(experts, proj_name)):
+            entry.await_bytes()
             return entry
     layers = [_submodule(e, proj_name) for e in experts]
     weights = [_weight(layer) for layer in layers]
@@ -277,6 +302,7 @@ def get_or_build_grouped_cache(experts: nn.ModuleList, proj_name: str, with_bwd:
         entry.enable_transposed()  # training starts: every expert also needs its transposed copy
     if entry.versions == cur:
         entry.remember_owners(experts, proj_name, layers, weights)
+        entry.await_bytes()
         return entry
     dirty = [i for i, (old, new) in enumerate(zip(entry.versions, cur)) if old != new]
     _quantize_dirty(entry, dirty, weights, modes)
@@ -299,7 +325,9 @@ def _quantize_dirty(entry: GroupedNVFP4Cache, dirty: list[int], weights: list[Te
             masked, mask = _mask_2to4(weights[i], modes[i])
             entry.masks[i] = mask.bool()
             staged.append(masked)
+    entry.await_bytes()
     quantize_weight_slots(staged, dirty, entry)
+    entry.bytes_written()
     CACHE_STATS["quantized"] += len(dirty)
 
 
@@ -322,6 +350,7 @@ def _carry_over(layers: list, cur: list, entry: GroupedNVFP4Cache) -> None:
         src_slots.setdefault(id(old), []).append((j, i))
     for key, pairs in src_slots.items():
         old = owners[key]
+        old.await_bytes()
         src = torch.tensor([j for j, _ in pairs], dtype=torch.long, device=entry.packed.device)
         dst = torch.tensor([i for _, i in pairs], dtype=torch.long, device=entry.packed.device)
         entry.packed.index_copy_(0, dst, old.packed.index_select(0, src))
@@ -335,6 +364,8 @@ def _carry_over(layers: list, cur: list, entry: GroupedNVFP4Cache) -> None:
             entry.versions[i] = cur[i]
             setattr(layers[i], SLOT_ATTR, (entry, i))
         CACHE_STATS["carried"] += len(pairs)
+    if src_slots:
+        entry.bytes_written()
 
 
 def _current_versions(layers: list, weights: list | None = None) -> list:
@@ -363,6 +394,7 @@ def seed_grouped_cache(experts: nn.ModuleList, proj_name: str, filled: dict) -> 
         store[proj_name] = entry
         _carry_over(layers, cur, entry)
     entry._owners = None  # versions change below
+    entry.await_bytes()
     for i, (packed, scales, g) in filled.items():
         entry.packed[i].copy_(packed.view(entry.packed[i].shape))
         entry.scales[i].copy_(scales.view(entry.scales[i].shape))
@@ -370,6 +402,7 @@ def seed_grouped_cache(experts: nn.ModuleList, proj_name: str, filled: dict) -> 
         entry.masks[i] = None
         entry.versions[i] = cur[i]
         setattr(layers[i], SLOT_ATTR, (entry, i))
+    entry.bytes_written()
     CACHE_STATS["carried"] += len(filled)
     return entry
 

@@ -14,17 +14,12 @@ from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .nvfp4 import _ptr, _require_cuda
+from .nvfp4 import _ptr, _raw_stream, _require_cuda
 
 DTYPE_CODES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}
 SCORE_FUNCTIONS = ("softmax", "sigmoid")
 GROUP_SCORES = ("top2", "max")
 MAX_EXPERTS, MAX_TOP_K = 512, 32
-
-
-# The raw handle of a device's current stream; the public route builds a Stream object first.
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
-    lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _launch(device: torch.device, what: str, fn, *args) -> None:

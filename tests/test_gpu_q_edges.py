@@ -462,3 +462,39 @@ def test_captured_training_step(moe_pkg, kw, fresh_cache):
     moe_pkg.nvfp4.invalidate_cache(two[0].experts)
     with torch.no_grad():
         assert torch.equal(one[0](x)[0], two[0](x)[0])
+
+
+@pytest.mark.parametrize("kw", [dict(), SCORED])
+def test_first_calls_on_two_streams(moe_pkg, kw):
+    """One call quantises the weights, the other takes what it wrote without a word from the user."""
+    torch.manual_seed(0)
+    cfg = moe_pkg.MoEConfig(d_model=2048, expert_hidden_dim=1024, num_experts=16, top_k=2, **kw)
+    layer = moe_pkg.SparseMoE(cfg).to(DEV)
+    x = _rows(64, 2048, 3, torch.bfloat16)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    with torch.no_grad():
+        for scale in (1.0, -0.5, 2.0):
+            for p in layer.experts.parameters():
+                p.mul_(scale)
+            moe_pkg.nvfp4.invalidate_cache(layer.experts)
+            torch.cuda.synchronize()
+            got = []
+            for s in streams:
+                with torch.cuda.stream(s):
+                    got.append(layer(x)[0])
+            torch.cuda.synchronize()
+            want = layer(x)[0]
+            assert all(torch.equal(want, g) for g in got)
+
+
+def test_a_layer_with_its_cache_can_be_copied(moe_pkg):
+    import copy
+
+    layer, x = _layer(moe_pkg, **SCORED), _rows(64, 256, 3, torch.bfloat16)
+    with torch.no_grad():
+        want = layer(x)[0]
+        other = copy.deepcopy(layer)
+        assert torch.equal(other(x)[0], want)
+        for p in other.experts.parameters():
+            p.mul_(2.0)
+        assert not torch.equal(other(x)[0], want) and torch.equal(layer(x)[0], want)
