@@ -575,7 +575,8 @@ int mcl4moe_route_scores_backward(const void* logits, int dtype, int64_t ld, con
  * stats (fp32 [rows, 2] or NULL) receives the two reciprocal root mean squares.
  * _backward reads stats (needed with post_weight or d_normed); d_stream / d_normed
  * are the gradients of y and h (either may be NULL: zero); outputs that are NULL are not computed; d_pre, d_post and the
- * gate's gradient of modes 1 and 2 are fp32, that of mode 3 has the gate's type.
+ * gate's gradient of modes 1 and 2 are fp32, that of mode 3 has the gate's type, or is
+ * fp32 with gate_grad_f32 (a caller that adds it up over rows).
  * The sums over rows are taken in a fixed order.  cols <= 16384.
  * ------------------------------------------------------------------------ */
 typedef struct mcl4moe_norm_args {
@@ -612,6 +613,7 @@ typedef struct mcl4moe_norm_args {
   void* d_gate;
   float* d_pre;
   float* d_post;
+  int gate_grad_f32;
 } mcl4moe_norm_args;
 
 int mcl4moe_residual_norm(const mcl4moe_norm_args* args, mcl4moe_stream_t stream);

@@ -147,6 +147,7 @@ class NormArgs(ctypes.Structure):
         ("stream_out", c_void_p), ("norm_out", c_void_p), ("stats", c_void_p),
         ("d_stream", c_void_p), ("ld_d_stream", c_int64), ("d_normed", c_void_p), ("ld_d_normed", c_int64),
         ("d_x", c_void_p), ("d_branch", c_void_p), ("d_gate", c_void_p), ("d_pre", c_void_p), ("d_post", c_void_p),
+        ("gate_grad_f32", c_int),
     ]
 
 

@@ -206,8 +206,16 @@ __device__ __forceinline__ void store8(T* row, const V8& v, int chunk, int tid, 
     }
   } else if constexpr (LAY == kEights) {
     const int c = col_of<kEights>(chunk, 0, tid, team);
-    if (c < cols)
+    if (c >= cols) return;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint2 lo = *reinterpret_cast<const uint2*>(&v.p[2 * h]), hi = *reinterpret_cast<const uint2*>(&v.p[2 * h + 1]);
+        *reinterpret_cast<uint4*>(row + c + 4 * h) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+      }
+    } else {
       *reinterpret_cast<uint4*>(row + c) = make_uint4(pack2<T>(v.p[0]), pack2<T>(v.p[1]), pack2<T>(v.p[2]), pack2<T>(v.p[3]));
+    }
   } else {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -542,8 +550,10 @@ __global__ void __launch_bounds__(NCH == 1 ? 256 : 512, NCH == 1 ? 3 : 1)
 
 // The columns' factors lie in shared memory behind the rows ahead, each thread's its own, so that
 // the registers hold two column sums and the row (three values a column) alone: 3 CTAs of 256
-// threads an SM instead of 2, and no spills with 16 columns a thread.
-template <typename TX, typename TU, int NCH, int LAY, bool GATED>
+// threads an SM instead of 2, and no spills with 16 columns a thread.  TG: type of an element-wise
+// gate's gradient, float for a caller that adds it up over rows (in one kernel with both types the
+// token gates' gradient with a float32 stream took 245 us for 236).
+template <typename TX, typename TU, int NCH, int LAY, bool GATED, typename TG>
 __global__ void __launch_bounds__(NCH == 1 ? 256 : 512, NCH == 1 ? kBwdCtas : 1)
     residual_norm_team_bwd_kernel(const NormArgs a, const TeamPlan plan, float* partial) {
   extern __shared__ __align__(16) char smem[];
@@ -667,9 +677,10 @@ __global__ void __launch_bounds__(NCH == 1 ? 256 : 512, NCH == 1 ? kBwdCtas : 1)
     for (int j = 0; j < NCH; ++j) {
       const V8 zu = mul(z[j], uh[j]);
       if (by_row) dot_g += dot8(ahead.kept(2 * j), zu);
-      if (full && a.d_gate != nullptr)
-        store8<TU, LAY>(row_at(static_cast<TU*>(a.d_gate), r, out_u), mul(mul(ahead.kept(2 * j), zu), slope8(act[j], a.gate_act)), j, tid,
-                        team, cols);
+      if (full && a.d_gate != nullptr) {
+        const V8 g = mul(mul(ahead.kept(2 * j), zu), slope8(act[j], a.gate_act));
+        store8<TG, LAY>(row_at(static_cast<TG*>(a.d_gate), r, uint32_t(cols * sizeof(TG))), g, j, tid, team, cols);
+      }
       acc_s[j] = full ? fma(act[j], zu, acc_s[j]) : by_row ? fma(zu, a1, acc_s[j]) : add(zu, acc_s[j]);
       z[j] = mul(factor(j), z[j]);
       if (post) dot_u += dot8(z[j], uh[j]);
@@ -794,7 +805,7 @@ __global__ void __launch_bounds__(kNormThreads) residual_norm_bwd_kernel(const N
       dot_u += g * kzu;
       dot_g += kzu * act_slope(g, a.gate_act);
       if (a.gate_mode == kGateFull && a.d_gate != nullptr)
-        store_f(a.d_gate, a.gate_dtype, r * a.cols + c, kzu * act_slope(g, a.gate_act));
+        store_f(a.d_gate, a.gate_grad_f32 ? 1 : a.gate_dtype, r * a.cols + c, kzu * act_slope(g, a.gate_act));
     }
     if (a.branch == nullptr) continue;
     if (a.gate_mode == kGateRow) {
@@ -984,10 +995,15 @@ int launch_team(const NormArgs& a, NormShape s, bool backward, float* partial, c
   s.plan.depth = LAY != kSingles ? depth : 0;
   const unsigned grid = unsigned((s.plan.teams + s.rows_per_cta - 1) / s.rows_per_cta);
   if (backward) {
-    static std::atomic<uint64_t> raised{0};
-    if (!raise_smem_limit(residual_norm_team_bwd_kernel<TX, TU, NCH, LAY, GATED>, kTeamSmem, raised))
-      return MCL4MOE_ERR_CUDA;
-    residual_norm_team_bwd_kernel<TX, TU, NCH, LAY, GATED><<<grid, s.threads, smem, stream>>>(a, s.plan, partial);
+    const auto launch = [&](auto kernel, std::atomic<uint64_t>& raised) {
+      if (!raise_smem_limit(kernel, kTeamSmem, raised)) return MCL4MOE_ERR_CUDA;
+      kernel<<<grid, s.threads, smem, stream>>>(a, s.plan, partial);
+      return MCL4MOE_OK;
+    };
+    static std::atomic<uint64_t> raised{0}, raised_f32{0};
+    if constexpr (GATED && sizeof(TU) == 2)
+      if (a.gate_grad_f32) return launch(residual_norm_team_bwd_kernel<TX, TU, NCH, LAY, GATED, float>, raised_f32);
+    return launch(residual_norm_team_bwd_kernel<TX, TU, NCH, LAY, GATED, TU>, raised);
   } else {
     static std::atomic<uint64_t> raised{0};
     if (LAY != kSingles && !raise_smem_limit(residual_norm_team_kernel<TX, TU, NCH, LAY, GATED>, kTeamSmem, raised))

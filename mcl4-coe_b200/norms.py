@@ -17,41 +17,43 @@ GATE_ACTIVATIONS = ("none", "sigmoid", "tanh")
 MAX_COLS = 16384
 _NONE, _CHANNEL, _ROW, _FULL = range(4)
 # Rows from which a gate shared by consecutive rows is summed inside the kernel (one partial
-# row of column sums per group); smaller groups are written out as one gate row per row, unless a
-# 16-bit gate's gradient would be rounded for each row then.
+# row of column sums per group); smaller groups are written out as one gate row per row.
 _MIN_GROUP_ROWS = 32
 _MAX_GROUPS = 65533
 
 
-def _gate_form(gate: Tensor, x: Tensor) -> tuple[Tensor, int, int]:
-    """(gate, mode, rows that share a gate row) for a gate that broadcasts to ``x``.  A 16-bit gate's gradient
-    is rounded when its rows are added up, not before: where they are added here and not in the kernel, the
-    gate goes in as float32 (element-wise then through the kernels of mixed types)."""
+def _gate_form(gate: Tensor, x: Tensor) -> tuple[Tensor, int, int, torch.Size | None]:
+    """(gate, mode, rows that share a gate row, None) for a gate that broadcasts to ``x``.  A 16-bit gate's
+    gradient is rounded where its rows are added up, not before: a gate of single values goes in as float32,
+    one that has to be written out a row each stays as it is, with ``x``'s shape in the last place, for the
+    autograd function to do that and to add up the rows of a float32 gradient."""
     if gate.ndim == 1 and gate.shape[0] == x.shape[-1]:
-        return gate.contiguous().view(1, -1), _CHANNEL, max(1, x.numel() // x.shape[-1])
+        return gate.contiguous().view(1, -1), _CHANNEL, max(1, x.numel() // x.shape[-1]), None
     if gate.ndim > x.ndim or any(g != 1 and g != s for g, s in zip(gate.shape[::-1], x.shape[::-1])):
         raise ValueError(f"gate {tuple(gate.shape)} does not broadcast to {tuple(x.shape)}")
     gate = gate.reshape((1,) * (x.ndim - gate.ndim) + tuple(gate.shape))
     lead, x_lead, d = gate.shape[:-1], x.shape[:-1], x.shape[-1]
     rows = x.numel() // max(1, d)
     if lead == x_lead and gate.shape[-1] == d and rows > 1:
-        return _rows(gate), _FULL, 1
+        return _rows(gate), _FULL, 1, None
     summed = gate.dtype != torch.float32 and gate.requires_grad and torch.is_grad_enabled()
     if gate.shape[-1] == 1 and d > 1:
         if summed and gate.numel() != rows:
             gate = gate.float()
-        return gate.expand(*x_lead, 1).reshape(rows).contiguous(), _ROW, 1
+        return gate.expand(*x_lead, 1).reshape(rows).contiguous(), _ROW, 1, None
     cut = max((i + 1 for i, s in enumerate(lead) if s != 1), default=0)
     groups = 1
     for s in lead[:cut]:
         groups *= s
     if lead[:cut] == x_lead[:cut]:
         share = max(1, rows // max(1, groups))
-        if groups == 1 or ((share >= _MIN_GROUP_ROWS or summed) and 0 < groups <= _MAX_GROUPS):
-            return gate.reshape(groups, d).contiguous(), _CHANNEL, share
-    if summed:
-        gate = gate.float()
-    return gate.expand(x.shape).reshape(rows, d).contiguous(), _FULL, 1
+        if groups == 1 or (share >= _MIN_GROUP_ROWS and groups <= _MAX_GROUPS):
+            return gate.reshape(groups, d).contiguous(), _CHANNEL, share, None
+    return (gate, _FULL, 1, x.shape) if summed else (_spread(gate, x.shape), _FULL, 1, None)
+
+
+def _spread(gate: Tensor, shape: torch.Size) -> Tensor:
+    return gate.expand(shape).reshape(-1, shape[-1]).contiguous()
 
 
 def _fill(args, x, branch, post, pre, gate, mode, gate_rows, act, norm_dtype, scales):
@@ -84,7 +86,11 @@ class _ResidualNorm(torch.autograd.Function):
     """Saves the inputs and the rows' two reciprocal root mean squares; the backward computes the rest again."""
 
     @staticmethod
-    def forward(ctx, x, branch, post, pre, gate, form):
+    def forward(ctx, x, branch, post, pre, gate, form, gate_shape):
+        ctx.gate_of = None if gate_shape is None else gate.shape  # what the gradient's rows are added up to
+        ctx.x_shape = gate_shape
+        if gate_shape is not None:
+            gate = _spread(gate, gate_shape)
         stats = x.new_empty((x.shape[0], 2), dtype=torch.float32)
         y, h = _norm_forward(x, branch, post, pre, gate, *form, stats)
         ctx.save_for_backward(x, branch, post, pre, gate, stats)
@@ -106,13 +112,13 @@ class _ResidualNorm(torch.autograd.Function):
     @staticmethod
     def _gradients(ctx, d_y, d_h):
         if d_y is None and d_h is None:
-            return (None,) * 6
+            return (None,) * 7
         x, branch, post, pre, gate, stats = ctx.saved_tensors
         mode = ctx.form[0]
         need = ctx.needs_input_grad
         if x.shape[0] == 0:
-            return tuple(torch.zeros_like(t) if n and t is not None else None
-                         for n, t in zip(need, (x, branch, post, pre, gate))) + (None,)
+            like = (x, branch, post, pre, gate if ctx.gate_of is None else gate.new_empty(ctx.gate_of))
+            return tuple(torch.zeros_like(t) if n and t is not None else None for n, t in zip(need, like)) + (None, None)
         lib = _lib.load()
         dev = x.device
         args = _fill(_lib.NormArgs(), x, branch, post, pre, gate, *ctx.form)
@@ -136,15 +142,18 @@ class _ResidualNorm(torch.autograd.Function):
         d_branch = out(need[1], branch, "d_branch")
         d_post = out(need[2], post, "d_post")
         d_pre = out(need[3], pre, "d_pre")
-        d_gate = out(need[4], gate, "d_gate", None if mode == _FULL else torch.float32)
+        args.gate_grad_f32 = int(ctx.gate_of is not None)
+        d_gate = out(need[4], gate, "d_gate", None if mode == _FULL and ctx.gate_of is None else torch.float32)
         ws, nbytes = None, 0
         if d_post is not None or d_pre is not None or (d_gate is not None and mode == _CHANNEL):
             nbytes = lib.mcl4moe_residual_norm_workspace_size(args.rows, args.cols, args.gate_mode, args.gate_rows)
             ws = x.new_empty((nbytes,), dtype=torch.uint8)
         _launch(dev, "mcl4moe_residual_norm_backward", lib.mcl4moe_residual_norm_backward, args, _ptr(ws), nbytes)
+        if d_gate is not None and ctx.gate_of is not None:
+            d_gate = d_gate.view(ctx.x_shape).sum_to_size(ctx.gate_of)
         if d_gate is not None and d_gate.dtype != gate.dtype:
             d_gate = d_gate.to(gate.dtype)
-        return d_x, d_branch, d_post, d_pre, d_gate, None
+        return d_x, d_branch, d_post, d_pre, d_gate, None, None
 
 
 def residual_norm(x: Tensor, branch: Tensor | None = None, *, post_weight: Tensor | None = None,
@@ -189,16 +198,16 @@ def residual_norm(x: Tensor, branch: Tensor | None = None, *, post_weight: Tenso
         norm_dtype = x.dtype if branch is None else branch.dtype
     elif norm_dtype not in DTYPE_CODES:
         raise ValueError(f"norm_dtype must be bf16, fp16 or fp32, got {norm_dtype}")
-    mode, gate_rows, gate_2d = _NONE, 0, None
+    mode, gate_rows, gate_2d, gate_shape = _NONE, 0, None, None
     if gate is not None:
-        gate_2d, mode, gate_rows = _gate_form(gate, x)
+        gate_2d, mode, gate_rows, gate_shape = _gate_form(gate, x)
     _refuse_tangents("residual_norm", x, branch, post_weight, pre_weight, gate)
     _require_cuda(x, "residual_norm")
     tensors = (_rows(x), None if branch is None else _rows(branch), _f32(post_weight), _f32(pre_weight), gate_2d)
     form = (mode, gate_rows, GATE_ACTIVATIONS.index(gate_activation), norm_dtype,
             (float(residual_scale), float(branch_scale), float(eps)))
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        y, h = _ResidualNorm.apply(*tensors, form)
+        y, h = _ResidualNorm.apply(*tensors, form, gate_shape)
     else:
         y, h = _norm_forward(*tensors, *form)
     if x.ndim != 2:

@@ -327,7 +327,7 @@ def test_scored_layer_grows_and_prunes(moe_pkg):
 @pytest.mark.parametrize("branch", [torch.float32, None])
 def test_gradient_of_a_16_bit_gate_is_rounded_once(moe_pkg, dtype, rows, shape, branch):
     """d gate = sum of dy act'(g) n over what the gate stands for.  Its terms cancel to a small rest, which
-    the rounding of single terms (2^-9 or 2^-12 of each) would bury; a sum of n float32 terms is off by
+    the rounding of single terms (2^-8 or 2^-11 of each) would bury; a sum of n float32 terms is off by
     at most (n + 64) 2^-24 of their magnitudes, the result by half a step of its type."""
     g = torch.Generator().manual_seed(5)
     (B, S), d = rows, 64
@@ -498,3 +498,24 @@ def test_a_layer_with_its_cache_can_be_copied(moe_pkg):
         for p in other.experts.parameters():
             p.mul_(2.0)
         assert not torch.equal(other(x)[0], want) and torch.equal(layer(x)[0], want)
+
+
+def test_broadcast_16_bit_gates_of_nothing_and_of_mixed_types(moe_pkg):
+    """No rows; a bf16 gate on an fp16 stream and a float32 branch (the kernels of mixed types)."""
+    for rows, shape in (((0, 5), (1, 5, 32)), ((3, 0), (3, 1, 32)), ((0, 5), (1, 1, 1))):
+        x = torch.empty(*rows, 32, device=DEV, dtype=torch.bfloat16)
+        gate = torch.ones(shape, device=DEV, dtype=torch.bfloat16).requires_grad_(True)
+        y, _ = moe_pkg.residual_norm(x, x.clone(), gate=gate)
+        (g,) = torch.autograd.grad(y, gate, torch.empty_like(y))
+        assert g.shape == gate.shape and not g.any()
+    gen = torch.Generator().manual_seed(2)
+    x, u, dy = (torch.randn(4, 6, 40, generator=gen) for _ in range(3))
+    gate = torch.randn(1, 6, 40, generator=gen).to(torch.bfloat16)
+    leaf = gate.to(DEV).requires_grad_(True)
+    y, _ = moe_pkg.residual_norm(x.half().to(DEV), u.to(DEV), gate=leaf)
+    (got,) = torch.autograd.grad(y, leaf, dy.half().to(DEV))
+    terms = dy.half().double() * u.double()
+    want = terms.sum(0, keepdim=True)
+    # four terms of a few float32 roundings, and half a step of bf16: eps / 2 = 2^-8 of the value
+    tol = 68 * 2.0 ** -24 * terms.abs().sum(0, keepdim=True) + torch.finfo(torch.bfloat16).eps / 2 * want.abs()
+    assert got.dtype == torch.bfloat16 and ((got.cpu().double() - want).abs() <= tol).all()
